@@ -1,0 +1,300 @@
+"""The operators of a transformer block's dense half: what is measured, in plain torch and through this package.
+
+Two operators that feed each other:
+
+``norm``     RMS norm of a residual stream, ``h = x + residual`` rounded to the stream's type, ``y = h * rstd * gamma``
+             with ``rstd = 1 / sqrt(mean(h^2) + eps)``; either ``y`` in the stream's type or 8-bit codes with one
+             scale per row. The codes do not depend on rstd (it cancels): ``t = h * gamma``,
+             ``code = round(t * top / max|t|)``, ``scale = max|t| * rstd / top`` with top 127 (s8) or 448 (e4m3).
+``product``  ``y = act((a @ w) * a_scale[row] * w_scale[col] + bias[col]) + residual`` with a and w both bf16, fp16,
+             e4m3 or s8; the scales belong to the 8-bit types. w is a constant, laid out once by the program.
+
+A case is a dict of plain values. ``own`` says which side ``run`` calls: False the plain form (32 bits, 64 at the
+borders between codes), True the package.
+"""
+import math
+
+import torch
+
+own = False
+
+_EPS = 1e-6
+_TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "s8": torch.int8,
+          "e4m3": torch.float8_e4m3fn}
+_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "s8": 1, "e4m3": 1}
+_TOP = {"s8": 127.0, "e4m3": 448.0}
+_ACTS = ("none", "relu", "silu", "gelu", "gelu_tanh")
+
+
+def _norm(name, rows, cols, dtype, out, residual, pad=0):
+    return {"name": name, "op": "norm", "rows": rows, "cols": cols, "dtype": dtype, "out": out, "residual": residual,
+            "pad": pad}
+
+
+def _product(name, m, k, n, dtype, out, layout="nk", bias=False, act="none", residual=False, pad=0):
+    return {"name": name, "op": "product", "m": m, "k": k, "n": n, "dtype": dtype, "out": out, "layout": layout,
+            "bias": bias, "act": act, "residual": residual, "pad": pad}
+
+
+def listed():
+    return [
+        # one token between two layers of a decoder: latency alone counts
+        _norm("norm one token bf16", 1, 4096, "bf16", "bf16", True),
+        # the FP32 stream of the 4096 x 512 int8 product's own configuration, coded for that product
+        _norm("norm 4096x512 f32 to s8", 4096, 512, "f32", "s8", False),
+        # ragged batch, width and row pitch that no vector load fits
+        _norm("norm 777x1001 f16 pitched", 777, 1001, "f16", "f16", True, pad=3),
+        # a prompt's tokens in front of an 8-bit product
+        _norm("norm 8192x4096 bf16 to e4m3", 8192, 4096, "bf16", "e4m3", True),
+        # one token through a square projection back into the stream: the weights' bytes alone count
+        _product("product one token bf16", 1, 4096, 4096, "bf16", "bf16", residual=True),
+        # a decode batch through an up projection in 8 bits
+        _product("product 16 tokens s8", 16, 2048, 8192, "s8", "bf16", act="silu"),
+        # odd in every size, row pitch not a multiple of 16 bytes
+        _product("product odd f16", 333, 1001, 777, "f16", "f16", layout="kn", bias=True, act="relu", residual=True, pad=2),
+        # the sizes of this framework's FP32 MatMul benchmark, 16-bit operands
+        _product("product 2048x512x2048 bf16", 2048, 512, 2048, "bf16", "bf16", layout="kn", bias=True, act="gelu"),
+        # the sizes of this framework's DynamicQuantizeMatMul benchmark, FP32 stream
+        _product("product 4096x512x2048 s8", 4096, 512, 2048, "s8", "f32", layout="kn", bias=True, residual=True),
+        # a prompt through a square projection in 8-bit floats
+        _product("product 4096^3 e4m3", 4096, 4096, 4096, "e4m3", "bf16", residual=True),
+        # a prompt through a down projection into an FP16 stream
+        _product("product 1500x8192x2048 f16", 1500, 8192, 2048, "f16", "f16", bias=True, residual=True),
+        # the largest: a long prompt through an up projection
+        _product("product 8192x4096x16384 bf16", 8192, 4096, 16384, "bf16", "bf16", bias=True, act="gelu_tanh"),
+    ]
+
+
+def _log(rng, lo, hi):
+    """A whole number of [lo, hi], spread over its logarithm; two in three are made a multiple of 16 where they can be."""
+    v = int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+    if v >= 64 and rng.random() < 0.67:
+        v -= v % 16
+    return max(lo, min(hi, v))
+
+
+def draw(rng):
+    if rng.random() < 0.4:
+        rows, cols = _log(rng, 1, 8192), _log(rng, 64, 8192)
+        while rows * cols > 8192 * 4096:
+            rows = max(1, rows // 2)
+        c = _norm("", rows, cols, rng.choice(["f32", "f16", "bf16"]), "", rng.random() < 0.6, rng.choice([0, 0, 0, 8, 5]))
+        c["out"] = rng.choice([c["dtype"], "s8", "e4m3"])
+    else:
+        m, k, n = _log(rng, 1, 8192), _log(rng, 64, 8192), _log(rng, 64, 16384)
+        while m * k * n > 8192 * 4096 * 16384 // 4:
+            m = max(1, m // 2)
+        dtype = rng.choice(["bf16", "f16", "s8", "e4m3"])
+        out = {"bf16": ["bf16"], "f16": ["f16"], "e4m3": ["bf16", "f16"], "s8": ["f32", "bf16", "f16"]}[dtype]
+        c = _product("", m, k, n, dtype, rng.choice(out), rng.choice(["kn", "nk"]), rng.random() < 0.5, rng.choice(_ACTS),
+                     rng.random() < 0.5, rng.choice([0, 0, 0, 16, 3]))
+    del c["name"]
+    return c
+
+
+def _ctx():
+    """The package's context on this device, on torch's stream: one for the program's life."""
+    global _context
+    if _context is None:
+        from onnxsharp_b200.runtime import Context
+
+        _context = Context(0)
+        _context.use_torch_stream()
+    return _context
+
+
+_context = None
+
+
+def _pitched(t, pad):
+    """The same values as rows of a wider buffer."""
+    if not pad:
+        return t
+    wide = torch.zeros((t.shape[0], t.shape[1] + pad), dtype=t.dtype, device=t.device)
+    wide[:, : t.shape[1]] = t
+    return wide[:, : t.shape[1]]
+
+
+def _codes(g, shape, dtype):
+    """What a quantiser hands on: normal rows that fill the 8-bit type's range."""
+    v = torch.randn(shape, generator=g, device="cuda") * (_TOP[dtype] / 4)
+    v = v.clamp(-_TOP[dtype], _TOP[dtype])
+    return v.round().to(torch.int8) if dtype == "s8" else v.to(torch.float8_e4m3fn)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    randn = lambda *shape: torch.randn(shape, generator=g, device="cuda")  # noqa: E731
+    rand = lambda *shape: torch.rand(shape, generator=g, device="cuda")  # noqa: E731
+    s = {"case": case}
+    if case["op"] == "norm":
+        rows, cols, dtype = case["rows"], case["cols"], _TYPES[case["dtype"]]
+        channel = torch.exp(0.5 * randn(cols))  # some channels of a stream are much larger than others
+        s["x"] = _pitched((randn(rows, cols) * channel).to(dtype), case["pad"])
+        s["gamma"] = (1.0 + 0.2 * randn(cols)).to(dtype)
+        s["residual"] = _pitched((randn(rows, cols) * channel).to(dtype), case["pad"]) if case["residual"] else None
+        s["sum"] = torch.empty((rows, cols), dtype=dtype, device="cuda") if case["residual"] else None
+        s["y"] = torch.empty((rows, cols), dtype=_TYPES[case["out"]], device="cuda")
+        s["scales"] = torch.empty(rows, device="cuda") if case["out"] in _TOP else None
+        return s
+    m, k, n, dtype = case["m"], case["k"], case["n"], case["dtype"]
+    shape = (n, k) if case["layout"] == "nk" else (k, n)
+    s["a_scale"] = s["w_scale"] = None
+    if dtype in _TOP:
+        a, s["w"] = _codes(g, (m, k), dtype), _codes(g, shape, dtype)
+        s["a_scale"] = (0.5 + rand(m)) * (4 / _TOP[dtype])
+        s["w_scale"] = (0.5 + rand(n)) * (4 / _TOP[dtype] / math.sqrt(k))
+    else:
+        a, s["w"] = randn(m, k).to(_TYPES[dtype]), (randn(*shape) / math.sqrt(k)).to(_TYPES[dtype])
+    s["a"] = _pitched(a, case["pad"])
+    s["bias"] = 0.1 * randn(n) if case["bias"] else None
+    s["residual"] = randn(m, n).to(_TYPES[case["out"]]) if case["residual"] else None
+    s["y"] = torch.empty((m, n), dtype=_TYPES[case["out"]], device="cuda")
+    if own:
+        from onnxsharp_b200.runtime import LinearWeights
+
+        s["weights"] = LinearWeights(_ctx(), s["w"], layout=1 if case["layout"] == "nk" else 0)
+    return s
+
+
+def run(state):
+    case = state["case"]
+    if case["op"] == "norm":
+        return _run_norm(state, case)
+    return _run_product(state, case)
+
+
+def _run_norm(s, case):
+    coded = case["out"] in _TOP
+    if own:
+        from onnxsharp_b200 import ops
+
+        if coded:
+            ops.rmsnorm_quant(_ctx(), s["x"], s["gamma"], _EPS, s["y"], s["scales"], residual=s["residual"], sum_out=s["sum"])
+        else:
+            ops.rmsnorm(_ctx(), s["x"], s["gamma"], _EPS, s["y"], residual=s["residual"], sum_out=s["sum"])
+        y, h, scales = s["y"], s["sum"], s["scales"]
+    else:
+        h = s["x"] if s["residual"] is None else (s["x"].float() + s["residual"].float()).to(s["x"].dtype)
+        v = h.float()
+        rstd = torch.rsqrt((v * v).mean(dim=1) + _EPS)
+        scales = None
+        if coded:
+            top = _TOP[case["out"]]
+            t = h.double() * s["gamma"].double()  # 64 bits: a code's border is hit exactly or not at all
+            peak = t.abs().amax(dim=1)
+            some = peak > 0
+            ratio = t * top / torch.where(some, peak, 1.0)[:, None]
+            if case["out"] == "s8":
+                y = ratio.round().to(torch.int8)
+            else:  # 3 bits after the leading one, steps of 2^-9 below 2^-6
+                step = torch.exp2(torch.frexp(ratio).exponent.clamp(min=-5).double() - 4)
+                y = ((ratio / step).round() * step).to(torch.float8_e4m3fn)
+            scales = torch.where(some, peak * rstd.double() / top, 1.0).float()
+        else:
+            y = (v * rstd[:, None] * s["gamma"].float()).to(h.dtype)
+        h = h if s["residual"] is not None else None
+    if coded:  # the codes are compared as the values that they stand for
+        codes = y if case["out"] == "s8" else y.to(torch.bfloat16)
+        y = torch.mul(codes, scales[:, None], out=torch.empty(codes.shape, dtype=s["x"].dtype, device="cuda"))
+    return {"y": y, "h": h, "scales": scales}
+
+
+def _act(v, act):
+    if act == "relu":
+        return v.clamp(min=0)
+    if act == "silu":
+        return v / (1 + torch.exp(-v))
+    if act == "gelu":
+        return 0.5 * v * (1 + torch.erf(v * (1 / math.sqrt(2))))
+    if act == "gelu_tanh":
+        return 0.5 * v * (1 + torch.tanh(math.sqrt(2 / math.pi) * (v + 0.044715 * v * v * v)))
+    return v
+
+
+def _run_product(s, case):
+    if own:
+        from onnxsharp_b200 import _lib
+        from onnxsharp_b200.runtime import linear
+
+        act = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU,
+               "gelu_tanh": _lib.ACT_GELU_TANH}[case["act"]]
+        return linear(_ctx(), s["a"], s["weights"], bias=s["bias"], act=act, residual=s["residual"], a_scale=s["a_scale"],
+                      w_scale=s["w_scale"], out=s["y"])
+    w = s["w"].float()
+    v = s["a"].float() @ (w.t() if case["layout"] == "nk" else w)
+    if s["a_scale"] is not None:
+        v = v * s["a_scale"][:, None] * s["w_scale"]
+    if s["bias"] is not None:
+        v = v + s["bias"]
+    v = _act(v, case["act"])
+    if s["residual"] is not None:
+        v = v + s["residual"].float()
+    return v.to(_TYPES[case["out"]])
+
+
+def work(case):
+    if case["op"] == "norm":
+        n, e = case["rows"] * case["cols"], _SIZE[case["dtype"]]
+        read = n * e * (2 if case["residual"] else 1) + case["cols"] * e
+        # codes go back to values for the comparison: those values are the pass's output
+        wrote = n * e * (1 if case["residual"] else 0) + n * (e if case["out"] in _TOP else _SIZE[case["out"]])
+        return {"bytes": read + wrote + (4 * case["rows"] if case["out"] in _TOP else 0), "flops": 4 * n}
+    m, k, n = case["m"], case["k"], case["n"]
+    e, o = _SIZE[case["dtype"]], _SIZE[case["out"]]
+    small = (4 * n if case["bias"] else 0) + (4 * (m + n) if case["dtype"] in _TOP else 0)
+    return {"bytes": (m * k + k * n) * e + m * n * o * (2 if case["residual"] else 1) + small, "flops": 2 * m * k * n}
+
+
+def exact(case, seed):
+    """run()'s outputs from the definition in 64 bits: row blocks of the product, the norm's sums and roots in double."""
+    s = prepare(case, seed)
+    if case["op"] == "norm":
+        x = s["x"].to(torch.float64)
+        h = None
+        if case["residual"]:
+            h = (x + s["residual"].to(torch.float64)).to(torch.float32).to(s["x"].dtype)  # the stream as it is kept
+            x = h.to(torch.float64)
+        inverse = 1.0 / torch.sqrt(x.pow(2).sum(dim=1, keepdim=True) / case["cols"] + _EPS)
+        weighed = torch.einsum("rc,c->rc", x, s["gamma"].to(torch.float64))
+        if case["out"] not in _TOP:
+            return {"y": weighed * inverse, "h": h, "scales": None}
+        top = _TOP[case["out"]]
+        peak = weighed.abs().max(dim=1, keepdim=True).values
+        part = weighed * top / torch.where(peak > 0, peak, torch.ones_like(peak))
+        if case["out"] == "s8":
+            code = torch.floor(part)
+            rest = part - code
+            up = (rest > 0.5) | ((rest == 0.5) & (torch.remainder(code, 2) == 1))
+            code = code + up.to(torch.float64)
+        else:
+            grid = torch.arange(0, 127, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn).to(torch.float64)
+            middle = (grid[:-1] + grid[1:]) / 2  # between neighbours; on one, the even code wins
+            low, high = torch.bucketize(part.abs(), middle), torch.bucketize(part.abs(), middle, right=True)
+            code = grid[torch.where(low % 2 == 0, low, high)] * torch.sign(part)
+        scale = torch.where(peak > 0, peak * inverse / top, torch.ones_like(peak))
+        return {"y": code * scale, "h": h, "scales": scale[:, 0]}
+    if case["m"] * case["k"] * case["n"] > 8192 * 4096 * 16384:
+        return None
+    w = s["w"].to(torch.float64)
+    w = w.T if case["layout"] == "nk" else w
+    blocks = []
+    for i in range(0, case["m"], 2048):
+        v = torch.mm(s["a"][i : i + 2048].to(torch.float64), w)
+        if s["a_scale"] is not None:
+            v = v * torch.outer(s["a_scale"][i : i + 2048].to(torch.float64), s["w_scale"].to(torch.float64))
+        if s["bias"] is not None:
+            v = v + s["bias"].to(torch.float64)
+        if case["act"] == "relu":
+            v = torch.where(v > 0, v, torch.zeros_like(v))
+        elif case["act"] == "silu":
+            v = v * torch.sigmoid(v)
+        elif case["act"] == "gelu":
+            v = v * torch.special.ndtr(v)
+        elif case["act"] == "gelu_tanh":
+            v = v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v.pow(3)))
+        if s["residual"] is not None:
+            v = v + s["residual"][i : i + 2048].to(torch.float64)
+        blocks.append(v)
+    return torch.cat(blocks)
