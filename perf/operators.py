@@ -1,6 +1,6 @@
-"""The operators of a transformer block's dense half: what is measured, in plain torch and through this package.
+"""The operators of a transformer block: what is measured, in plain torch and through this package.
 
-Two operators that feed each other:
+Three operators that feed one another:
 
 ``norm``     RMS norm of a residual stream, ``h = x + residual`` rounded to the stream's type, ``y = h * rstd * gamma``
              with ``rstd = 1 / sqrt(mean(h^2) + eps)``; either ``y`` in the stream's type or 8-bit codes with one
@@ -8,6 +8,11 @@ Two operators that feed each other:
              ``code = round(t * top / max|t|)``, ``scale = max|t| * rstd / top`` with top 127 (s8) or 448 (e4m3).
 ``product``  ``y = act((a @ w) * a_scale[row] * w_scale[col] + bias[col]) + residual`` with a and w both bf16, fp16,
              e4m3 or s8; the scales belong to the 8-bit types. w is a constant, laid out once by the program.
+``window``   causal attention over a cache with a sliding window and a few first tokens that stay visible: the query at
+             position p sees the keys j <= p with j > p - window or j < sinks. q is [B, T, heads, D], the cache
+             [B, S, kv heads, D] with lengths[b] tokens written; what lies behind them is never looked at (here: NaN).
+             Query t of sequence b stands at lengths[b] - T + t, or at t ("padded" batches); a row that stands
+             outside 0 .. lengths[b] - 1 is padding and comes out as zeros.
 
 A case is a dict of plain values. ``own`` says which side ``run`` calls: False the plain form (32 bits, 64 at the
 borders between codes), True the package.
@@ -36,6 +41,11 @@ def _product(name, m, k, n, dtype, out, layout="nk", bias=False, act="none", res
             "bias": bias, "act": act, "residual": residual, "pad": pad}
 
 
+def _window(name, batch, tokens, size, heads, kv_heads, dim, dtype, window, sinks, padded=False):
+    return {"name": name, "op": "window", "batch": batch, "tokens": tokens, "size": size, "heads": heads,
+            "kv_heads": kv_heads, "dim": dim, "dtype": dtype, "window": window, "sinks": sinks, "padded": padded}
+
+
 def listed():
     return [
         # one token between two layers of a decoder: latency alone counts
@@ -48,20 +58,20 @@ def listed():
         _norm("norm 8192x4096 bf16 to e4m3", 8192, 4096, "bf16", "e4m3", True),
         # one token through a square projection back into the stream: the weights' bytes alone count
         _product("product one token bf16", 1, 4096, 4096, "bf16", "bf16", residual=True),
-        # a decode batch through an up projection in 8 bits
-        _product("product 16 tokens s8", 16, 2048, 8192, "s8", "bf16", act="silu"),
+        # a decode batch through an up projection in 8-bit floats
+        _product("product 16 tokens e4m3", 16, 2048, 8192, "e4m3", "bf16", act="silu"),
         # odd in every size, row pitch not a multiple of 16 bytes
         _product("product odd f16", 333, 1001, 777, "f16", "f16", layout="kn", bias=True, act="relu", residual=True, pad=2),
-        # the sizes of this framework's FP32 MatMul benchmark, 16-bit operands
-        _product("product 2048x512x2048 bf16", 2048, 512, 2048, "bf16", "bf16", layout="kn", bias=True, act="gelu"),
         # the sizes of this framework's DynamicQuantizeMatMul benchmark, FP32 stream
         _product("product 4096x512x2048 s8", 4096, 512, 2048, "s8", "f32", layout="kn", bias=True, residual=True),
-        # a prompt through a square projection in 8-bit floats
-        _product("product 4096^3 e4m3", 4096, 4096, 4096, "e4m3", "bf16", residual=True),
-        # a prompt through a down projection into an FP16 stream
-        _product("product 1500x8192x2048 f16", 1500, 8192, 2048, "f16", "f16", bias=True, residual=True),
         # the largest: a long prompt through an up projection
         _product("product 8192x4096x16384 bf16", 8192, 4096, 16384, "bf16", "bf16", bias=True, act="gelu_tanh"),
+        # a decode batch over ragged caches longer than the window: the keys' and values' bytes count
+        _window("window 16 sequences one token", 16, 1, 8192, 32, 8, 128, "bf16", 4096, 4),
+        # two prompts several windows long
+        _window("window prompts 2x4096", 2, 4096, 4096, 16, 4, 128, "bf16", 1024, 16),
+        # a padded ragged batch in this framework's own head size, window shorter than a tile
+        _window("window 3x333 padded f16", 3, 333, 333, 6, 2, 64, "f16", 100, 3, padded=True),
     ]
 
 
@@ -74,12 +84,23 @@ def _log(rng, lo, hi):
 
 
 def draw(rng):
-    if rng.random() < 0.4:
+    op = rng.random()
+    if op < 0.3:
         rows, cols = _log(rng, 1, 8192), _log(rng, 64, 8192)
         while rows * cols > 8192 * 4096:
             rows = max(1, rows // 2)
         c = _norm("", rows, cols, rng.choice(["f32", "f16", "bf16"]), "", rng.random() < 0.6, rng.choice([0, 0, 0, 8, 5]))
         c["out"] = rng.choice([c["dtype"], "s8", "e4m3"])
+    elif op < 0.6:
+        heads, kv_heads = rng.choice([(8, 8), (8, 2), (16, 4), (12, 1), (32, 8), (5, 5)])
+        tokens = _log(rng, 1, 12) if rng.random() < 0.5 else _log(rng, 16, 4096)
+        batch, size = _log(rng, 1, 16), _log(rng, max(tokens, 64), 8192)
+        while batch > 1 and batch * heads * tokens * size > 2 * 16 * 4096 * 4096:
+            batch = max(1, batch // 2)
+        while heads * tokens * size > 2 * 16 * 4096 * 4096:
+            size = max(tokens, size // 2)
+        c = _window("", batch, tokens, size, heads, kv_heads, rng.choice([64, 128]), rng.choice(["f16", "bf16"]),
+                    _log(rng, 1, 2 * size), rng.choice([0, 1, 4, 16, 200]), tokens == size)
     else:
         m, k, n = _log(rng, 1, 8192), _log(rng, 64, 8192), _log(rng, 64, 16384)
         while m * k * n > 8192 * 4096 * 16384 // 4:
@@ -122,6 +143,11 @@ def _codes(g, shape, dtype):
     return v.round().to(torch.int8) if dtype == "s8" else v.to(torch.float8_e4m3fn)
 
 
+def _lengths(case):
+    """Tokens of each sequence: ragged, the first as long as the cache; some are shorter than the queries are many."""
+    return [max(1, case["size"] - b * case["size"] // case["batch"]) for b in range(case["batch"])]
+
+
 def prepare(case, seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -137,6 +163,16 @@ def prepare(case, seed):
         s["sum"] = torch.empty((rows, cols), dtype=dtype, device="cuda") if case["residual"] else None
         s["y"] = torch.empty((rows, cols), dtype=_TYPES[case["out"]], device="cuda")
         s["scales"] = torch.empty(rows, device="cuda") if case["out"] in _TOP else None
+        return s
+    if case["op"] == "window":
+        b, t, size, h, hk, d = (case[x] for x in ("batch", "tokens", "size", "heads", "kv_heads", "dim"))
+        dtype = _TYPES[case["dtype"]]
+        s["lengths"] = torch.tensor(_lengths(case), dtype=torch.int32, device="cuda")
+        s["starts"] = torch.zeros(b, dtype=torch.int32, device="cuda") if case["padded"] else None
+        s["q"] = randn(b, t, h, d).to(dtype)
+        unwritten = (torch.arange(size, device="cuda") >= s["lengths"][:, None])[:, :, None, None]
+        s["k"], s["v"] = (torch.where(unwritten, math.nan, randn(b, size, hk, d)).to(dtype) for _ in range(2))
+        s["y"] = torch.empty((b, t, h, d), dtype=dtype, device="cuda")
         return s
     m, k, n, dtype = case["m"], case["k"], case["n"], case["dtype"]
     shape = (n, k) if case["layout"] == "nk" else (k, n)
@@ -162,6 +198,8 @@ def run(state):
     case = state["case"]
     if case["op"] == "norm":
         return _run_norm(state, case)
+    if case["op"] == "window":
+        return _run_window(state, case)
     return _run_product(state, case)
 
 
@@ -199,6 +237,36 @@ def _run_norm(s, case):
         codes = y if case["out"] == "s8" else y.to(torch.bfloat16)
         y = torch.mul(codes, scales[:, None], out=torch.empty(codes.shape, dtype=s["x"].dtype, device="cuda"))
     return {"y": y, "h": h, "scales": scales}
+
+
+def _visible(s, case):
+    """[B, T, S]: which keys each query sees."""
+    first = s["starts"] if s["starts"] is not None else s["lengths"] - case["tokens"]
+    p = (first[:, None] + torch.arange(case["tokens"], device="cuda"))[:, :, None]
+    j = torch.arange(case["size"], device="cuda")
+    live = (p >= 0) & (p < s["lengths"][:, None, None])
+    return live & (j <= p) & ((j > p - case["window"]) | (j < case["sinks"]))
+
+
+def _run_window(s, case):
+    scale = case["dim"] ** -0.5
+    if own:
+        from onnxsharp_b200.runtime import attention_window
+
+        return attention_window(_ctx(), s["q"], s["k"], s["v"], s["lengths"], scale, window=case["window"],
+                                sinks=case["sinks"], starts=s["starts"], out=s["y"])
+    b, t, size, h, hk, d = (case[x] for x in ("batch", "tokens", "size", "heads", "kv_heads", "dim"))
+    seen = _visible(s, case)[:, None]
+    written = (torch.arange(size, device="cuda") < s["lengths"][:, None])[:, None, :, None]
+    q = s["q"].float().view(b, t, hk, h // hk, d).permute(0, 2, 3, 1, 4).reshape(b, hk, (h // hk) * t, d)
+    k = s["k"].float().permute(0, 2, 3, 1)
+    v = torch.where(written, s["v"].float().permute(0, 2, 1, 3), 0.0)
+    scores = torch.where(seen[:, :, None], (q @ k).view(b, hk, h // hk, t, size) * scale, -math.inf)
+    top = scores.amax(dim=-1, keepdim=True).clamp(min=torch.finfo(torch.float32).min)
+    e = torch.exp(scores - top)
+    total = e.sum(dim=-1, keepdim=True)
+    y = (e.view(b, hk, (h // hk) * t, size) @ v).view(b, hk, h // hk, t, d) / torch.where(total > 0, total, 1.0)
+    return y.permute(0, 3, 1, 2, 4).reshape(b, t, h, d).to(s["q"].dtype)
 
 
 def _act(v, act):
@@ -241,6 +309,19 @@ def work(case):
         # codes go back to values for the comparison: those values are the pass's output
         wrote = n * e * (1 if case["residual"] else 0) + n * (e if case["out"] in _TOP else _SIZE[case["out"]])
         return {"bytes": read + wrote + (4 * case["rows"] if case["out"] in _TOP else 0), "flops": 4 * n}
+    if case["op"] == "window":
+        t, w, sinks, pairs, keys = case["tokens"], case["window"], case["sinks"], 0, 0
+        for length in _lengths(case):
+            first = 0 if case["padded"] else length - t
+            low, high = max(0, first), min(length, first + t)  # positions of the rows that are not padding
+            for p in range(low, high):
+                pairs += min(p + 1, w + min(sinks, max(0, p + 1 - w)))
+            if high > low:
+                edge = max(0, low - w + 1)
+                keys += high - edge + min(sinks, edge)
+        e, d = _SIZE[case["dtype"]], case["dim"]
+        tokens = case["batch"] * t * case["heads"] * d
+        return {"bytes": 2 * tokens * e + 2 * keys * case["kv_heads"] * d * e, "flops": 4 * pairs * d * case["heads"]}
     m, k, n = case["m"], case["k"], case["n"]
     e, o = _SIZE[case["dtype"]], _SIZE[case["out"]]
     small = (4 * n if case["bias"] else 0) + (4 * (m + n) if case["dtype"] in _TOP else 0)
@@ -275,6 +356,22 @@ def exact(case, seed):
             code = grid[torch.where(low % 2 == 0, low, high)] * torch.sign(part)
         scale = torch.where(peak > 0, peak * inverse / top, torch.ones_like(peak))
         return {"y": code * scale, "h": h, "scales": scale[:, 0]}
+    if case["op"] == "window":
+        y = torch.zeros(s["q"].shape, dtype=torch.float64, device="cuda")
+        group = case["heads"] // case["kv_heads"]
+        for b, length in enumerate(_lengths(case)):
+            first = 0 if case["padded"] else length - case["tokens"]
+            rows = [t for t in range(case["tokens"]) if 0 <= first + t < length]
+            if not rows:
+                continue
+            at = torch.arange(first + rows[0], first + rows[-1] + 1, device="cuda")[:, None]
+            key = torch.arange(length, device="cuda")[None]
+            hidden = (key > at) | ((at - key >= case["window"]) & (key >= case["sinks"]))
+            for h in range(case["heads"]):
+                dots = torch.mm(s["q"][b, rows[0] : rows[-1] + 1, h].double(), s["k"][b, :length, h // group].double().T)
+                weights = torch.softmax((dots / math.sqrt(case["dim"])).masked_fill(hidden, -math.inf), dim=1)
+                y[b, rows[0] : rows[-1] + 1, h] = torch.mm(weights, s["v"][b, :length, h // group].double())
+        return y
     if case["m"] * case["k"] * case["n"] > 8192 * 4096 * 16384:
         return None
     w = s["w"].to(torch.float64)
