@@ -62,7 +62,13 @@ enum osc_status {
  * instead of the reference's VectorMath restated bit for bit. The tensor-core
  * conv entries always compute the fast form (their sums are not bit-identical
  * to the reference's anyway); the other entries accept the plain codes. */
-enum osc_act { OSC_ACT_NONE = 0, OSC_ACT_SILU = 1, OSC_ACT_RELU = 2, OSC_ACT_SIGMOID = 3, OSC_ACT_FAST = 16 };
+enum osc_act { OSC_ACT_NONE = 0, OSC_ACT_SILU = 1, OSC_ACT_RELU = 2, OSC_ACT_SIGMOID = 3,
+               OSC_ACT_GELU = 4,       /* v * Phi(v); osc_linear only */
+               OSC_ACT_GELU_TANH = 5,  /* its tanh form; osc_linear only */
+               OSC_ACT_FAST = 16 };
+
+/* Element types of the entries that take more than FP32 (osc_rmsnorm, osc_linear). */
+enum osc_dtype { OSC_F32 = 0, OSC_F16 = 1, OSC_BF16 = 2, OSC_S8 = 3, OSC_E4M3 = 4 };
 
 typedef struct osc_ctx osc_ctx;
 typedef struct osc_gemm_weights osc_gemm_weights;
@@ -352,6 +358,39 @@ OSC_API int osc_dqmm_shard_f32(osc_ctx* ctx, const float* a, int m, int k, int l
  * skipped (Quantizer.MinMax). */
 OSC_API int osc_minmax_f32(osc_ctx* ctx, const float* x, long count, float* minmax_out);
 
+/* ------------------------------------------------------------ product with epilogue (16 and 8 bits)
+ * No counterpart in the reference (its MatMul is FP32 and its fused residual
+ * belongs to Conv): the products of a transformer block.
+ *
+ *   y[i, j] = round(act((sum_t a[i, t] * w[t, j]) * a_scale[i] * w_scale[j] + bias[j]) + residual[i, j])
+ *
+ * a [m, k] and w have one type: OSC_F16, OSC_BF16, OSC_E4M3 (FP32 sums on the
+ * tensor cores) or OSC_S8 (exact S32 sums). Everything after the sum is FP32,
+ * rounded once to y.
+ *
+ * osc_linear_prepack lays the constant w out once (layout 0: [k, n] row-major,
+ * ONNX MatMul; 1: [n, k], ONNX Gemm transB=1; `w` is a device pointer, or a
+ * host pointer with host != 0) and returns after the copy is complete. Not
+ * during stream capture. OSC_S8: k < 131072. The weights must outlive every
+ * call and captured graph that uses them. */
+typedef struct osc_linear_weights osc_linear_weights;
+OSC_API int osc_linear_prepack(osc_ctx* ctx, int dtype, const void* w, int k, int n, int layout, int host,
+                               osc_linear_weights** out);
+OSC_API int osc_linear_weights_free(osc_linear_weights* w);
+
+/* m >= 0 (0: nothing is done). lda, ldr, ldy: row pitches in elements (0 =
+ * dense), of any alignment; rows that are 16-byte aligned travel by TMA. The
+ * scales (8-bit types only) and the bias are FP32 and may be NULL: a_scale [m]
+ * (what osc_rmsnorm writes), w_scale n_scale entries (1 or n), bias [n].
+ * out_dtype: OSC_F32, OSC_F16 or OSC_BF16, also the residual's type. act: any
+ * osc_act up to OSC_ACT_GELU_TANH. residual may be NULL, and may be y itself
+ * (same pointer and pitch); no other argument may overlap y. Uses no scratch
+ * memory, so calls on different streams or in different graphs share nothing
+ * but the weights. */
+OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const osc_linear_weights* w,
+                       const float* a_scale, const float* w_scale, int n_scale, const float* bias, int act,
+                       const void* residual, long long ldr, int out_dtype, void* y, long long ldy);
+
 /* ------------------------------------------------------------ FusedAttention
  * Replaces AttentionLayer.Forward (src/OnnxSharp/Ops/AttentionOps.cs:249-351),
  * heads form: q, k, v are [B, T, H*D] (the fused node's inputs
@@ -426,6 +465,28 @@ OSC_API int osc_yolo_decode_f32(osc_ctx* ctx, int B, int nc, const float* const*
  * gamma / beta may be NULL. */
 OSC_API int osc_layernorm_f32(osc_ctx* ctx, const float* x, int outer, int inner, const float* gamma,
                               const float* beta, float eps, float* y);
+
+/* RMS norm of a residual stream (no counterpart in the reference; beside
+ * LayerNormalization). x, residual, sum, gamma and y have one type T = dtype
+ * (OSC_F32, OSC_F16 or OSC_BF16):
+ *
+ *   h = round(x + residual) (h = x without a residual), written to sum when given
+ *   rstd = 1 / sqrt(mean(h^2) + eps), FP32 sums;  y = round(h * rstd * gamma)
+ *   t = h * gamma, top = 127 (OSC_S8) or 448 (OSC_E4M3):
+ *   q = round_to_even(t * top / max|t|),  scales[row] = max|t| * rstd / top
+ *
+ * so that q * scale stands for y. Either y or q (with scales) may be NULL,
+ * gamma too (ones); sum needs a residual. The *_ld are row pitches in elements
+ * (0 = dense), of any alignment. sum may be x's or residual's own buffer (same
+ * pointer and pitch), and so may y where sum is not that buffer; nothing else may
+ * overlap. eps >= 1e-30. A row whose max|t| is below 2^-80 gets codes 0 and
+ * scale 1; one whose max|t| is not finite in FP32 gets codes 0 and scale NaN
+ * (its y is what the formula gives). q goes with scales as a and a_scale into
+ * osc_linear. No scratch memory. */
+OSC_API int osc_rmsnorm(osc_ctx* ctx, int dtype, const void* x, long long x_ld, const void* residual,
+                        long long res_ld, long long rows, int cols, const void* gamma, float eps, void* sum,
+                        long long sum_ld, void* y, long long y_ld, int q_dtype, void* q, long long q_ld,
+                        float* scales);
 
 /* Attention of YOLO11's PSA block (sequence T = H*W, not limited to 128):
  * qkv [B, heads*(2*kd + hd), T] -> out [B, heads*hd, T] with

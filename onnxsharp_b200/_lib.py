@@ -30,7 +30,21 @@ STATUS_NAMES = {
 
 # activation codes (enum osc_act)
 ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID = 0, 1, 2, 3
+ACT_GELU, ACT_GELU_TANH = 4, 5  # osc_linear only
 ACT_FAST = 16  # OR into conv2d_direct's activation: hardware ex2/rcp Sigmoid/SiLU
+
+# element types (enum osc_dtype)
+F32, F16, BF16, S8, E4M3 = 0, 1, 2, 3, 4
+_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": S8,
+           "torch.float8_e4m3fn": E4M3}
+
+
+def dtype_code(dtype) -> int:
+    """enum osc_dtype of a torch dtype."""
+    try:
+        return _DTYPES[str(dtype)]
+    except KeyError:
+        raise TypeError(f"{dtype} is not float32, float16, bfloat16, int8 or float8_e4m3fn") from None
 
 
 class OscError(RuntimeError):
@@ -119,6 +133,10 @@ SIGNATURES: dict[str, tuple] = {
     "osc_dqmm_f32": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp]),
     "osc_dqmm_shard_f32": (i32, [vp, vp, i32, i32, i32, vp, vp, i32, vp, vp, vp, i32, i32, vp, vp, vp]),
     "osc_minmax_f32": (i32, [vp, vp, C.c_long, vp]),
+    # product with epilogue (16 and 8 bits)
+    "osc_linear_prepack": (i32, [vp, i32, vp, i32, i32, i32, i32, pp]),
+    "osc_linear_weights_free": (i32, [vp]),
+    "osc_linear": (i32, [vp, vp, i32, i64, vp, vp, vp, i32, vp, i32, vp, i64, i32, vp, i64]),
     # FusedAttention
     "osc_attention_f32": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp]),
     # graph glue
@@ -134,6 +152,7 @@ SIGNATURES: dict[str, tuple] = {
     "osc_dfl_f32": (i32, [vp, vp, i32, i32, i32, i32, vp]),
     "osc_yolo_decode_f32": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "osc_layernorm_f32": (i32, [vp, vp, i32, i32, vp, vp, f32, vp]),
+    "osc_rmsnorm": (i32, [vp, i32, vp, i64, vp, i64, i64, i32, vp, f32, vp, i64, vp, i64, i32, vp, i64, vp]),
     "osc_psa_attention_f32": (i32, [vp, vp, i64, i32, i32, i32, i32, i32, f32, vp, i64]),
 }
 

@@ -1,0 +1,1039 @@
+// linear.cu — the matrix product of a transformer block with everything around
+// it in its epilogue, on the sm_100a tensor cores:
+//
+//   y[i, j] = round(act((sum_t a[i, t] * w[t, j]) * a_scale[i] * w_scale[j] + bias[j]) + residual[i, j])
+//
+// for bf16, fp16 (kind::f16), e4m3 (kind::f8f6f4, FP32 sums) and s8 (kind::i8,
+// exact S32 sums) operands; everything after the sum is FP32 and rounded once.
+// It stands beside the FP32 MatMul (gemm_tf32x3.cu) and the per-tensor u8
+// DynamicQuantizeMatMul (dqmm_i8.cu) of the reference's operators
+// (src/OnnxSharp/Ops/DnnOps.cs:2789-3102, Ops/QuantizedMatMulOps.cs:115-201);
+// the reference has no 16-bit product and no residual in a product.
+//
+// Orientation. The weights are the MMA's 128-row operand and the tokens its N
+// side, so a TMEM lane is an output column: the epilogue thread keeps that
+// column's scale and bias in registers, and a warp's residual loads and output
+// stores of one token are 32 consecutive elements whatever the row pitch or
+// alignment of y is. The token side of a tile can be any multiple of 16, which
+// is what fits ragged batches and evens out the last wave.
+//
+// Weights are laid out once as blocks of 128 columns x 128 bytes of K, each
+// 16 KB contiguous: one TMA box reads one block as one run of DRAM pages, and
+// K tails and ragged last columns are zeros of the copy.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "runtime.h"
+#include "sm100.cuh"
+#include "vmath.cuh"
+
+struct osc_linear_weights {
+  int device = 0;
+  int dtype = 0;
+  int k = 0, n = 0;
+  int num_kb = 0, tiles = 0;  // blocks of 128 bytes of K, blocks of 128 columns
+  uint8_t* blocks = nullptr;  // [tiles][num_kb][128][128]
+  CUtensorMap map;            // the blocks as rows of 128 bytes, 128 of them a box
+};
+
+namespace osc {
+namespace {
+
+enum : int { LIN_F16 = 0, LIN_F8 = 1, LIN_I8 = 2 };  // MMA kinds
+
+constexpr int kCols = 128;               // output columns of a CTA
+constexpr int kKB = 128;                 // bytes of K in a block: one swizzle row
+constexpr int kWBytes = kCols * kKB;     // 16 KB
+constexpr int kMaxStages = 8;
+constexpr int kEpiWarps = 8;
+constexpr int kLoadWarps = 4;            // rows of A that no TMA box fits
+constexpr int kSmemTail = 512;           // barriers
+constexpr int kSmemOne = 232448 - 1024;  // one CTA per SM: the ring and the tail
+constexpr int kSmemTwo = 115712 - 1024;  // two CTAs per SM
+constexpr int kMaxSplit = 8;             // portable cluster size
+
+struct LinArgs {
+  int M, N, num_kb, last_steps;  // last_steps: 32-byte K steps of the last block
+  int bn;                        // tokens of a tile
+  int stages, stage_bytes;
+  int tiles_m, tiles_n;          // token tiles, column tiles (of 256 for a CTA pair)
+  int split;                     // CTAs that share a tile's K
+  uint32_t idesc;
+  const float* a_scale;
+  const float* w_scale;
+  int w_scale_n;
+  const float* bias;
+  int act;
+  int out;                       // osc_dtype of y and the residual
+  const void* residual;
+  long long ldr;
+  void* y;
+  long long ldy;
+  const uint8_t* a;              // for rows that no TMA box fits
+  long long lda_bytes;
+  int k_bytes;
+};
+
+struct LinBars {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t exit_bar;
+  uint32_t tmem_slot;
+  int abort_flag;
+  int no_abort;
+};
+static_assert(sizeof(LinBars) <= kSmemTail, "barriers fit the tail");
+
+template <int KIND>
+__device__ __forceinline__ void mma_one(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  if constexpr (KIND == LIN_F16) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  } else if constexpr (KIND == LIN_F8) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  } else {
+    mma_i8(d, da, db, idesc, acc);
+  }
+}
+
+template <int KIND>
+__device__ __forceinline__ void mma_two(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  if constexpr (KIND == LIN_F16) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  } else if constexpr (KIND == LIN_F8) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ epilogue
+// An accumulator word as the FP32 sum (S32 sums are rounded once, to FP32).
+template <int KIND>
+__device__ __forceinline__ float sum_of(uint32_t r) {
+  return KIND == LIN_I8 ? static_cast<float>(static_cast<int32_t>(r)) : __uint_as_float(r);
+}
+
+// SiLU and tanh-GELU come from the hardware ex2 / rcp instructions (relative
+// error under 1e-6 where the sigmoid is not saturated, see fast_sigmoid), two
+// orders below the rounding of a 16-bit output and below an FP32 product's own.
+template <int NV>
+__device__ __forceinline__ void activate(float (&v)[NV], int act) {
+  switch (act) {
+    case OSC_ACT_SILU:
+#pragma unroll
+      for (int t = 0; t < NV; ++t) v[t] = act_fast<ACT_SILU>(v[t]);
+      break;
+    case OSC_ACT_RELU:
+#pragma unroll
+      for (int t = 0; t < NV; ++t) v[t] = v[t] < 0.0f ? 0.0f : v[t];  // keeps a NaN
+      break;
+    case OSC_ACT_SIGMOID:
+#pragma unroll
+      for (int t = 0; t < NV; ++t) v[t] = fast_sigmoid(v[t]);
+      break;
+    case OSC_ACT_GELU:  // v * Phi(v)
+#pragma unroll
+      for (int t = 0; t < NV; ++t) v[t] = 0.5f * v[t] * (1.0f + erff(v[t] * 0.70710678118654752f));
+      break;
+    case OSC_ACT_GELU_TANH:  // 0.5 * (1 + tanh(u)) = sigmoid(2u), u = sqrt(2/pi) (v + 0.044715 v^3)
+#pragma unroll
+      for (int t = 0; t < NV; ++t)
+        v[t] *= fast_sigmoid(1.5957691216057308f * (v[t] + 0.044715f * v[t] * v[t] * v[t]));
+      break;
+    default: break;
+  }
+}
+
+// The residual's raw words of tokens i0 .. i0 + NV - 1 (those below M) at column j.
+template <int NV>
+__device__ __forceinline__ void load_residual(const LinArgs& p, int i0, int step, int i_end, int j, uint32_t (&r)[NV]) {
+  if (p.out == OSC_F32) {
+    const uint32_t* src = static_cast<const uint32_t*>(p.residual) + j;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      r[t] = i < i_end ? src[static_cast<long long>(i) * p.ldr] : 0u;
+    }
+  } else {
+    const uint16_t* src = static_cast<const uint16_t*>(p.residual) + j;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      r[t] = i < i_end ? src[static_cast<long long>(i) * p.ldr] : 0u;
+    }
+  }
+}
+
+// Scale, bias, activation, residual, rounding and the stores of tokens
+// i0, i0 + step, ... (those below i_end) at column j. The residual's words were
+// loaded by the thread that stores, so y may be the residual's own buffer.
+template <int NV>
+__device__ __forceinline__ void finish(const LinArgs& p, float (&v)[NV], const uint32_t (&res)[NV], int i0, int step,
+                                       int i_end, int j, float ws, float bs) {
+  if (p.a_scale != nullptr) {
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      v[t] *= (i < i_end ? p.a_scale[i] : 0.0f) * ws;
+    }
+  } else if (p.w_scale != nullptr) {
+#pragma unroll
+    for (int t = 0; t < NV; ++t) v[t] *= ws;
+  }
+  if (p.bias != nullptr) {
+#pragma unroll
+    for (int t = 0; t < NV; ++t) v[t] += bs;
+  }
+  activate<NV>(v, p.act);
+  if (p.out == OSC_F32) {
+    float* dst = static_cast<float*>(p.y) + j;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      const float o = p.residual != nullptr ? v[t] + __uint_as_float(res[t]) : v[t];
+      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = o;
+    }
+  } else if (p.out == OSC_BF16) {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.y) + j;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      const float o = p.residual != nullptr ? v[t] + __uint_as_float(res[t] << 16) : v[t];
+      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = __float2bfloat16_rn(o);
+    }
+  } else {
+    __half* dst = static_cast<__half*>(p.y) + j;
+#pragma unroll
+    for (int t = 0; t < NV; ++t) {
+      const int i = i0 + t * step;
+      const float o =
+          p.residual != nullptr ? v[t] + __half2float(__ushort_as_half(static_cast<unsigned short>(res[t]))) : v[t];
+      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = __float2half_rn(o);
+    }
+  }
+}
+
+__device__ __forceinline__ float column_scale(const LinArgs& p, int j, bool in) {
+  if (p.w_scale == nullptr) return 1.0f;
+  return in ? p.w_scale[p.w_scale_n > 1 ? j : 0] : 0.0f;
+}
+
+// One epilogue warp's share of a tile: its 32 columns (TMEM lanes) and every
+// second group of 16 tokens, the next group's residual in flight while this
+// one is finished.
+template <int KIND>
+__device__ __forceinline__ void drain_tile(const LinArgs& p, uint32_t tmem_lane, int half, int m0, int j, float ws,
+                                           float bs, uint32_t (&res)[16]) {
+  const bool in = j < p.N;
+  const int i_end = in ? min(p.M, m0 + p.bn) : 0;
+  for (int c = half; c * 16 < p.bn; c += 2) {
+    const int i0 = m0 + c * 16;
+    if (i0 >= p.M) break;
+    uint32_t r[16], next[16];
+    tmem_ld16(tmem_lane + c * 16, r);
+    if (p.residual != nullptr) load_residual<16>(p, i0 + 32, 1, i_end, j, next);
+    tmem_wait_ld();
+    float v[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) v[t] = sum_of<KIND>(r[t]);
+    finish<16>(p, v, res, i0, 1, i_end, j, ws, bs);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) res[t] = next[t];
+  }
+}
+
+// ------------------------------------------------------------------ rows of A that no TMA box fits
+// kLoadWarps warps write the token operand of a stage themselves, in the
+// layout the 128-byte-swizzled TMA box would have: a lane takes four bytes of a
+// row from the one or two aligned words that hold them (each holds a byte of
+// the row, so neither lies outside the tensor's allocation), bytes past K and
+// rows past M are zeros.
+__device__ __forceinline__ void load_rows(const LinArgs& p, uint8_t* dst, int row0, int rows, int kb, int w, int lane) {
+  const int off = kb * kKB + lane * 4;
+  const int valid = min(4, p.k_bytes - off);  // <= 0: nothing of the row here
+  constexpr int U = 8;
+  for (int r0 = w; r0 < rows; r0 += kLoadWarps * U) {
+    uint32_t w0[U], w1[U], sh[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = row0 + r0 + u * kLoadWarps;
+      w0[u] = w1[u] = sh[u] = 0u;
+      if (r0 + u * kLoadWarps < rows && i < p.M && valid > 0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p.a + static_cast<long long>(i) * p.lda_bytes + off);
+        const uint32_t s = static_cast<uint32_t>(at & 3u);
+        const uint32_t* word = reinterpret_cast<const uint32_t*>(at - s);
+        w0[u] = word[0];
+        if (static_cast<int>(s) + valid > 4) w1[u] = word[1];
+        sh[u] = 8u * s;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * kLoadWarps;
+      if (r < rows) {
+        uint32_t v = __funnelshift_r(w0[u], w1[u], sh[u]);
+        if (valid < 4) v = valid > 0 ? v & ((1u << (8 * valid)) - 1u) : 0u;
+        *reinterpret_cast<uint32_t*>(dst + r * kKB + ((((lane >> 2) ^ r) & 7) << 4) + (lane & 3) * 4) = v;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ many tokens
+// Persistent CTAs (or CTA pairs, cta_group::2: 256 columns a tile, each CTA
+// streams its own 128 columns of weights and half of the tokens) walk the
+// tiles, eight token tiles by all column tiles at a time so that the tiles in
+// flight share operands in L2. Two 256-column TMEM accumulators: the MMA warp
+// fills one while the epilogue warps empty the other.
+__device__ __forceinline__ void tile_at(const LinArgs& p, int t, int& tm, int& tn) {
+  constexpr int kGroup = 8;
+  const int per = kGroup * p.tiles_n;
+  const int g = t / per, in = t - g * per;
+  const int h = min(kGroup, p.tiles_m - g * kGroup);
+  tn = in / h;
+  tm = g * kGroup + (in - tn * h);
+}
+
+template <int KIND, bool PAIR, bool ATMA>
+__global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)), 1)
+    k_linear_tiles(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
+                   const __grid_constant__ LinArgs p, int* __restrict__ err) {
+  static_assert(ATMA || !PAIR, "rows without a TMA box are loaded by single CTAs");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  LinBars* b = reinterpret_cast<LinBars*>(ring + p.stages * p.stage_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int P = PAIR ? 2 : 1;
+  const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+  const int first = static_cast<int>(blockIdx.x) / P, walkers = static_cast<int>(gridDim.x) / P;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int arows = p.bn / P;  // token rows of this CTA
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&b->full[s], ATMA ? 1 : 1 + kLoadWarps);
+      mbar_init(&b->empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&b->acc_full[i], 1);
+      mbar_init(&b->acc_empty[i], P * kEpiWarps);
+    }
+    mbar_init(&b->exit_bar, 1);
+    b->abort_flag = 0;
+    b->no_abort = 0;
+    fence_mbar_init();
+    tma_prefetch(&mW);
+    if (ATMA) tma_prefetch(&mA);
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(&b->tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&b->tmem_slot, 512);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  if (PAIR) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = b->tmem_slot;
+  griddep_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full0 = PAIR ? mapa_shared(&b->full[0], 0) : 0u;
+      int kc = 0;       // k-blocks issued so far
+      bool waited = false;
+      int pre = 0;      // weight blocks issued before the previous kernel was waited for
+      bool ok = true;
+      auto load_w = [&](int s, int tn, int kb) {
+        uint8_t* st = ring + s * p.stage_bytes;
+        const int row = ((tn * P + rank) * p.num_kb + kb) * kCols;
+        if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * (kWBytes + (ATMA ? arows * kKB : 0)));
+        if (PAIR) tma_load_2d_pair(st, &mW, full0 + static_cast<uint32_t>(s * 8), 0, row);
+        else tma_load_2d(st, &mW, &b->full[s], 0, row);
+      };
+      for (int t = first; t < tiles && ok; t += walkers) {
+        int tm, tn;
+        tile_at(p, t, tm, tn);
+        if (!waited) {
+          // the weights were laid out before this launch was made: their first
+          // blocks travel while the previous kernel on the stream drains
+          pre = min(p.stages, p.num_kb);
+          for (int kb = 0; kb < pre; ++kb) load_w(kb, tn, kb);
+          griddep_wait();
+          waited = true;
+        }
+        for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
+          const int s = kc % p.stages;
+          if (kc >= pre) {
+            if (!mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err)) {
+              ok = false;
+              break;
+            }
+            load_w(s, tn, kb);
+          }
+          if (ATMA) {
+            uint8_t* st = ring + s * p.stage_bytes + kWBytes;
+            const int row = tm * p.bn + rank * arows;
+            if (PAIR) tma_load_2d_pair(st, &mA, full0 + static_cast<uint32_t>(s * 8), kb * kKB, row);
+            else tma_load_2d(st, &mA, &b->full[s], kb * kKB, row);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t own = PAIR ? mapa_shared(b, 0) : 0u, peer = PAIR ? mapa_shared(b, 1) : 0u;
+      auto commit = [&](uint64_t* bar) {
+        if (PAIR) {
+          const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uint8_t*>(bar) - reinterpret_cast<uint8_t*>(b));
+          mma_commit_pair(own + off);
+          mma_commit_pair(peer + off);
+        } else {
+          mma_commit(bar);
+        }
+      };
+      int kc = 0, it = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += walkers, ++it) {
+        const int buf = it & 1;
+        if (!mbar_wait(&b->acc_empty[buf], ((it >> 1) & 1u) ^ 1u, &b->abort_flag, err)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(buf * 256);
+        for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
+          const int s = kc % p.stages;
+          if (!mbar_wait(&b->full[s], (kc / p.stages) & 1u, &b->abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t base = smem_addr(ring + s * p.stage_bytes);
+          const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
+          const int steps = kb + 1 == p.num_kb ? p.last_steps : 4;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < steps) {
+              const uint64_t off = static_cast<uint64_t>(kk * 2);  // 32 bytes of K
+              if (PAIR) mma_two<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+              else mma_one<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+            }
+          commit(&b->empty[s]);
+        }
+        if (ok) commit(&b->acc_full[buf]);
+      }
+    }
+  } else if (warp < 2 + kEpiWarps) {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t acce0 = PAIR ? mapa_shared(&b->acc_empty[0], 0) : 0u;
+    griddep_wait();
+    int it = 0;
+    for (int t = first; t < tiles; t += walkers, ++it) {
+      int tm, tn;
+      tile_at(p, t, tm, tn);
+      const int m0 = tm * p.bn;
+      const int j = (tn * P + rank) * kCols + q * 32 + lane;
+      const bool in = j < p.N;
+      const float ws = column_scale(p, j, in);
+      const float bs = p.bias != nullptr && in ? p.bias[j] : 0.0f;
+      uint32_t res[16];
+      if (p.residual != nullptr) load_residual<16>(p, m0 + half * 16, 1, in ? min(p.M, m0 + p.bn) : 0, j, res);
+      const int buf = it & 1;
+      const bool ok = mbar_wait(&b->acc_full[buf], (it >> 1) & 1u, &b->abort_flag, err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      drain_tile<KIND>(p, tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * 256), half, m0, j,
+                       ws, bs, res);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(acce0 + static_cast<uint32_t>(buf * 8));
+        else mbar_arrive(&b->acc_empty[buf]);
+      }
+    }
+  } else {
+    griddep_wait();
+    const int w = warp - 2 - kEpiWarps;
+    int kc = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += walkers) {
+      int tm, tn;
+      tile_at(p, t, tm, tn);
+      for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
+        const int s = kc % p.stages;
+        ok = mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        load_rows(p, ring + s * p.stage_bytes + kWBytes, tm * p.bn, arows, kb, w, lane);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->full[s]);
+      }
+    }
+  }
+
+  // Leave once nothing is in flight: after a wait that ran out the copies get
+  // time to land, and a CTA of a pair stays until its peer has finished with it.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    if (b->abort_flag) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 50ull * 1000ull * 1000ull) {
+      }
+    }
+    if (PAIR) {
+      mbar_arrive_cluster(mapa_shared(&b->exit_bar, rank ^ 1));
+      mbar_wait(&b->exit_bar, 0, &b->no_abort, err);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ few tokens
+// The weights' bytes bound these products, so every SM has to stream: a
+// cluster of `split` CTAs shares a tile of 128 columns, each sums its own run
+// of K blocks, and the partial sums meet in the cluster's shared memory, where
+// CTA r adds the tokens of its slice in the order of the CTAs (the same result
+// on every run; no workspace in global memory). Two CTAs fit an SM.
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int KIND, bool ATMA>
+__global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)), 2)
+    k_linear_split(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
+                   const __grid_constant__ LinArgs p, uint32_t tmem_cols, int* __restrict__ err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  LinBars* b = reinterpret_cast<LinBars*>(ring + p.stages * p.stage_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.split;  // CTA of the cluster: clusters are runs of `split` blocks
+  const int tile = static_cast<int>(blockIdx.x) / p.split;
+  const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
+  const int kb0 = static_cast<int>(static_cast<long long>(rank) * p.num_kb / p.split);
+  const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * p.num_kb / p.split);
+  const int m0 = tm * p.bn;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&b->full[s], ATMA ? 1 : 1 + kLoadWarps);
+      mbar_init(&b->empty[s], 1);
+    }
+    mbar_init(&b->acc_full[0], 1);
+    b->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch(&mW);
+    if (ATMA) tma_prefetch(&mA);
+  }
+  if (warp == 1) {
+    tmem_alloc(&b->tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = b->tmem_slot;
+  griddep_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const int pre = min(p.stages, kb1 - kb0);
+      auto load_w = [&](int s, int kb) {
+        mbar_arrive_expect_tx(&b->full[s], kWBytes + (ATMA ? p.bn * kKB : 0));
+        tma_load_2d(ring + s * p.stage_bytes, &mW, &b->full[s], 0, (tn * p.num_kb + kb) * kCols);
+      };
+      for (int kc = 0; kc < pre; ++kc) load_w(kc, kb0 + kc);  // laid out before this launch was made
+      griddep_wait();
+      for (int kc = 0; kc < kb1 - kb0; ++kc) {
+        const int s = kc % p.stages;
+        if (kc >= pre) {
+          if (!mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err)) break;
+          load_w(s, kb0 + kc);
+        }
+        if (ATMA) tma_load_2d(ring + s * p.stage_bytes + kWBytes, &mA, &b->full[s], (kb0 + kc) * kKB, m0);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int kc = 0; kc < kb1 - kb0; ++kc) {
+        const int s = kc % p.stages;
+        if (!mbar_wait(&b->full[s], (kc / p.stages) & 1u, &b->abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t base = smem_addr(ring + s * p.stage_bytes);
+        const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
+        const int steps = kb0 + kc + 1 == p.num_kb ? p.last_steps : 4;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (kk < steps) {
+            const uint64_t off = static_cast<uint64_t>(kk * 2);
+            mma_one<KIND>(tmem, dw + off, da + off, p.idesc, (kc | kk) != 0 ? 1u : 0u);
+          }
+        mma_commit(&b->empty[s]);
+      }
+      if (ok) mma_commit(&b->acc_full[0]);
+    }
+  } else if (warp >= 2 + kEpiWarps) {
+    griddep_wait();
+    const int w = warp - 2 - kEpiWarps;
+    for (int kc = 0; kc < kb1 - kb0; ++kc) {
+      const int s = kc % p.stages;
+      const bool ok = mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      load_rows(p, ring + s * p.stage_bytes + kWBytes, m0, p.bn, kb0 + kc, w, lane);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->full[s]);
+    }
+  }
+
+  const bool epi = warp >= 2 && warp < 2 + kEpiWarps;
+  const int q = warp & 3, half = (warp - 2) >> 2;
+  const int col = q * 32 + lane;
+  const int j = tn * kCols + col;
+  const bool in = j < p.N;
+  const int tokens = min(p.bn, p.M - m0);
+  float ws = 0.0f, bs = 0.0f;
+  bool ok = false;
+  if (epi) {
+    griddep_wait();
+    ws = column_scale(p, j, in);
+    bs = p.bias != nullptr && in ? p.bias[j] : 0.0f;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    if (p.split == 1) {
+      uint32_t res[16];
+      if (p.residual != nullptr) load_residual<16>(p, m0 + half * 16, 1, in ? m0 + tokens : 0, j, res);
+      ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
+      if (__all_sync(0xffffffffu, ok)) {
+        tc_fence_after();
+        drain_tile<KIND>(p, lane_base, half, m0, j, ws, bs, res);
+      }
+    } else {
+      ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        // every block of this CTA has been multiplied: the ring is free and
+        // takes the partial sums, [token][column]
+        tc_fence_after();
+        uint32_t* part = reinterpret_cast<uint32_t*>(ring);
+        for (int c = half; c * 16 < tokens; c += 2) {
+          uint32_t r[16];
+          tmem_ld16(lane_base + c * 16, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int t = 0; t < 16; ++t) part[(c * 16 + t) * kCols + col] = r[t];
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    if (epi) {
+      const int slice = (tokens + p.split - 1) / p.split;
+      const int lo = rank * slice, hi = min(tokens, lo + slice);
+      const uint32_t own = smem_addr(ring) + static_cast<uint32_t>(col * 4);
+      uint32_t peer[kMaxSplit];
+#pragma unroll
+      for (int c = 0; c < kMaxSplit; ++c)
+        if (c < p.split) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[c]) : "r"(own), "r"(c));
+      constexpr int U = 4;
+      for (int i = lo + half; i < hi; i += 2 * U) {
+        uint32_t res[U];
+        const int i_end = in ? m0 + hi : 0;
+        if (p.residual != nullptr) load_residual<U>(p, m0 + i, 2, i_end, j, res);
+        uint32_t acc[U] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c)
+          if (c < p.split) {
+            uint32_t part[U];
+#pragma unroll
+            for (int t = 0; t < U; ++t) part[t] = ld_cluster(peer[c] + static_cast<uint32_t>(min(i + 2 * t, hi - 1) * kCols * 4));
+#pragma unroll
+            for (int t = 0; t < U; ++t)
+              acc[t] = KIND == LIN_I8 ? acc[t] + part[t] : __float_as_uint(__uint_as_float(acc[t]) + __uint_as_float(part[t]));
+          }
+        float v[U];
+#pragma unroll
+        for (int t = 0; t < U; ++t) v[t] = sum_of<KIND>(acc[t]);
+        finish<U>(p, v, res, m0 + i, 2, i_end, j, ws, bs);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();  // a CTA stays until its partial sums have been read
+  }
+  __syncwarp();
+  __syncthreads();
+  if (threadIdx.x == 0 && b->abort_flag) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 50ull * 1000ull * 1000ull) {
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+// ------------------------------------------------------------------ the weights' layout
+// [k, n] (or [n, k]) -> [tiles][num_kb][128][128 bytes], zeros past n and k.
+// A CTA moves a tile of 32 columns x one block of K through shared memory, so
+// both sides run along their contiguous axis.
+template <typename T>
+__global__ void k_linear_pack(const T* __restrict__ w, int k, int n, int n_major, int num_kb, T* __restrict__ blocks) {
+  constexpr int KE = kKB / static_cast<int>(sizeof(T));
+  __shared__ T tile[32][KE + 4 / sizeof(T)];
+  const int kb = blockIdx.x, c0 = static_cast<int>(blockIdx.y) * 32;
+  const int t0 = kb * KE;
+  if (n_major) {
+    for (int x = threadIdx.x; x < 32 * KE; x += blockDim.x) {
+      const int c = x / KE, t = x % KE;
+      tile[c][t] = c0 + c < n && t0 + t < k ? w[static_cast<size_t>(c0 + c) * k + t0 + t] : T(0);
+    }
+  } else {
+    for (int x = threadIdx.x; x < 32 * KE; x += blockDim.x) {
+      const int c = x % 32, t = x / 32;
+      tile[c][t] = c0 + c < n && t0 + t < k ? w[static_cast<size_t>(t0 + t) * n + c0 + c] : T(0);
+    }
+  }
+  __syncthreads();
+  T* dst = blocks + ((static_cast<size_t>(c0 / kCols) * num_kb + kb) * kCols + c0 % kCols) * KE;
+  for (int x = threadIdx.x; x < 32 * KE; x += blockDim.x) dst[x] = tile[x / KE][x % KE];
+}
+
+// ------------------------------------------------------------------ host side
+int dtype_bytes(int dtype) {
+  switch (dtype) {
+    case OSC_F32: return 4;
+    case OSC_F16:
+    case OSC_BF16: return 2;
+    case OSC_S8:
+    case OSC_E4M3: return 1;
+    default: return 0;
+  }
+}
+
+struct LinPlan {
+  bool split_kernel;
+  bool pair;
+  int bn, split;
+};
+
+int div_up(int a, int b) { return (a + b - 1) / b; }
+
+// Which kernel, tile and split: the fewest cycles by a count of what a tile
+// costs. One k-block is four MMAs of max(50, bn / 2) cycles.
+LinPlan choose(int num_sms, int m, int n, int num_kb, bool atma) {
+  LinPlan best{};
+  double best_t = 1e300;
+  const int cols = div_up(n, kCols);
+  auto consider = [&](LinPlan c, double t) {
+    if (t < best_t) {
+      best_t = t;
+      best = c;
+    }
+  };
+  for (int bn = 16; bn <= 128; bn += 16) {
+    if (bn > 16 && bn - 16 >= m) break;
+    const double tiles = static_cast<double>(cols) * div_up(m, bn);
+    for (int split = 1; split <= kMaxSplit; split *= 2) {
+      if (split > num_kb) break;
+      const double waves = std::ceil(tiles * split / (2 * num_sms));
+      const double kb = div_up(num_kb, split);
+      consider({true, false, bn, split},
+               waves * (kb * std::max(2 * 4 * std::max(50.0, bn / 2.0), 2 * (kWBytes + bn * kKB) / 40.0) + 1500 + 10 * bn) + (split > 1 ? 1500 : 0));
+    }
+  }
+  for (int pair = 0; pair <= (atma ? 1 : 0); ++pair) {
+    const int step = pair ? 32 : 16;
+    for (int bn = step; bn <= 256; bn += step) {
+      if (bn > step && bn - step >= m) break;
+      const double tiles = static_cast<double>(div_up(cols, pair ? 2 : 1)) * div_up(m, bn);
+      const double waves = std::ceil(tiles / (num_sms / (pair ? 2 : 1)));
+      const double bytes = kWBytes + static_cast<double>(bn) * kKB / (pair ? 2 : 1);
+      consider({false, pair != 0, bn, 1},
+               waves * num_kb * std::max(4 * std::max(50.0, bn / 2.0), bytes / 60.0) + 2500 + 20.0 * bn);
+    }
+  }
+  return best;
+}
+
+template <int KIND>
+int launch_tiles(osc_ctx* ctx, const LinPlan& pl, bool atma, const CUtensorMap& mW, const CUtensorMap& mA,
+                 const LinArgs& p) {
+  void (*kern)(CUtensorMap, CUtensorMap, LinArgs, int*) =
+      pl.pair ? k_linear_tiles<KIND, true, true> : atma ? k_linear_tiles<KIND, false, true> : k_linear_tiles<KIND, false, false>;
+  const int smem = p.stages * p.stage_bytes + kSmemTail + 1024;
+  OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(kern), smem));
+  const int per = pl.pair ? 2 : 1;
+  const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, ctx->num_sms / per) * per));
+  cfg.blockDim = dim3(64 + 32 * (kEpiWarps + (atma ? 0 : kLoadWarps)));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.pair ? 2 : 1;
+  prof_begin(ctx);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mW, mA, p, ctx->d_err);
+  if (e != cudaSuccess) return cuda_fail(e, "k_linear_tiles launch");
+  return check_launch(ctx, "k_linear_tiles");
+}
+
+template <int KIND>
+int launch_split(osc_ctx* ctx, bool atma, const CUtensorMap& mW, const CUtensorMap& mA, const LinArgs& p) {
+  void (*kern)(CUtensorMap, CUtensorMap, LinArgs, uint32_t, int*) =
+      atma ? k_linear_split<KIND, true> : k_linear_split<KIND, false>;
+  const int smem = p.stages * p.stage_bytes + kSmemTail + 1024;
+  OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(kern), smem));
+  uint32_t cols = 32;
+  while (cols < static_cast<uint32_t>(p.bn)) cols *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * p.split));
+  cfg.blockDim = dim3(64 + 32 * (kEpiWarps + (atma ? 0 : kLoadWarps)));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  prof_begin(ctx);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mW, mA, p, cols, ctx->d_err);
+  if (e != cudaSuccess) return cuda_fail(e, "k_linear_split launch");
+  return check_launch(ctx, "k_linear_split");
+}
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0; }
+
+int linear_prepack(osc_ctx* ctx, int dtype, const void* w, int k, int n, int layout, int host,
+                   osc_linear_weights** out) {
+  const int e = dtype_bytes(dtype);
+  const size_t bytes = static_cast<size_t>(k) * n * e;
+  auto* d = new (std::nothrow) osc_linear_weights();
+  if (d == nullptr) return fail(OSC_ENOMEM, "osc_linear_prepack: out of host memory");
+  d->device = ctx->device;
+  d->dtype = dtype;
+  d->k = k;
+  d->n = n;
+  d->num_kb = static_cast<int>((static_cast<long long>(k) * e + kKB - 1) / kKB);
+  d->tiles = div_up(n, kCols);
+  const size_t packed = static_cast<size_t>(d->tiles) * d->num_kb * kWBytes;
+  void* staged = nullptr;
+  cudaError_t err = cudaMalloc(&d->blocks, packed);
+  if (err == cudaSuccess && host) {
+    err = cudaMalloc(&staged, bytes);
+    if (err == cudaSuccess) err = cudaMemcpyAsync(staged, w, bytes, cudaMemcpyHostToDevice, ctx->stream);
+    w = staged;
+  }
+  int st = OSC_OK;
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    st = fail(OSC_ENOMEM, "osc_linear_prepack: %s", cudaGetErrorString(err));
+  }
+  if (st == OSC_OK) {
+    const dim3 grid(static_cast<unsigned>(d->num_kb), static_cast<unsigned>(d->tiles * (kCols / 32)));
+    prof_begin(ctx);
+    if (e == 2)
+      k_linear_pack<uint16_t><<<grid, 256, 0, ctx->stream>>>(static_cast<const uint16_t*>(w), k, n, layout, d->num_kb,
+                                                            reinterpret_cast<uint16_t*>(d->blocks));
+    else
+      k_linear_pack<uint8_t><<<grid, 256, 0, ctx->stream>>>(static_cast<const uint8_t*>(w), k, n, layout, d->num_kb,
+                                                           d->blocks);
+    st = check_launch(ctx, "k_linear_pack");
+  }
+  if (st == OSC_OK) {
+    const uint64_t dims[2] = {kKB, static_cast<uint64_t>(d->tiles) * d->num_kb * kCols};
+    const uint64_t pitch[1] = {kKB};
+    const uint32_t box[2] = {kKB, kCols};
+    st = encode_tiled(&d->map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, d->blocks, dims, pitch, box,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  // the products start on the blocks before the previous kernel on their stream
+  // is done, so the blocks are complete before the handle is given out
+  const cudaError_t synced = cudaStreamSynchronize(ctx->stream);
+  if (st == OSC_OK && synced != cudaSuccess) st = cuda_fail(synced, "osc_linear_prepack");
+  cudaFree(staged);
+  if (st != OSC_OK) {
+    cudaFree(d->blocks);
+    delete d;
+    return st;
+  }
+  *out = d;
+  return OSC_OK;
+}
+
+}  // namespace
+}  // namespace osc
+
+using namespace osc;
+
+extern "C" {
+
+OSC_API int osc_linear_prepack(osc_ctx* ctx, int dtype, const void* w, int k, int n, int layout, int host,
+                               osc_linear_weights** out) {
+  if (out == nullptr) return fail(OSC_EINVAL, "osc_linear_prepack: out is null");
+  *out = nullptr;
+  if (ctx == nullptr) return fail(OSC_EINVAL, "null context");
+  if (dtype != OSC_F16 && dtype != OSC_BF16 && dtype != OSC_S8 && dtype != OSC_E4M3)
+    return fail(OSC_EINVAL, "osc_linear_prepack: dtype %d is not f16, bf16, s8 or e4m3", dtype);
+  if (w == nullptr || k <= 0 || n <= 0) return fail(OSC_EINVAL, "osc_linear_prepack: bad W [%d, %d]", k, n);
+  if (layout != 0 && layout != 1) return fail(OSC_EINVAL, "osc_linear_prepack: layout %d", layout);
+  // |s8 * s8| <= 2^14: k products stay inside S32
+  if (dtype == OSC_S8 && k >= (1 << 17)) return fail(OSC_EINVAL, "osc_linear_prepack: k %d overflows S32 sums", k);
+  // rows of 128 bytes are TMA coordinates (signed 32 bits); the grid's y axis holds groups of 32 columns
+  const long long kb = (static_cast<long long>(k) * dtype_bytes(dtype) + kKB - 1) / kKB;
+  if (div_up(n, 32) > 65532 || (static_cast<long long>(div_up(n, kCols)) + 1) * kb * kCols >= (1ll << 31))
+    return fail(OSC_EINVAL, "osc_linear_prepack: W [%d, %d] is too large", k, n);
+  if (!aligned(w, dtype_bytes(dtype))) return fail(OSC_EINVAL, "osc_linear_prepack: W is not aligned to its type");
+  OSC_TRY(enter(ctx));
+  if (capturing(ctx)) return fail(OSC_EINVAL, "osc_linear_prepack: the stream is being captured");
+  if (fault_injected("prepack")) return fail(OSC_EFAULT_INJECTED, "injected failure (prepack)");
+  return linear_prepack(ctx, dtype, w, k, n, layout, host, out);
+}
+
+OSC_API int osc_linear_weights_free(osc_linear_weights* w) {
+  if (w == nullptr) return OSC_OK;
+  cudaSetDevice(w->device);
+  cudaDeviceSynchronize();
+  cudaFree(w->blocks);
+  delete w;
+  return OSC_OK;
+}
+
+OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const osc_linear_weights* w,
+                       const float* a_scale, const float* w_scale, int n_scale, const float* bias, int act,
+                       const void* residual, long long ldr, int out_dtype, void* y, long long ldy) {
+  if (ctx == nullptr) return fail(OSC_EINVAL, "null context");
+  if (w == nullptr) return fail(OSC_EINVAL, "osc_linear: null weights");
+  if (w->device != ctx->device) return fail(OSC_EINVAL, "osc_linear: weights of device %d on device %d", w->device, ctx->device);
+  if (m < 0) return fail(OSC_EINVAL, "osc_linear: m = %d", m);
+  const bool coded = w->dtype == OSC_S8 || w->dtype == OSC_E4M3;
+  if (out_dtype != OSC_F32 && out_dtype != OSC_F16 && out_dtype != OSC_BF16)
+    return fail(OSC_EINVAL, "osc_linear: output dtype %d is not f32, f16 or bf16", out_dtype);
+  if (act < OSC_ACT_NONE || act > OSC_ACT_GELU_TANH) return fail(OSC_EINVAL, "osc_linear: activation %d", act);
+  if (!coded && (a_scale != nullptr || w_scale != nullptr))
+    return fail(OSC_EINVAL, "osc_linear: scales belong to 8-bit operands");
+  if (w_scale != nullptr && n_scale != 1 && n_scale != w->n)
+    return fail(OSC_EINVAL, "osc_linear: %d column scales for %d columns", n_scale, w->n);
+  if (lda == 0) lda = w->k;
+  if (ldy == 0) ldy = w->n;
+  if (ldr == 0) ldr = w->n;
+  if (lda < w->k || ldy < w->n || (residual != nullptr && ldr < w->n))
+    return fail(OSC_EINVAL, "osc_linear: a row pitch (%lld, %lld, %lld) below the row's length", lda, ldy, ldr);
+  if (m == 0) return OSC_OK;
+  if (a == nullptr || y == nullptr) return fail(OSC_EINVAL, "osc_linear: null pointer");
+  const int e = dtype_bytes(w->dtype), o = dtype_bytes(out_dtype);
+  if (!aligned(a, e) || !aligned(y, o) || !aligned(residual, o) || !aligned(a_scale, 4) || !aligned(w_scale, 4) ||
+      !aligned(bias, 4))
+    return fail(OSC_EINVAL, "osc_linear: a pointer is not aligned to its type");
+  OSC_TRY(enter(ctx));
+  if (fault_injected("launch")) return fail(OSC_EFAULT_INJECTED, "injected failure (launch)");
+
+  const bool atma = aligned(a, 16) && (m == 1 || (lda * e) % 16 == 0);
+  const LinPlan pl = choose(ctx->num_sms, m, w->n, w->num_kb, atma);
+  LinArgs p = {};
+  p.M = m;
+  p.N = w->n;
+  p.num_kb = w->num_kb;
+  p.k_bytes = w->k * e;
+  p.last_steps = div_up(p.k_bytes - (w->num_kb - 1) * kKB, 32);
+  p.bn = pl.bn;
+  p.split = pl.split;
+  const int arows = pl.pair ? pl.bn / 2 : pl.bn;
+  p.stage_bytes = kWBytes + arows * kKB;
+  p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemTwo : kSmemOne) - kSmemTail) / p.stage_bytes);
+  p.tiles_m = div_up(m, pl.bn);
+  p.tiles_n = div_up(w->n, pl.pair ? 2 * kCols : kCols);
+  if (static_cast<long long>(p.tiles_m) * p.tiles_n * pl.split >= (1ll << 31) || m > (1 << 30))
+    return fail(OSC_EINVAL, "osc_linear: %d rows are too many", m);
+  const uint32_t rows = pl.pair ? 256u : 128u;
+  const uint32_t size = (static_cast<uint32_t>(pl.bn >> 3) << 17) | ((rows >> 4) << 24);
+  p.a_scale = a_scale;
+  p.w_scale = w_scale;
+  p.w_scale_n = n_scale;
+  p.bias = bias;
+  p.act = act;
+  p.out = out_dtype;
+  p.residual = residual;
+  p.ldr = ldr;
+  p.y = y;
+  p.ldy = ldy;
+  p.a = static_cast<const uint8_t*>(a);
+  p.lda_bytes = lda * e;
+
+  CUtensorMap mA{};
+  if (atma) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.k_bytes), static_cast<uint64_t>(m)};
+    const uint64_t pitch[1] = {m == 1 ? round_up(static_cast<size_t>(p.k_bytes), 16) : static_cast<uint64_t>(lda) * e};
+    const uint32_t box[2] = {kKB, static_cast<uint32_t>(arows)};
+    OSC_TRY(encode_tiled(&mA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B));
+  }
+  switch (w->dtype) {
+    case OSC_F16:
+    case OSC_BF16: {
+      const uint32_t fmt = w->dtype == OSC_BF16 ? 1u : 0u;
+      p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | size;  // F32 sums
+      return pl.split_kernel ? launch_split<LIN_F16>(ctx, atma, w->map, mA, p)
+                             : launch_tiles<LIN_F16>(ctx, pl, atma, w->map, mA, p);
+    }
+    case OSC_E4M3:
+      p.idesc = (1u << 4) | size;  // both operands E4M3, F32 sums
+      return pl.split_kernel ? launch_split<LIN_F8>(ctx, atma, w->map, mA, p)
+                             : launch_tiles<LIN_F8>(ctx, pl, atma, w->map, mA, p);
+    default:
+      p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | size;  // both operands signed, S32 sums
+      return pl.split_kernel ? launch_split<LIN_I8>(ctx, atma, w->map, mA, p)
+                             : launch_tiles<LIN_I8>(ctx, pl, atma, w->map, mA, p);
+  }
+}
+
+}  // extern "C"

@@ -93,6 +93,62 @@ def layernorm(ctx, x, gamma, beta, eps, y, inner=None):
     return y
 
 
+def _rows(name, t, ctx, like=None):
+    """(row pitch, rows, columns) of a [..., columns] device tensor whose rows follow one another at one pitch."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise ValueError(f"{name} has no columns: {tuple(t.shape)}")
+    if like is not None and t.shape != like.shape:
+        raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(like.shape)}")
+    cols = int(t.shape[-1])
+    if t.dim() == 1 or t.is_contiguous():
+        if t.stride(-1) != 1 and cols > 1:
+            raise ValueError(f"{name}: elements of a row must be adjacent")
+        return cols, t.numel() // cols, cols
+    ok = t.stride(-1) == 1 or cols == 1
+    for d in range(t.dim() - 2):  # leading dimensions fold into one run of rows
+        ok = ok and (t.shape[d] == 1 or t.stride(d) == t.stride(d + 1) * t.shape[d + 1])
+    if not ok or (t.shape[-2] > 1 and t.stride(-2) < cols):
+        raise ValueError(f"{name}: rows must be dense and follow one another at one pitch")
+    return max(int(t.stride(-2)), cols), t.numel() // cols, cols
+
+
+def _rmsnorm(ctx, x, gamma, eps, residual, sum_out, y, q, scales):
+    ld, rows, cols = _rows("x", x, ctx)
+    pitch = {"residual": 0, "sum_out": 0, "y": 0, "q": 0}
+    for name, t in (("residual", residual), ("sum_out", sum_out), ("y", y), ("q", q)):
+        if t is not None:
+            pitch[name] = _rows(name, t, ctx, x)[0]
+            if name != "q" and t.dtype != x.dtype:
+                raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
+    if gamma is not None:
+        _rows("gamma", gamma, ctx)
+        if gamma.dtype != x.dtype or gamma.numel() != cols or not gamma.is_contiguous():
+            raise ValueError(f"gamma must be {cols} adjacent {x.dtype} values")
+    if scales is not None:
+        _rows("scales", scales, ctx)
+        if str(scales.dtype) != "torch.float32" or scales.numel() != rows or not scales.is_contiguous():
+            raise ValueError(f"scales must be {rows} adjacent float32 values")
+    call("osc_rmsnorm", ctx.handle, _lib.dtype_code(x.dtype), ptr(x), ld, ptr(residual), pitch["residual"], rows, cols,
+         ptr(gamma), float(eps), ptr(sum_out), pitch["sum_out"], ptr(y), pitch["y"],
+         0 if q is None else _lib.dtype_code(q.dtype), ptr(q), pitch["q"], ptr(scales))
+
+
+def rmsnorm(ctx, x, gamma, eps, y, residual=None, sum_out=None):
+    """y = RMS norm over the last axis of h = x + residual (rounded to x's type; kept in sum_out when given),
+    times gamma. float32, float16 or bfloat16, all of one type; rows may be pitched views."""
+    _rmsnorm(ctx, x, gamma, eps, residual, sum_out, y, None, None)
+    return y
+
+
+def rmsnorm_quant(ctx, x, gamma, eps, q, scales, residual=None, sum_out=None, y=None):
+    """The same norm as 8-bit codes q (int8 or float8_e4m3fn) with one float32 scale per row, q * scale standing
+    for y: what runtime.linear takes as a and a_scale. y, when given, gets the unquantised rows too."""
+    _rmsnorm(ctx, x, gamma, eps, residual, sum_out, y, q, scales)
+    return q, scales
+
+
 def psa_attention(ctx, qkv, out, heads, kd, hd, scale):
     """qkv [B, heads*(2kd+hd), H, W] (view) -> out [B, heads*hd, H, W] (view)."""
     n, _, h, w, qs = _nchw(qkv)

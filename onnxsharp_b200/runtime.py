@@ -307,6 +307,76 @@ def matmul_integer(ctx: Context, a, a_zero_point: int, w: "DqmmWeights", out=Non
     return out
 
 
+class LinearWeights:
+    """Constant w of linear(), laid out once: a [k, n] (layout 0) or [n, k] (layout 1) bfloat16, float16,
+    float8_e4m3fn or int8 tensor, on the context's device or on the host. Keep it while calls or captured graphs
+    that use it are alive."""
+
+    def __init__(self, ctx: Context, w, layout: int = 0):
+        if w.dim() != 2 or not w.is_contiguous():
+            raise ValueError("LinearWeights: w must be a dense matrix")
+        if w.is_cuda and w.device.index != ctx.device:
+            raise ValueError(f"LinearWeights: w is on {w.device}, the context on cuda:{ctx.device}")
+        k, n = (w.shape[1], w.shape[0]) if layout else (w.shape[0], w.shape[1])
+        h = C.c_void_p()
+        call("osc_linear_prepack", ctx.handle, _lib.dtype_code(w.dtype), ptr(w), int(k), int(n), int(layout),
+             0 if w.is_cuda else 1, C.byref(h))
+        self.handle = h
+        self.k, self.n, self.dtype = int(k), int(n), w.dtype
+        self._finalizer = weakref.finalize(self, _lib.load().osc_linear_weights_free, h)
+
+
+def _pitch(name: str, t, ctx: Context, rows: int, cols: int) -> int:
+    """Row pitch of a [rows, cols] device tensor with adjacent elements."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"linear: {name} is on {t.device}, the context on cuda:{ctx.device}")
+    if tuple(t.shape) != (rows, cols):
+        raise ValueError(f"linear: {name} is {tuple(t.shape)}, expected {(rows, cols)}")
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"linear: the rows of {name} must be dense")
+    return max(int(t.stride(0)), cols) if rows > 1 else cols
+
+
+def _vector(name: str, t, ctx: Context, *sizes: int):
+    if t is None:
+        return None
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"linear: {name} is on {t.device}, the context on cuda:{ctx.device}")
+    if str(t.dtype) != "torch.float32" or t.numel() not in sizes or not t.is_contiguous():
+        raise ValueError(f"linear: {name} must be {' or '.join(map(str, sizes))} adjacent float32 values")
+    return ptr(t)
+
+
+def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NONE, residual=None, a_scale=None,
+           w_scale=None, out=None, out_dtype=None):
+    """act((a @ w) * a_scale[:, None] * w_scale + bias) + residual for 16- and 8-bit operands, rounded once.
+    a [m, k] has w's type and may be a pitched view; a_scale [m], w_scale [n] or [1] (8-bit types) and bias [n] are
+    float32. The result is float32, float16 or bfloat16: out's, the residual's, out_dtype, else a's type (8-bit: float32).
+    out may be the residual itself."""
+    import torch
+
+    if a.dim() != 2:
+        raise ValueError(f"linear: a is {tuple(a.shape)}, expected (m, {w.k})")
+    m = int(a.shape[0])
+    if a.dtype != w.dtype:
+        raise TypeError(f"linear: a is {a.dtype}, the weights are {w.dtype}")
+    if out is None:
+        if out_dtype is None:
+            coded = a.dtype in (torch.int8, torch.float8_e4m3fn)
+            out_dtype = residual.dtype if residual is not None else torch.float32 if coded else a.dtype
+        out = torch.empty((m, w.n), dtype=out_dtype, device=a.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise TypeError(f"linear: out is {out.dtype}, not {out_dtype}")
+    if residual is not None and residual.dtype != out.dtype:
+        raise TypeError(f"linear: the residual is {residual.dtype}, the result {out.dtype}")
+    lda, ldy = _pitch("a", a, ctx, m, w.k), _pitch("out", out, ctx, m, w.n)
+    ldr = 0 if residual is None else _pitch("residual", residual, ctx, m, w.n)
+    call("osc_linear", ctx.handle, ptr(a), m, lda, w.handle, _vector("a_scale", a_scale, ctx, m),
+         _vector("w_scale", w_scale, ctx, 1, w.n), 0 if w_scale is None else int(w_scale.numel()),
+         _vector("bias", bias, ctx, w.n), int(act), ptr(residual), ldr, _lib.dtype_code(out.dtype), ptr(out), ldy)
+    return out
+
+
 def minmax(ctx: Context, x, out=None):
     """{min(x, 0), max(x, 0)} over all elements of x (NaN skipped), as a 2-float device tensor."""
     import torch
