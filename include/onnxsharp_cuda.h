@@ -405,6 +405,31 @@ OSC_API int osc_attention_f32(osc_ctx* ctx, const float* q, const float* k, cons
                               int mask_rows, int B, int T, int H, int D, float scale, int out_head_space,
                               float* out);
 
+/* Causal attention over a cache with a sliding window and a few first tokens
+ * that stay visible (no counterpart in the reference, whose FusedAttention has
+ * neither cache nor causal mask). q and out are [B, T, H, D], k and v
+ * [B, S, HK, D] (S: the cache's capacity; H a multiple of HK, at most 128 query
+ * heads on a key/value head; D 64 or 128), all of one type (OSC_F16 or
+ * OSC_BF16). *_strides (host arrays) give the element distances of a tensor's
+ * first three axes: multiples of 8 (16 bytes), base addresses likewise; the D
+ * axis is dense. lengths [B] (device): how many tokens of the sequence the
+ * cache holds, this call's among them. Query t of sequence b stands at position
+ * starts[b] + t, or, with starts NULL, at lengths[b] - T + t.
+ *
+ *   the query at position p sees the keys j <= p with j > p - window or j < sinks
+ *   out = softmax(scale * q k^T over the seen keys) v
+ *
+ * FP32 scores, softmax and sums; the probabilities are rounded to the type for
+ * the product with v, the result once more. Queries outside 0 .. lengths[b] - 1
+ * (padding) give zeros. What the cache holds at and behind lengths[b] does not
+ * matter (NaN included); v before it must be finite. window >= 1 (INT_MAX:
+ * none), sinks >= 0, scale > 0. out may not overlap the inputs. No scratch
+ * memory; results do not change from run to run. */
+OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const long long* q_strides, const void* k,
+                                 const long long* k_strides, const void* v, const long long* v_strides,
+                                 const int* lengths, const int* starts, int B, int T, int S, int H, int HK, int D,
+                                 int window, int sinks, float scale, void* out, const long long* out_strides);
+
 /* ------------------------------------------------------------ graph glue (YOLO11n-shaped graph)
  * NCHW tensors may be channel slices of larger buffers: *_nstride is the
  * element distance between consecutive images (0 = dense), so a Split output

@@ -139,6 +139,7 @@ SIGNATURES: dict[str, tuple] = {
     "osc_linear": (i32, [vp, vp, i32, i64, vp, vp, vp, i32, vp, i32, vp, i64, i32, vp, i64]),
     # FusedAttention
     "osc_attention_f32": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, i32, vp]),
+    "osc_attention_window": (i32, [vp, i32, vp, vp, vp, vp, vp, vp, vp, vp] + [i32] * 8 + [f32, vp, vp]),
     # graph glue
     "osc_conv2d_ex_f32": (i32, [vp, vp, i64, i32, i32, i32, i32, vp] + [i32] * 8 + [vp, i32, vp, i64, vp, i64, i32,
                                                                                    i32]),

@@ -1,0 +1,828 @@
+// attention_window.cu — causal attention over a cache with a sliding window and
+// a few first tokens that stay visible, 16-bit, grouped heads:
+//
+//   the query at position p sees the keys j <= p with j > p - window or j < sinks
+//   out = softmax(scale * q k^T over the seen keys) v, FP32 inside, rounded once
+//
+// It stands beside FusedAttention (attention_tf32x3.cu: FP32, every key, an
+// additive mask; src/OnnxSharp/Ops/AttentionOps.cs:249-351); the reference has
+// no cache, window or grouped heads.
+//
+// Both kernels below make one pass over the keys with the running maximum and
+// sum of the softmax in FP32 registers and split the rows of a key/value head:
+// row r of a tile is token r / G, query head r % G of the group (G query heads
+// share a key/value head), so a key is read once for the group. A masked score
+// is -inf by selection, whatever was computed for it; keys at and behind a
+// sequence's length are never used (V rows there are zeroed where a tile
+// brings them along: 0 * NaN would not vanish).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "runtime.h"
+#include "sm100.cuh"
+
+namespace osc {
+namespace {
+
+struct WinArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int* lengths;
+  const int* starts;  // null: the queries end at the length
+  long long q_b, q_t, q_h, k_b, k_s, k_h, v_b, v_s, v_h, o_b, o_t, o_h;
+  int B, T, S, H, HK, G;
+  int window, sinks;
+  float scale2;       // scale * log2(e): softmax in powers of two
+  int tokens;         // tokens of a 128-row tile (k_window_tiles)
+  int split;          // CTAs that share a row tile's keys (k_window_rows)
+  int row_tiles;
+};
+
+constexpr int kFarPos = 1 << 30;
+
+// Position of query 0 and the sequence's length, made safe whatever the device
+// holds: a start at or behind the length is padding, and so is one below -T.
+__device__ __forceinline__ void place_of(const WinArgs& p, int b, int& first, int& len) {
+  len = max(0, min(p.lengths[b], p.S));
+  first = p.starts != nullptr ? max(-kFarPos, min(p.starts[b], len)) : len - p.T;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ------------------------------------------------------------------ many rows
+// A CTA takes two tiles of 128 rows (2 * tokens consecutive tokens of one
+// key/value head's group) and walks the 128-key tiles that either sees: first
+// the tiles of the sinks, then those of the window. Per tile, S = Q K^T (both
+// from shared memory) goes to TMEM, a thread of the tile's softmax warpgroup
+// reads its row's 128 scores, writes exp2 of them back over S as 16-bit P, and
+// O += P V takes P from TMEM and V as it lies, [key][d] (MN-major). While one
+// tile's scores are in the softmax the tensor cores work on the other's.
+// O is rescaled only when a row's maximum has grown by more than 2^8 (P stays
+// below 2^8, exact in FP32 sums, no overflow in FP16), which after the first
+// tiles hardly happens.
+constexpr int kKeys = 128;
+constexpr int kWinThreads = 64 + 256;
+constexpr float kLazy = 8.0f;
+
+struct WinBars {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full;
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+template <int D>
+struct WinCfg {
+  static constexpr int CH = D / 64;                    // 128-byte columns of a row
+  static constexpr int TILE = CH * kKeys * 128;        // a [128][D] tile
+  static constexpr int SMEM = 1024 + 6 * TILE + 512;   // two Q tiles, two stages of K and V
+};
+
+struct Span {  // the key tiles of a CTA, in order
+  int sink_tiles, lo_tile, n;
+  __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : lo_tile + i - sink_tiles; }
+};
+
+struct Rows {  // live positions of a 128-row tile: none if lo > hi
+  int lo, hi;
+};
+
+__device__ __forceinline__ Rows live_rows(const WinArgs& p, int first, int len, int t0, int tokens) {
+  return {max(first + t0, 0), min(min(first + t0 + tokens, first + p.T) - 1, len - 1)};
+}
+// Some row of the tile sees some key of [j0, j0 + 128).
+__device__ __forceinline__ bool needs(const WinArgs& p, const Rows& r, int j0) {
+  return r.lo <= r.hi && j0 <= r.hi && (j0 + kKeys - 1 > r.lo - p.window || j0 < p.sinks);
+}
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// MN-major 16-bit operand as a 128-byte-swizzled TMA box lays it: rows of 64
+// elements along N, 8-row groups of K 1024 bytes apart, 64-column groups `lbo` apart.
+__device__ __forceinline__ uint64_t sdesc_mn16(uint32_t saddr, uint32_t lbo) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16) |
+         (static_cast<uint64_t>(1024u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46) |
+         (static_cast<uint64_t>(2u) << 61);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kWinThreads, 1)
+    k_window_tiles(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
+                   const __grid_constant__ CUtensorMap mV, const __grid_constant__ WinArgs p, int* __restrict__ err) {
+  using Cfg = WinCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;
+  uint8_t* sk = smem + 2 * Cfg::TILE;
+  uint8_t* sv = smem + 4 * Cfg::TILE;
+  WinBars* bar = reinterpret_cast<WinBars*>(smem + 6 * Cfg::TILE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // late tokens see the most keys of a prompt: they start first
+  const int t0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * p.tokens;
+  const int hk = blockIdx.y, b = blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar->q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->k_full[i], 1);
+      mbar_init(&bar->k_empty[i], 1);
+      mbar_init(&bar->v_full[i], 1);
+      mbar_init(&bar->v_empty[i], 1);
+      mbar_init(&bar->s_full[i], 1);
+      mbar_init(&bar->p_ready[i], 4);
+    }
+    mbar_init(&bar->o_full, 1);
+    bar->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch(&mQ);
+    tma_prefetch(&mK);
+    tma_prefetch(&mV);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bar->tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar->tmem_slot;
+  griddep_launch();
+  griddep_wait();
+
+  int first, len;
+  place_of(p, b, first, len);
+  const Rows rows[2] = {live_rows(p, first, len, t0, p.tokens), live_rows(p, first, len, t0 + p.tokens, p.tokens)};
+  const Rows both = live_rows(p, first, len, t0, 2 * p.tokens);
+  Span span{0, 0, 0};
+  if (both.lo <= both.hi) {
+    const int lo = both.lo >= p.window ? both.lo - p.window + 1 : 0;
+    span.lo_tile = lo / kKeys;
+    span.sink_tiles = min((min(p.sinks, both.hi + 1) + kKeys - 1) / kKeys, span.lo_tile);
+    span.n = span.sink_tiles + both.hi / kKeys - span.lo_tile + 1;
+  }
+
+  if (warp == 0) {
+    if (lane == 0 && span.n > 0) {
+      const int tiles_q = t0 + p.tokens < p.T ? 2 : 1;
+      const uint32_t box = static_cast<uint32_t>(p.tokens * p.G * 128);
+      mbar_arrive_expect_tx(&bar->q_full, tiles_q * Cfg::CH * box);
+      for (int w = 0; w < tiles_q; ++w)
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full, c * 64, hk * p.G, t0 + w * p.tokens, b);
+      for (int i = 0; i < span.n; ++i) {
+        const int s = i & 1;
+        const uint32_t free = ((i >> 1) & 1u) ^ 1u;
+        const int j0 = span.at(i) * kKeys;
+        if (!mbar_wait(&bar->k_empty[s], free, &bar->abort_flag, err)) break;
+        mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
+        if (!mbar_wait(&bar->v_empty[s], free, &bar->abort_flag, err)) break;
+        mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
+      }
+    }
+  } else if (warp == 1) {
+    // all lanes follow the loop (they clear V rows behind the length); lane 0 issues
+    constexpr uint32_t fmt = BF16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) |
+                                 (static_cast<uint32_t>(128 >> 4) << 24);
+    constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) |
+                                 (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+    bool ok = span.n > 0 && mbar_wait(&bar->q_full, 0, &bar->abort_flag, err);
+    uint32_t seen[2] = {0u, 0u};  // PV products issued per tile
+    auto scores = [&](int w, int i) {
+      if (lane == 0) {
+        const uint32_t q0 = smem_addr(sq + w * Cfg::TILE), k0 = smem_addr(sk + (i & 1) * Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c) {
+          const uint64_t dq = sdesc_kmajor_sw128(q0 + c * kKeys * 128), dk = sdesc_kmajor_sw128(k0 + c * kKeys * 128);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16_ss(tmem + static_cast<uint32_t>(w * kKeys), dq + kk * 2, dk + kk * 2, idesc_s, (c | kk) != 0 ? 1u : 0u);
+        }
+        mma_commit(&bar->s_full[w]);
+      }
+      __syncwarp();
+    };
+    auto wait = [&](uint64_t* m, uint32_t parity) {
+      ok = ok && mbar_wait(m, parity, &bar->abort_flag, err);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    if (wait(&bar->k_full[0], 0)) {
+      tc_fence_after();
+      for (int w = 0; w < 2; ++w)
+        if (needs(p, rows[w], span.at(0) * kKeys)) scores(w, 0);
+      if (lane == 0) mma_commit(&bar->k_empty[0]);
+      for (int i = 0; i < span.n && ok; ++i) {
+        const int s = i & 1, j0 = span.at(i) * kKeys;
+        if (!wait(&bar->v_full[s], (i >> 1) & 1u)) break;
+        if (j0 + kKeys > len) {
+          // V rows behind the length: whatever the cache holds there must not meet P's zeros
+          for (int x = (len - j0) * 8 + lane; x < kKeys * 8; x += 32)
+            for (int c = 0; c < Cfg::CH; ++c)
+              *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_async_smem();
+          __syncwarp();
+        }
+        const bool more = i + 1 < span.n;
+        if (more && !wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u)) break;
+        for (int w = 0; w < 2 && ok; ++w) {
+          if (needs(p, rows[w], j0)) {
+            if (!wait(&bar->p_ready[w], seen[w] & 1u)) break;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint64_t dv = sdesc_mn16(smem_addr(sv + s * Cfg::TILE), kKeys * 128);
+#pragma unroll
+              for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                mma_f16_ts(tmem + 256u + static_cast<uint32_t>(w * 128), tmem + static_cast<uint32_t>(w * kKeys + kk * 8),
+                           dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o, seen[w] != 0 || kk != 0 ? 1u : 0u);
+            }
+            __syncwarp();
+            ++seen[w];
+          }
+          if (more && needs(p, rows[w], span.at(i + 1) * kKeys)) scores(w, i + 1);
+        }
+        if (lane == 0 && ok) {
+          mma_commit(&bar->v_empty[s]);
+          if (more) mma_commit(&bar->k_empty[s ^ 1]);
+        }
+      }
+      if (lane == 0 && ok) mma_commit(&bar->o_full);
+    }
+  } else {
+    const int w = (warp - 2) >> 2, q = warp & 3;
+    const int r = q * 32 + lane;                     // row of the tile
+    const int t = t0 + w * p.tokens + r / p.G;       // its token
+    const int head = hk * p.G + r % p.G;
+    const bool mine = r < p.tokens * p.G && t < p.T;
+    const int pos = first + t;
+    const bool live = mine && pos >= 0 && pos < len;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const uint32_t s_at = lane_base + static_cast<uint32_t>(w * kKeys), o_at = lane_base + 256u + static_cast<uint32_t>(w * 128);
+    float m = -INFINITY, l = 0.0f;
+    uint32_t count = 0;
+    bool ok = true;
+    for (int i = 0; i < span.n && ok; ++i) {
+      const int j0 = span.at(i) * kKeys;
+      if (!needs(p, rows[w], j0)) continue;
+      ok = mbar_wait(&bar->s_full[w], count & 1u, &bar->abort_flag, err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, s[g]);
+      tmem_wait_ld();
+      // keys [j0 + from, j0 + to] and those below `sunk` are seen
+      const bool whole = j0 + kKeys - 1 <= rows[w].lo && (j0 > rows[w].hi - p.window || j0 + kKeys <= p.sinks) &&
+                         rows[w].lo == first + t0 + w * p.tokens;  // no row before position 0
+      if (!whole) {
+        const int to = live ? pos - j0 : -1;
+        const int from = pos >= p.window ? pos - p.window + 1 - j0 : -j0;
+        const int sunk = p.sinks - j0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const int j = g * 32 + x;
+            if (!(j <= to && (j >= from || j < sunk))) s[g][x] = 0xff800000u;  // -inf
+          }
+      }
+      float top[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        top[g] = __uint_as_float(s[g][0]);
+#pragma unroll
+        for (int x = 1; x < 32; ++x) top[g] = fmaxf(top[g], __uint_as_float(s[g][x]));
+      }
+      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
+      if (__any_sync(0xffffffffu, peak > m + kLazy)) {  // the first tile of a row among them (m = -inf)
+        const float next = fmaxf(m, peak);
+        const float alpha = next == -INFINITY ? 1.0f : exp2_fast(m - next);
+        l *= alpha;
+        m = next;
+        if (count > 0) {
+          // the scores' commit came after the last P V of this tile: O is at rest
+#pragma unroll
+          for (int g = 0; g < D / 32; ++g) {
+            uint32_t o[32];
+            tmem_ld32(o_at + g * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
+            tmem_st32(o_at + g * 32, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const int j = h * 64 + 2 * x;
+          const float e0 = exp2_fast(fmaf(__uint_as_float(s[j >> 5][j & 31]), p.scale2, -base));
+          const float e1 = exp2_fast(fmaf(__uint_as_float(s[j >> 5][(j & 31) + 1]), p.scale2, -base));
+          sum[x & 3] += e0 + e1;
+          pk[x] = pack2<BF16>(e0, e1);
+        }
+        tmem_st32(s_at + h * 32, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->p_ready[w]);
+      ++count;
+    }
+    if (ok && count > 0) {
+      ok = mbar_wait(&bar->o_full, 0, &bar->abort_flag, err);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok) {
+      const float inv = live && l > 0.0f ? 1.0f / l : 0.0f;
+      uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o_b + static_cast<long long>(t) * p.o_t + head * p.o_h;
+#pragma unroll
+      for (int g = 0; g < D / 32; ++g) {
+        uint32_t o[32];
+        if (count > 0) {
+          tmem_ld32(o_at + g * 32, o);
+          tmem_wait_ld();
+        }
+        if (mine) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (live)
+              v = make_uint4(pack2<BF16>(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv),
+                             pack2<BF16>(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv),
+                             pack2<BF16>(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv),
+                             pack2<BF16>(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv));
+            *reinterpret_cast<uint4*>(dst + g * 32 + x) = v;
+          }
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncwarp();
+  __syncthreads();
+  if (threadIdx.x == 0 && bar->abort_flag) {  // copies in flight land before the CTA leaves
+    const uint64_t c0 = globaltimer_ns();
+    while (globaltimer_ns() - c0 < 50ull * 1000ull * 1000ull) {
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+// A decode step: 16 rows (tokens x grouped heads) against a long cache, bound
+// by the cache's bytes. The seen keys of the row tile are numbered through
+// (sinks, then the window), cut into runs for the CTAs of a cluster and walked
+// in tiles of 64 by cp.async; each of four warps takes 16 keys of a tile with
+// its own running maximum, sum and O (mma.sync m16n8k16: at 16 rows the tensor
+// rate is not the limit, and the 128-row tcgen05 tile would be seven eighths
+// empty). Warps, then CTAs, are joined in a fixed order, through shared memory
+// and the cluster's shared memory: no workspace, the same bits every run.
+constexpr int kRowKeys = 64, kRowStages = 3, kRowThreads = 128;
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 bytes; valid == false writes zeros without reading src.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int D>
+struct RowCfg {
+  static constexpr int TILE = kRowKeys * D * 2;
+  static constexpr int SMEM = kRowStages * 2 * TILE;
+  // after the last tile the ring holds the warps' O [4][16][D], the CTA's O [16][D], maxima and sums
+  static constexpr int OFF_CTA = 4 * 16 * D * 4, OFF_M = OFF_CTA + 16 * D * 4, OFF_L = OFF_M + 4 * 16 * 4,
+                       OFF_CM = OFF_L + 4 * 16 * 4, OFF_CL = OFF_CM + 64;
+  static_assert(OFF_CL + 64 <= SMEM, "the join fits the ring");
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kRowThreads, 2) k_window_rows(const __grid_constant__ WinArgs p) {
+  using Cfg = RowCfg<D>;
+  extern __shared__ __align__(1024) uint8_t ring[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.split, rt = static_cast<int>(blockIdx.x) / p.split;
+  const int hk = blockIdx.y, b = blockIdx.z;
+  griddep_launch();
+  griddep_wait();
+  int first, len;
+  place_of(p, b, first, len);
+  const int row0 = rt * 16, nrows = p.T * p.G;
+  const int t_lo = row0 / p.G, t_hi = min(row0 + 15, nrows - 1) / p.G;
+  const int lo_pos = max(first + t_lo, 0), hi_pos = min(first + t_hi, len - 1);
+  auto out_row = [&](int r) {
+    return static_cast<uint16_t*>(p.out) + b * p.o_b + static_cast<long long>((row0 + r) / p.G) * p.o_t +
+           (hk * p.G + (row0 + r) % p.G) * p.o_h;
+  };
+  if (lo_pos > hi_pos) {  // padding alone: the same in the whole cluster
+    if (rank == 0)
+      for (int x = tid; x < 16 * D / 8; x += kRowThreads) {
+        const int r = x / (D / 8);
+        if (row0 + r < nrows) *reinterpret_cast<uint4*>(out_row(r) + (x % (D / 8)) * 8) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    return;
+  }
+  const int lo = lo_pos >= p.window ? lo_pos - p.window + 1 : 0;
+  const int nsink = min(p.sinks, lo);
+  const int total = nsink + hi_pos - lo + 1;
+  const int tiles = (total + kRowKeys - 1) / kRowKeys;
+  const int i0 = static_cast<int>(static_cast<long long>(rank) * tiles / p.split);
+  const int i1 = static_cast<int>(static_cast<long long>(rank + 1) * tiles / p.split);
+
+  // a thread copies the same 16 bytes of every (128 / CHUNKS)-th row of a tile
+  constexpr int CHUNKS = D / 8, ROWS_STEP = kRowThreads / CHUNKS;
+  const int ch = tid % CHUNKS, crow = tid / CHUNKS;
+  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + b * p.k_b + hk * p.k_h + ch * 8;
+  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + b * p.v_b + hk * p.v_h + ch * 8;
+  const uint32_t ring_at = smem_addr(ring);
+  auto fetch = [&](int i) {
+    const uint32_t at = ring_at + static_cast<uint32_t>(((i - i0) % kRowStages) * 2 * Cfg::TILE);
+#pragma unroll
+    for (int x = 0; x < kRowKeys / ROWS_STEP; ++x) {
+      const int row = crow + x * ROWS_STEP;
+      const int vi = i * kRowKeys + row;
+      const bool valid = vi < total;
+      const long long j = !valid ? 0 : vi < nsink ? vi : lo + vi - nsink;
+      const uint32_t off = static_cast<uint32_t>(row * D * 2 + ((ch ^ (row & 7)) << 4));
+      cp_async16(at + off, kbase + j * p.k_s, valid);
+      cp_async16(at + Cfg::TILE + off, vbase + j * p.v_s, valid);
+    }
+  };
+
+  // Q: the A fragments of 16 rows, straight from global memory
+  const int ra = lane >> 2, rb = ra + 8;
+  uint32_t qf[D / 16][4];
+  {
+    const bool in_a = row0 + ra < nrows, in_b = row0 + rb < nrows;
+    auto q_row = [&](int r) {
+      return static_cast<const uint16_t*>(p.q) + b * p.q_b + static_cast<long long>((row0 + r) / p.G) * p.q_t +
+             (hk * p.G + (row0 + r) % p.G) * p.q_h + (lane & 3) * 2;
+    };
+    const uint16_t* qa = q_row(in_a ? ra : 0);
+    const uint16_t* qb = q_row(in_b ? rb : 0);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qf[ks][0] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16) : 0u;
+      qf[ks][1] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16) : 0u;
+      qf[ks][2] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16 + 8) : 0u;
+      qf[ks][3] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16 + 8) : 0u;
+    }
+  }
+  // positions of this thread's two rows; -1 sees nothing
+  auto pos_of = [&](int r) {
+    const int pos = first + (row0 + r) / p.G;
+    return row0 + r < nrows && pos >= 0 && pos < len ? pos : -1;
+  };
+  const int pos_a = pos_of(ra), pos_b = pos_of(rb);
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[x][e] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+#pragma unroll
+  for (int s = 0; s < kRowStages - 1; ++s) {
+    if (i0 + s < i1) fetch(i0 + s);
+    cp_async_commit();
+  }
+  for (int i = i0; i < i1; ++i) {
+    cp_async_wait<kRowStages - 2>();
+    __syncthreads();
+    if (i + kRowStages - 1 < i1) fetch(i + kRowStages - 1);
+    cp_async_commit();
+    const uint32_t at = ring_at + static_cast<uint32_t>(((i - i0) % kRowStages) * 2 * Cfg::TILE);
+    float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    {
+      const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+      const uint32_t krow = at + static_cast<uint32_t>(key * D * 2);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t kf[4];
+        ldmatrix4(kf, krow + static_cast<uint32_t>((((ks * 2 + ((lane >> 3) & 1)) ^ (key & 7)) << 4)));
+        mma_16816<BF16>(s[0], qf[ks], kf[0], kf[1]);
+        mma_16816<BF16>(s[1], qf[ks], kf[2], kf[3]);
+      }
+    }
+    // c0, c1 belong to row a, c2, c3 to row b
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int vi = i * kRowKeys + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
+        const int j = vi < nsink ? vi : lo + vi - nsink;
+        const int pos = e < 2 ? pos_a : pos_b;
+        const bool seen = vi < total && j <= pos && (pos - j < p.window || j < p.sinks);
+        s[n][e] = seen ? s[n][e] * p.scale2 : -INFINITY;
+      }
+    float alpha[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float next = fmaxf(m[h], top);
+      const float base = next == -INFINITY ? 0.0f : next;
+      alpha[h] = exp2_fast(m[h] - base);
+      m[h] = next;
+      float sum = 0.0f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[n][2 * h + e] = exp2_fast(s[n][2 * h + e] - base);
+          sum += s[n][2 * h + e];
+        }
+      l[h] = l[h] * alpha[h] + sum;
+    }
+    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+      for (int x = 0; x < D / 8; ++x) {
+        o[x][0] *= alpha[0];
+        o[x][1] *= alpha[0];
+        o[x][2] *= alpha[1];
+        o[x][3] *= alpha[1];
+      }
+    }
+    const uint32_t pf[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]), pack2<BF16>(s[1][0], s[1][1]),
+                            pack2<BF16>(s[1][2], s[1][3])};
+    {
+      const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+      const uint32_t vrow = at + Cfg::TILE + static_cast<uint32_t>(key * D * 2);
+#pragma unroll
+      for (int dn = 0; dn < D / 16; ++dn) {
+        uint32_t vf[4];
+        ldmatrix4_trans(vf, vrow + static_cast<uint32_t>((((dn * 2 + (lane >> 4)) ^ (key & 7)) << 4)));
+        mma_16816<BF16>(o[2 * dn], pf, vf[0], vf[1]);
+        mma_16816<BF16>(o[2 * dn + 1], pf, vf[2], vf[3]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // join the warps: each leaves its O, maximum and sum in the ring
+  float* wo = reinterpret_cast<float*>(ring);
+  float* co = reinterpret_cast<float*>(ring + Cfg::OFF_CTA);
+  float* wm = reinterpret_cast<float*>(ring + Cfg::OFF_M);
+  float* wl = reinterpret_cast<float*>(ring + Cfg::OFF_L);
+  float* cm = reinterpret_cast<float*>(ring + Cfg::OFF_CM);
+  float* cl = reinterpret_cast<float*>(ring + Cfg::OFF_CL);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    const int r = ra + 8 * h;
+    if ((lane & 3) == 0) {
+      wm[warp * 16 + r] = m[h];
+      wl[warp * 16 + r] = l[h];
+    }
+#pragma unroll
+    for (int x = 0; x < D / 8; ++x)
+      *reinterpret_cast<float2*>(wo + (warp * 16 + r) * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * h], o[x][2 * h + 1]);
+  }
+  __syncthreads();
+  auto weight = [](float part, float whole) { return part == -INFINITY ? 0.0f : exp2_fast(part - whole); };
+  for (int x = tid; x < 16 * D; x += kRowThreads) {
+    const int r = x / D;
+    const float top = fmaxf(fmaxf(wm[r], wm[16 + r]), fmaxf(wm[32 + r], wm[48 + r]));
+    float acc = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float f = weight(wm[y * 16 + r], top);
+      acc = fmaf(f, wo[y * 16 * D + x], acc);
+      sum = fmaf(f, wl[y * 16 + r], sum);
+    }
+    co[x] = acc;
+    if (x % D == 0) {
+      cm[r] = top;
+      cl[r] = sum;
+    }
+  }
+  if (p.split > 1) cluster_sync_all();
+  else __syncthreads();
+  // then the CTAs: CTA `rank` finishes the pairs of columns rank, rank + split, ...
+  const uint32_t co_at = smem_addr(co), cm_at = smem_addr(cm), cl_at = smem_addr(cl);
+  for (int x = rank * kRowThreads + tid; x < 16 * D / 2; x += p.split * kRowThreads) {
+    const int r = x / (D / 2);
+    if (row0 + r >= nrows) continue;
+    float top = -INFINITY;
+    for (int c = 0; c < p.split; ++c) {
+      uint32_t at;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(cm_at + r * 4), "r"(c));
+      top = fmaxf(top, ld_cluster_f(at));
+    }
+    float a0 = 0.0f, a1 = 0.0f, sum = 0.0f;
+    for (int c = 0; c < p.split; ++c) {
+      uint32_t at_m, at_l, at_o;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(cm_at + r * 4), "r"(c));
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_l) : "r"(cl_at + r * 4), "r"(c));
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(co_at + x * 8), "r"(c));
+      const float f = weight(ld_cluster_f(at_m), top);
+      sum = fmaf(f, ld_cluster_f(at_l), sum);
+      a0 = fmaf(f, ld_cluster_f(at_o), a0);
+      a1 = fmaf(f, ld_cluster_f(at_o + 4), a1);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    *reinterpret_cast<uint32_t*>(out_row(r) + (x % (D / 2)) * 2) = pack2<BF16>(a0 * inv, a1 * inv);
+  }
+  if (p.split > 1) cluster_sync_all();  // a CTA stays until its part has been read
+}
+
+// ------------------------------------------------------------------ host side
+template <int D, bool BF16>
+int launch_tiles(osc_ctx* ctx, const WinArgs& p) {
+  using Cfg = WinCfg<D>;
+  CUtensorMap mQ, mK, mV;
+  const uint32_t box_q[4] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tokens), 1};
+  const uint32_t box_k[4] = {64, kKeys, 1, 1};
+  const uint64_t one = D * 2;  // a stride for axes of length one
+  auto stride = [&](long long elems, int n) { return n > 1 ? static_cast<uint64_t>(elems) * 2 : one; };
+  const uint64_t dq[4] = {D, static_cast<uint64_t>(p.H), static_cast<uint64_t>(p.T), static_cast<uint64_t>(p.B)};
+  const uint64_t sq[3] = {stride(p.q_h, p.H), stride(p.q_t, p.T), stride(p.q_b, p.B)};
+  const uint64_t dk[4] = {D, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.HK), static_cast<uint64_t>(p.B)};
+  const uint64_t sk[3] = {stride(p.k_s, p.S), stride(p.k_h, p.HK), stride(p.k_b, p.B)};
+  const uint64_t sv[3] = {stride(p.v_s, p.S), stride(p.v_h, p.HK), stride(p.v_b, p.B)};
+  const auto type = CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  OSC_TRY(encode_tiled(&mQ, type, 4, p.q, dq, sq, box_q, CU_TENSOR_MAP_SWIZZLE_128B));
+  OSC_TRY(encode_tiled(&mK, type, 4, p.k, dk, sk, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
+  OSC_TRY(encode_tiled(&mV, type, 4, p.v, dk, sv, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
+  OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(k_window_tiles<D, BF16>), Cfg::SMEM));
+  const dim3 grid((p.T + 2 * p.tokens - 1) / (2 * p.tokens), p.HK, p.B);
+  return launch_pdl(ctx, k_window_tiles<D, BF16>, grid, dim3(kWinThreads), Cfg::SMEM, "k_window_tiles", mQ, mK, mV, p,
+                    ctx->d_err);
+}
+
+template <int D, bool BF16>
+int launch_rows(osc_ctx* ctx, const WinArgs& p) {
+  using Cfg = RowCfg<D>;
+  OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(k_window_rows<D, BF16>), Cfg::SMEM));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.row_tiles * p.split), p.HK, p.B);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  prof_begin(ctx);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_window_rows<D, BF16>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "k_window_rows launch");
+  return check_launch(ctx, "k_window_rows");
+}
+
+template <int D, bool BF16>
+int launch(osc_ctx* ctx, WinArgs& p) {
+  const long long rows = static_cast<long long>(p.T) * p.G;
+  if (rows <= 32) {
+    p.row_tiles = static_cast<int>((rows + 15) / 16);
+    // CTAs to fill the SMs twice, each with two tiles of keys at least
+    const long long keys = std::min<long long>(p.S, static_cast<long long>(p.window) + p.T + p.sinks);
+    const long long groups = static_cast<long long>(p.row_tiles) * p.HK * p.B;
+    p.split = 1;
+    while (p.split < 8 && groups * p.split < 2ll * ctx->num_sms && keys > 2ll * p.split * 2 * kRowKeys) p.split *= 2;
+    return launch_rows<D, BF16>(ctx, p);
+  }
+  p.tokens = 128 / p.G;
+  return launch_tiles<D, BF16>(ctx, p);
+}
+
+}  // namespace
+}  // namespace osc
+
+using namespace osc;
+
+extern "C" {
+
+OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const long long* q_strides, const void* k,
+                                 const long long* k_strides, const void* v, const long long* v_strides,
+                                 const int* lengths, const int* starts, int B, int T, int S, int H, int HK, int D,
+                                 int window, int sinks, float scale, void* out, const long long* out_strides) {
+  if (ctx == nullptr) return fail(OSC_EINVAL, "null context");
+  if (dtype != OSC_F16 && dtype != OSC_BF16) return fail(OSC_EINVAL, "osc_attention_window: dtype %d is not f16 or bf16", dtype);
+  if (B < 0 || T < 0 || S <= 0 || H <= 0 || HK <= 0 || T > kFarPos || S > kFarPos)
+    return fail(OSC_EINVAL, "osc_attention_window: bad shape B %d T %d S %d heads %d / %d", B, T, S, H, HK);
+  if (H % HK != 0 || H / HK > 128) return fail(OSC_EINVAL, "osc_attention_window: %d heads over %d key/value heads", H, HK);
+  if (D != 64 && D != 128) return fail(OSC_EUNSUPPORTED, "osc_attention_window: head size %d (64 and 128 are built)", D);
+  if (window < 1 || sinks < 0) return fail(OSC_EINVAL, "osc_attention_window: window %d, sinks %d", window, sinks);
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(OSC_EINVAL, "osc_attention_window: scale %g", static_cast<double>(scale));
+  if (HK > 65535 || B > 65535) return fail(OSC_EINVAL, "osc_attention_window: %d sequences, %d key/value heads: at most 65535", B, HK);
+  if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || out_strides == nullptr)
+    return fail(OSC_EINVAL, "osc_attention_window: null strides");
+  if (B == 0 || T == 0) return OSC_OK;
+  if (q == nullptr || k == nullptr || v == nullptr || out == nullptr || lengths == nullptr)
+    return fail(OSC_EINVAL, "osc_attention_window: null pointer");
+  auto fits = [](const void* at, const long long* s, int n0, int n1, int n2) {
+    const int n[3] = {n0, n1, n2};
+    bool ok = reinterpret_cast<uintptr_t>(at) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (n[i] == 1 || (s[i] >= 0 && s[i] % 8 == 0 && s[i] < (1ll << 39)));
+    return ok;
+  };
+  if (!fits(q, q_strides, B, T, H) || !fits(k, k_strides, B, S, HK) || !fits(v, v_strides, B, S, HK) ||
+      !fits(out, out_strides, B, T, H))
+    return fail(OSC_EINVAL, "osc_attention_window: head rows must start on 16-byte boundaries (strides in multiples of 8 elements)");
+  if (reinterpret_cast<uintptr_t>(lengths) % 4 != 0 || reinterpret_cast<uintptr_t>(starts) % 4 != 0)
+    return fail(OSC_EINVAL, "osc_attention_window: a pointer is not aligned to its type");
+  OSC_TRY(enter(ctx));
+  if (fault_injected("launch")) return fail(OSC_EFAULT_INJECTED, "injected failure (launch)");
+  WinArgs p = {};
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.lengths = lengths;
+  p.starts = starts;
+  p.q_b = q_strides[0], p.q_t = q_strides[1], p.q_h = q_strides[2];
+  p.k_b = k_strides[0], p.k_s = k_strides[1], p.k_h = k_strides[2];
+  p.v_b = v_strides[0], p.v_s = v_strides[1], p.v_h = v_strides[2];
+  p.o_b = out_strides[0], p.o_t = out_strides[1], p.o_h = out_strides[2];
+  p.B = B;
+  p.T = T;
+  p.S = S;
+  p.H = H;
+  p.HK = HK;
+  p.G = H / HK;
+  p.window = window;
+  p.sinks = std::min(sinks, kFarPos);
+  p.scale2 = scale * 1.4426950408889634f;
+  if (D == 64) return dtype == OSC_BF16 ? launch<64, true>(ctx, p) : launch<64, false>(ctx, p);
+  return dtype == OSC_BF16 ? launch<128, true>(ctx, p) : launch<128, false>(ctx, p);
+}
+
+}  // extern "C"

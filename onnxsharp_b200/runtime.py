@@ -402,6 +402,42 @@ def attention(ctx: Context, q, k, v, heads: int, scale: float, mask=None, out_he
     return out
 
 
+def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int | None = None, sinks: int = 0,
+                     starts=None, out=None):
+    """Causal attention over a cache: q [B, T, heads, D], k and v [B, capacity, kv heads, D] (float16 or bfloat16,
+    views with 16-byte-aligned rows), lengths [B] int32 tokens in the cache. Query t stands at lengths - T + t, or at
+    starts + t; it sees the keys up to its own position that lie less than `window` back (None: all) or among the
+    first `sinks`. Padding queries (outside 0 .. lengths - 1) give zeros."""
+    import torch
+
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"attention_window: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    B, T, H, D = (int(x) for x in q.shape)
+    S, HK = int(k.shape[1]), int(k.shape[2])
+    if out is None:
+        out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    if out.shape != q.shape:
+        raise ValueError(f"attention_window: out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+        if not t.is_cuda or t.device.index != ctx.device:
+            raise ValueError(f"attention_window: {name} is on {t.device}, the context on cuda:{ctx.device}")
+        if t.dtype != q.dtype:
+            raise TypeError(f"attention_window: {name} is {t.dtype}, q is {q.dtype}")
+        if t.stride(3) != 1:
+            raise ValueError(f"attention_window: the last axis of {name} must be dense")
+    for name, t in (("lengths", lengths), ("starts", starts)):
+        if t is not None and (not t.is_cuda or t.device.index != ctx.device or t.dtype != torch.int32
+                              or t.numel() != B or not t.is_contiguous()):
+            raise ValueError(f"attention_window: {name} must be {B} adjacent int32 values on cuda:{ctx.device}")
+    if lengths is None:
+        raise ValueError("attention_window: lengths are needed")
+    st = [(C.c_longlong * 3)(*t.stride()[:3]) for t in (q, k, v, out)]
+    call("osc_attention_window", ctx.handle, _lib.dtype_code(q.dtype), ptr(q), st[0], ptr(k), st[1], ptr(v), st[2],
+         ptr(lengths), ptr(starts), B, T, S, H, HK, D, 2**31 - 1 if window is None else int(window), int(sinks),
+         float(scale), ptr(out), st[3])
+    return out
+
+
 def _is_device(x) -> bool:
     return bool(getattr(x, "is_cuda", False))
 
