@@ -90,6 +90,20 @@ struct LinBars {
 };
 static_assert(sizeof(LinBars) <= kSmemTail, "barriers fit the tail");
 
+// Where a walk around the ring stands: counted along, since a division by the
+// number of stages per k-block (some 150 dependent cycles) held every k-block
+// up to 920 cycles, whatever its tile.
+struct RingPos {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 template <int KIND>
 __device__ __forceinline__ void mma_one(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   if constexpr (KIND == LIN_F16) {
@@ -362,51 +376,55 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
   const uint32_t tmem = b->tmem_slot;
   griddep_launch();
 
+  // The producer and the MMA warp walk their loops as whole warps; one lane issues.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool ok = mbar_wait(bar, parity, &b->abort_flag, err);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full0 = PAIR ? mapa_shared(&b->full[0], 0) : 0u;
-      int kc = 0;       // k-blocks issued so far
-      bool waited = false;
-      int pre = 0;      // weight blocks issued before the previous kernel was waited for
-      bool ok = true;
-      auto load_w = [&](int s, int tn, int kb) {
+    const uint32_t full0 = PAIR ? mapa_shared(&b->full[0], 0) : 0u;
+    RingPos at;
+    bool waited = false;
+    int pre = 0;  // weight blocks issued before the previous kernel was waited for, not yet joined by their tokens
+    bool ok = true;
+    auto load_w = [&](int s, int row) {
+      if (elect_one()) {
         uint8_t* st = ring + s * p.stage_bytes;
-        const int row = ((tn * P + rank) * p.num_kb + kb) * kCols;
         if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * (kWBytes + (ATMA ? arows * kKB : 0)));
         if (PAIR) tma_load_2d_pair(st, &mW, full0 + static_cast<uint32_t>(s * 8), 0, row);
         else tma_load_2d(st, &mW, &b->full[s], 0, row);
-      };
-      for (int t = first; t < tiles && ok; t += walkers) {
-        int tm, tn;
-        tile_at(p, t, tm, tn);
-        if (!waited) {
-          // the weights were laid out before this launch was made: their first
-          // blocks travel while the previous kernel on the stream drains
-          pre = min(p.stages, p.num_kb);
-          for (int kb = 0; kb < pre; ++kb) load_w(kb, tn, kb);
-          griddep_wait();
-          waited = true;
+      }
+    };
+    for (int t = first; t < tiles && ok; t += walkers) {
+      int tm, tn;
+      tile_at(p, t, tm, tn);
+      const int w_row = (tn * P + rank) * p.num_kb * kCols, a_row = tm * p.bn + rank * arows;
+      if (!waited) {
+        // the weights were laid out before this launch was made: their first
+        // blocks travel while the previous kernel on the stream drains
+        pre = min(p.stages, p.num_kb);
+        for (int kb = 0; kb < pre; ++kb) load_w(kb, w_row + kb * kCols);
+        griddep_wait();
+        waited = true;
+      }
+      for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
+        const int s = at.s;
+        if (pre > 0) {
+          --pre;
+        } else {
+          ok = wait(&b->empty[s], at.phase ^ 1u);
+          if (!ok) break;
+          load_w(s, w_row + kb * kCols);
         }
-        for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
-          const int s = kc % p.stages;
-          if (kc >= pre) {
-            if (!mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err)) {
-              ok = false;
-              break;
-            }
-            load_w(s, tn, kb);
-          }
-          if (ATMA) {
-            uint8_t* st = ring + s * p.stage_bytes + kWBytes;
-            const int row = tm * p.bn + rank * arows;
-            if (PAIR) tma_load_2d_pair(st, &mA, full0 + static_cast<uint32_t>(s * 8), kb * kKB, row);
-            else tma_load_2d(st, &mA, &b->full[s], kb * kKB, row);
-          }
+        if (ATMA && elect_one()) {
+          uint8_t* st = ring + s * p.stage_bytes + kWBytes;
+          if (PAIR) tma_load_2d_pair(st, &mA, full0 + static_cast<uint32_t>(s * 8), kb * kKB, a_row);
+          else tma_load_2d(st, &mA, &b->full[s], kb * kKB, a_row);
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t own = PAIR ? mapa_shared(b, 0) : 0u, peer = PAIR ? mapa_shared(b, 1) : 0u;
       auto commit = [&](uint64_t* bar) {
         if (PAIR) {
@@ -417,33 +435,33 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
           mma_commit(bar);
         }
       };
-      int kc = 0, it = 0;
+      RingPos at;
+      int it = 0;
       bool ok = true;
       for (int t = first; t < tiles && ok; t += walkers, ++it) {
         const int buf = it & 1;
-        if (!mbar_wait(&b->acc_empty[buf], ((it >> 1) & 1u) ^ 1u, &b->abort_flag, err)) break;
+        if (!wait(&b->acc_empty[buf], ((it >> 1) & 1u) ^ 1u)) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(buf * 256);
-        for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
-          const int s = kc % p.stages;
-          if (!mbar_wait(&b->full[s], (kc / p.stages) & 1u, &b->abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
+          const int s = at.s;
+          ok = wait(&b->full[s], at.phase);
+          if (!ok) break;
           const uint32_t base = smem_addr(ring + s * p.stage_bytes);
           const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
           const int steps = kb + 1 == p.num_kb ? p.last_steps : 4;
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            if (kk < steps) {
-              const uint64_t off = static_cast<uint64_t>(kk * 2);  // 32 bytes of K
-              if (PAIR) mma_two<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-              else mma_one<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-            }
-          commit(&b->empty[s]);
+            for (int kk = 0; kk < 4; ++kk)
+              if (kk < steps) {
+                const uint64_t off = static_cast<uint64_t>(kk * 2);  // 32 bytes of K
+                if (PAIR) mma_two<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+                else mma_one<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+              }
+            commit(&b->empty[s]);
+            if (kb + 1 == p.num_kb) commit(&b->acc_full[buf]);
+          }
         }
-        if (ok) commit(&b->acc_full[buf]);
       }
     }
   } else if (warp < 2 + kEpiWarps) {
@@ -477,14 +495,14 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
   } else {
     griddep_wait();
     const int w = warp - 2 - kEpiWarps;
-    int kc = 0;
+    RingPos at;
     bool ok = true;
     for (int t = first; t < tiles && ok; t += walkers) {
       int tm, tn;
       tile_at(p, t, tm, tn);
-      for (int kb = 0; kb < p.num_kb; ++kb, ++kc) {
-        const int s = kc % p.stages;
-        ok = mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err);
+      for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
+        const int s = at.s;
+        ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         load_rows(p, ring + s * p.stage_bytes + kWBytes, tm * p.bn, arows, kb, w, lane);
@@ -567,37 +585,40 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
   const uint32_t tmem = b->tmem_slot;
   griddep_launch();
 
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool ok = mbar_wait(bar, parity, &b->abort_flag, err);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
   if (warp == 0) {
-    if (lane == 0) {
-      const int pre = min(p.stages, kb1 - kb0);
-      auto load_w = [&](int s, int kb) {
+    const int pre = min(p.stages, kb1 - kb0);
+    const int w_row = (tn * p.num_kb + kb0) * kCols;
+    auto load_w = [&](int s, int kc) {
+      if (elect_one()) {
         mbar_arrive_expect_tx(&b->full[s], kWBytes + (ATMA ? p.bn * kKB : 0));
-        tma_load_2d(ring + s * p.stage_bytes, &mW, &b->full[s], 0, (tn * p.num_kb + kb) * kCols);
-      };
-      for (int kc = 0; kc < pre; ++kc) load_w(kc, kb0 + kc);  // laid out before this launch was made
-      griddep_wait();
-      for (int kc = 0; kc < kb1 - kb0; ++kc) {
-        const int s = kc % p.stages;
-        if (kc >= pre) {
-          if (!mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err)) break;
-          load_w(s, kb0 + kc);
-        }
-        if (ATMA) tma_load_2d(ring + s * p.stage_bytes + kWBytes, &mA, &b->full[s], (kb0 + kc) * kKB, m0);
+        tma_load_2d(ring + s * p.stage_bytes, &mW, &b->full[s], 0, w_row + kc * kCols);
       }
+    };
+    for (int kc = 0; kc < pre; ++kc) load_w(kc, kc);  // laid out before this launch was made
+    griddep_wait();
+    RingPos at;
+    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
+      const int s = at.s;
+      if (kc >= pre) {
+        if (!wait(&b->empty[s], at.phase ^ 1u)) break;
+        load_w(s, kc);
+      }
+      if (ATMA && elect_one())
+        tma_load_2d(ring + s * p.stage_bytes + kWBytes, &mA, &b->full[s], (kb0 + kc) * kKB, m0);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = true;
-      for (int kc = 0; kc < kb1 - kb0; ++kc) {
-        const int s = kc % p.stages;
-        if (!mbar_wait(&b->full[s], (kc / p.stages) & 1u, &b->abort_flag, err)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t base = smem_addr(ring + s * p.stage_bytes);
-        const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
-        const int steps = kb0 + kc + 1 == p.num_kb ? p.last_steps : 4;
+    RingPos at;
+    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
+      const int s = at.s;
+      if (!wait(&b->full[s], at.phase)) break;
+      const uint32_t base = smem_addr(ring + s * p.stage_bytes);
+      const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
+      const int steps = kb0 + kc + 1 == p.num_kb ? p.last_steps : 4;
+      if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           if (kk < steps) {
@@ -605,15 +626,16 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
             mma_one<KIND>(tmem, dw + off, da + off, p.idesc, (kc | kk) != 0 ? 1u : 0u);
           }
         mma_commit(&b->empty[s]);
+        if (kc + 1 == kb1 - kb0) mma_commit(&b->acc_full[0]);
       }
-      if (ok) mma_commit(&b->acc_full[0]);
     }
   } else if (warp >= 2 + kEpiWarps) {
     griddep_wait();
     const int w = warp - 2 - kEpiWarps;
-    for (int kc = 0; kc < kb1 - kb0; ++kc) {
-      const int s = kc % p.stages;
-      const bool ok = mbar_wait(&b->empty[s], ((kc / p.stages) & 1u) ^ 1u, &b->abort_flag, err);
+    RingPos at;
+    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
+      const int s = at.s;
+      const bool ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
       if (!__all_sync(0xffffffffu, ok)) break;
       load_rows(p, ring + s * p.stage_bytes + kWBytes, m0, p.bn, kb0 + kc, w, lane);
       fence_async_smem();
@@ -629,7 +651,6 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
   const bool in = j < p.N;
   const int tokens = min(p.bn, p.M - m0);
   float ws = 0.0f, bs = 0.0f;
-  bool ok = false;
   if (epi) {
     griddep_wait();
     ws = column_scale(p, j, in);
@@ -638,15 +659,14 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
     if (p.split == 1) {
       uint32_t res[16];
       if (p.residual != nullptr) load_residual<16>(p, m0 + half * 16, 1, in ? m0 + tokens : 0, j, res);
-      ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
+      const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
         drain_tile<KIND>(p, lane_base, half, m0, j, ws, bs, res);
       }
     } else {
-      ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
+      const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
+      if (__all_sync(0xffffffffu, ok)) {
         // every block of this CTA has been multiplied: the ring is free and
         // takes the partial sums, [token][column]
         tc_fence_after();

@@ -37,6 +37,22 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// True in one lane of a converged warp, the same one every time. A loop that
+// the whole warp walks, with its TMA, MMA and commit instructions under this
+// predicate, keeps their operands in uniform registers; in a branch taken by
+// one lane each of them is first moved there, one instruction after the other.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one)
+      :
+      : "memory");
+  return one != 0;
+}
+
 // ---------------------------------------------------------------- cp.async
 // 4-byte asynchronous global -> shared copy; valid == false writes a zero
 // (src-size 0) without reading src.
