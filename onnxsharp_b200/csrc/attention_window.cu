@@ -187,39 +187,50 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     span.n = span.sink_tiles + both.hi / kKeys - span.lo_tile + 1;
   }
 
+  // The producer and the MMA warp walk their loops as whole warps; one lane issues.
+  auto wait = [&](uint64_t* m, uint32_t parity) {
+    const bool ok = mbar_wait(m, parity, &bar->abort_flag, err);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
   if (warp == 0) {
-    if (lane == 0 && span.n > 0) {
+    if (span.n > 0) {
       const int tiles_q = t0 + p.tokens < p.T ? 2 : 1;
       const uint32_t box = static_cast<uint32_t>(p.tokens * p.G * 128);
-      mbar_arrive_expect_tx(&bar->q_full, tiles_q * Cfg::CH * box);
-      for (int w = 0; w < tiles_q; ++w)
-        for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full, c * 64, hk * p.G, t0 + w * p.tokens, b);
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&bar->q_full, tiles_q * Cfg::CH * box);
+        for (int w = 0; w < tiles_q; ++w)
+          for (int c = 0; c < Cfg::CH; ++c)
+            tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full, c * 64, hk * p.G, t0 + w * p.tokens, b);
+      }
       for (int i = 0; i < span.n; ++i) {
         const int s = i & 1;
         const uint32_t free = ((i >> 1) & 1u) ^ 1u;
         const int j0 = span.at(i) * kKeys;
-        if (!mbar_wait(&bar->k_empty[s], free, &bar->abort_flag, err)) break;
-        mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
-        for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
-        if (!mbar_wait(&bar->v_empty[s], free, &bar->abort_flag, err)) break;
-        mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
-        for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
+        if (!wait(&bar->k_empty[s], free)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
+          for (int c = 0; c < Cfg::CH; ++c)
+            tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
+        }
+        if (!wait(&bar->v_empty[s], free)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
+          for (int c = 0; c < Cfg::CH; ++c)
+            tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
+        }
       }
     }
   } else if (warp == 1) {
-    // all lanes follow the loop (they clear V rows behind the length); lane 0 issues
+    // (all lanes clear the V rows behind the length)
     constexpr uint32_t fmt = BF16 ? 1u : 0u;
     constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) |
                                  (static_cast<uint32_t>(128 >> 4) << 24);
     constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) |
                                  (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-    bool ok = span.n > 0 && mbar_wait(&bar->q_full, 0, &bar->abort_flag, err);
+    bool ok = span.n > 0 && wait(&bar->q_full, 0);
     uint32_t seen[2] = {0u, 0u};  // PV products issued per tile
     auto scores = [&](int w, int i) {
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t q0 = smem_addr(sq + w * Cfg::TILE), k0 = smem_addr(sk + (i & 1) * Cfg::TILE);
         for (int c = 0; c < Cfg::CH; ++c) {
           const uint64_t dq = sdesc_kmajor_sw128(q0 + c * kKeys * 128), dk = sdesc_kmajor_sw128(k0 + c * kKeys * 128);
@@ -229,21 +240,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         }
         mma_commit(&bar->s_full[w]);
       }
-      __syncwarp();
     };
-    auto wait = [&](uint64_t* m, uint32_t parity) {
-      ok = ok && mbar_wait(m, parity, &bar->abort_flag, err);
-      ok = __all_sync(0xffffffffu, ok);
-      return ok;
-    };
-    if (wait(&bar->k_full[0], 0)) {
+    if (ok && (ok = wait(&bar->k_full[0], 0))) {
       tc_fence_after();
       for (int w = 0; w < 2; ++w)
         if (needs(p, rows[w], span.at(0) * kKeys)) scores(w, 0);
-      if (lane == 0) mma_commit(&bar->k_empty[0]);
+      if (elect_one()) mma_commit(&bar->k_empty[0]);
       for (int i = 0; i < span.n && ok; ++i) {
         const int s = i & 1, j0 = span.at(i) * kKeys;
-        if (!wait(&bar->v_full[s], (i >> 1) & 1u)) break;
+        if (!(ok = wait(&bar->v_full[s], (i >> 1) & 1u))) break;
         if (j0 + kKeys > len) {
           // V rows behind the length: whatever the cache holds there must not meet P's zeros
           for (int x = (len - j0) * 8 + lane; x < kKeys * 8; x += 32)
@@ -253,29 +258,28 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           __syncwarp();
         }
         const bool more = i + 1 < span.n;
-        if (more && !wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u)) break;
+        if (more && !(ok = wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u))) break;
         for (int w = 0; w < 2 && ok; ++w) {
           if (needs(p, rows[w], j0)) {
-            if (!wait(&bar->p_ready[w], seen[w] & 1u)) break;
+            if (!(ok = wait(&bar->p_ready[w], seen[w] & 1u))) break;
             tc_fence_after();
-            if (lane == 0) {
+            if (elect_one()) {
               const uint64_t dv = sdesc_mn16(smem_addr(sv + s * Cfg::TILE), kKeys * 128);
 #pragma unroll
               for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
                 mma_f16_ts(tmem + 256u + static_cast<uint32_t>(w * 128), tmem + static_cast<uint32_t>(w * kKeys + kk * 8),
                            dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o, seen[w] != 0 || kk != 0 ? 1u : 0u);
             }
-            __syncwarp();
             ++seen[w];
           }
           if (more && needs(p, rows[w], span.at(i + 1) * kKeys)) scores(w, i + 1);
         }
-        if (lane == 0 && ok) {
+        if (ok && elect_one()) {
           mma_commit(&bar->v_empty[s]);
           if (more) mma_commit(&bar->k_empty[s ^ 1]);
         }
       }
-      if (lane == 0 && ok) mma_commit(&bar->o_full);
+      if (ok && elect_one()) mma_commit(&bar->o_full);
     }
   } else {
     const int w = (warp - 2) >> 2, q = warp & 3;

@@ -49,7 +49,8 @@ constexpr int kCols = 128;               // output columns of a CTA
 constexpr int kKB = 128;                 // bytes of K in a block: one swizzle row
 constexpr int kWBytes = kCols * kKB;     // 16 KB
 constexpr int kMaxStages = 8;
-constexpr int kEpiWarps = 8;
+constexpr int kTileEpi = 16;             // epilogue warps of k_linear_tiles
+constexpr int kSplitEpi = 8;             // of k_linear_split: two CTAs share an SM
 constexpr int kLoadWarps = 4;            // rows of A that no TMA box fits
 constexpr int kSmemTail = 512;           // barriers
 constexpr int kSmemOne = 232448 - 1024;  // one CTA per SM: the ring and the tail
@@ -70,9 +71,9 @@ struct LinArgs {
   int act;
   int out;                       // osc_dtype of y and the residual
   const void* residual;
-  long long ldr;
+  long long ldr_bytes;
   void* y;
-  long long ldy;
+  long long ldy_bytes;
   const uint8_t* a;              // for rows that no TMA box fits
   long long lda_bytes;
   int k_bytes;
@@ -179,103 +180,135 @@ __device__ __forceinline__ void activate(float (&v)[NV], int act) {
   }
 }
 
-// The residual's raw words of tokens i0 .. i0 + NV - 1 (those below M) at column j.
-template <int NV>
-__device__ __forceinline__ void load_residual(const LinArgs& p, int i0, int step, int i_end, int j, uint32_t (&r)[NV]) {
-  if (p.out == OSC_F32) {
-    const uint32_t* src = static_cast<const uint32_t*>(p.residual) + j;
+// Raw words of column j (already in `base`) at tokens i0, i0 + step, ...: those below i_end.
+template <typename T, int NV>
+__device__ __forceinline__ void load_words(const char* base, long long pitch, int i0, int step, int i_end,
+                                           uint32_t (&r)[NV]) {
+  const char* at = base + i0 * pitch;
+  const long long by = step * pitch;
+  if (i0 + (NV - 1) * step < i_end) {
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      r[t] = i < i_end ? src[static_cast<long long>(i) * p.ldr] : 0u;
-    }
+    for (int t = 0; t < NV; ++t) r[t] = *reinterpret_cast<const T*>(at + t * by);
   } else {
-    const uint16_t* src = static_cast<const uint16_t*>(p.residual) + j;
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      r[t] = i < i_end ? src[static_cast<long long>(i) * p.ldr] : 0u;
-    }
+    for (int t = 0; t < NV; ++t) r[t] = i0 + t * step < i_end ? *reinterpret_cast<const T*>(at + t * by) : T(0);
+  }
+}
+template <typename T, int NV>
+__device__ __forceinline__ void store_words(char* base, long long pitch, int i0, int step, int i_end,
+                                            const uint32_t (&r)[NV]) {
+  char* at = base + i0 * pitch;
+  const long long by = step * pitch;
+  if (i0 + (NV - 1) * step < i_end) {
+#pragma unroll
+    for (int t = 0; t < NV; ++t) *reinterpret_cast<T*>(at + t * by) = static_cast<T>(r[t]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < NV; ++t)
+      if (i0 + t * step < i_end) *reinterpret_cast<T*>(at + t * by) = static_cast<T>(r[t]);
   }
 }
 
-// Scale, bias, activation, residual, rounding and the stores of tokens
-// i0, i0 + step, ... (those below i_end) at column j. The residual's words were
-// loaded by the thread that stores, so y may be the residual's own buffer.
+// What an epilogue thread keeps of its column.
+struct Column {
+  const char* residual;  // null: none
+  char* y;
+  float scale, bias;
+};
+__device__ __forceinline__ Column column_of(const LinArgs& p, int j) {
+  Column c;
+  const bool in = j < p.N;
+  const long long off = static_cast<long long>(j) * (p.out == OSC_F32 ? 4 : 2);
+  c.residual = p.residual != nullptr ? static_cast<const char*>(p.residual) + off : nullptr;
+  c.y = static_cast<char*>(p.y) + off;
+  c.scale = p.w_scale == nullptr ? 1.0f : in ? p.w_scale[p.w_scale_n > 1 ? j : 0] : 0.0f;
+  c.bias = p.bias != nullptr && in ? p.bias[j] : 0.0f;
+  return c;
+}
+
 template <int NV>
-__device__ __forceinline__ void finish(const LinArgs& p, float (&v)[NV], const uint32_t (&res)[NV], int i0, int step,
-                                       int i_end, int j, float ws, float bs) {
-  if (p.a_scale != nullptr) {
+__device__ __forceinline__ void load_residual(const LinArgs& p, const Column& c, int i0, int step, int i_end,
+                                              uint32_t (&r)[NV]) {
+  if (c.residual == nullptr) return;
+  if (p.out == OSC_F32) load_words<uint32_t, NV>(c.residual, p.ldr_bytes, i0, step, i_end, r);
+  else load_words<uint16_t, NV>(c.residual, p.ldr_bytes, i0, step, i_end, r);
+}
+
+// Scale (as[t] * the column's), bias, activation, residual, rounding and the
+// stores of tokens i0, i0 + step, ... (those below i_end). The residual's words
+// were loaded by the thread that stores, so y may be the residual's own buffer.
+template <int NV>
+__device__ __forceinline__ void finish(const LinArgs& p, const Column& c, float (&v)[NV], const float (&as)[NV],
+                                       uint32_t (&res)[NV], int i0, int step, int i_end) {
+  if (p.a_scale != nullptr || p.w_scale != nullptr) {
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      v[t] *= (i < i_end ? p.a_scale[i] : 0.0f) * ws;
-    }
-  } else if (p.w_scale != nullptr) {
-#pragma unroll
-    for (int t = 0; t < NV; ++t) v[t] *= ws;
+    for (int t = 0; t < NV; ++t) v[t] *= as[t] * c.scale;
   }
   if (p.bias != nullptr) {
 #pragma unroll
-    for (int t = 0; t < NV; ++t) v[t] += bs;
+    for (int t = 0; t < NV; ++t) v[t] += c.bias;
   }
   activate<NV>(v, p.act);
   if (p.out == OSC_F32) {
-    float* dst = static_cast<float*>(p.y) + j;
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      const float o = p.residual != nullptr ? v[t] + __uint_as_float(res[t]) : v[t];
-      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = o;
-    }
+    for (int t = 0; t < NV; ++t) res[t] = __float_as_uint(c.residual != nullptr ? v[t] + __uint_as_float(res[t]) : v[t]);
+    store_words<uint32_t, NV>(c.y, p.ldy_bytes, i0, step, i_end, res);
   } else if (p.out == OSC_BF16) {
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.y) + j;
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      const float o = p.residual != nullptr ? v[t] + __uint_as_float(res[t] << 16) : v[t];
-      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = __float2bfloat16_rn(o);
-    }
+    for (int t = 0; t < NV; ++t)
+      res[t] = __bfloat16_as_ushort(__float2bfloat16_rn(c.residual != nullptr ? v[t] + __uint_as_float(res[t] << 16) : v[t]));
+    store_words<uint16_t, NV>(c.y, p.ldy_bytes, i0, step, i_end, res);
   } else {
-    __half* dst = static_cast<__half*>(p.y) + j;
 #pragma unroll
-    for (int t = 0; t < NV; ++t) {
-      const int i = i0 + t * step;
-      const float o =
-          p.residual != nullptr ? v[t] + __half2float(__ushort_as_half(static_cast<unsigned short>(res[t]))) : v[t];
-      if (i < i_end) dst[static_cast<long long>(i) * p.ldy] = __float2half_rn(o);
-    }
+    for (int t = 0; t < NV; ++t)
+      res[t] = __half_as_ushort(__float2half_rn(
+          c.residual != nullptr ? v[t] + __half2float(__ushort_as_half(static_cast<unsigned short>(res[t]))) : v[t]));
+    store_words<uint16_t, NV>(c.y, p.ldy_bytes, i0, step, i_end, res);
   }
-}
-
-__device__ __forceinline__ float column_scale(const LinArgs& p, int j, bool in) {
-  if (p.w_scale == nullptr) return 1.0f;
-  return in ? p.w_scale[p.w_scale_n > 1 ? j : 0] : 0.0f;
 }
 
 // One epilogue warp's share of a tile: its 32 columns (TMEM lanes) and every
-// second group of 16 tokens, the next group's residual in flight while this
-// one is finished.
-template <int KIND>
-__device__ __forceinline__ void drain_tile(const LinArgs& p, uint32_t tmem_lane, int half, int m0, int j, float ws,
-                                           float bs, uint32_t (&res)[16]) {
-  const bool in = j < p.N;
-  const int i_end = in ? min(p.M, m0 + p.bn) : 0;
-  for (int c = half; c * 16 < p.bn; c += 2) {
-    const int i0 = m0 + c * 16;
-    if (i0 >= p.M) break;
-    uint32_t r[16], next[16];
-    tmem_ld16(tmem_lane + c * 16, r);
-    if (p.residual != nullptr) load_residual<16>(p, i0 + 32, 1, i_end, j, next);
-    tmem_wait_ld();
-    float v[16];
-#pragma unroll
-    for (int t = 0; t < 16; ++t) v[t] = sum_of<KIND>(r[t]);
-    finish<16>(p, v, res, i0, 1, i_end, j, ws, bs);
-#pragma unroll
-    for (int t = 0; t < 16; ++t) res[t] = next[t];
+// PARTS-th group of 16 tokens from group `part` on, the next group's residual
+// and row scales in flight while this one is finished. A row scale is loaded by
+// one lane and handed round.
+template <int KIND, int PARTS>
+struct TileShare {
+  uint32_t res[16];
+  float as;
+  __device__ __forceinline__ void fetch(const LinArgs& p, const Column& c, int i0, int i_end, int lane, uint32_t (&r)[16],
+                                        float& a) {
+    load_residual<16>(p, c, i0, 1, i_end, r);
+    a = 1.0f;
+    if (p.a_scale != nullptr) a = i0 + (lane & 15) < p.M ? p.a_scale[i0 + (lane & 15)] : 0.0f;
   }
-}
+  __device__ __forceinline__ void begin(const LinArgs& p, const Column& c, int part, int m0, int j, int lane) {
+    fetch(p, c, m0 + part * 16, j < p.N ? min(p.M, m0 + p.bn) : 0, lane, res, as);
+  }
+  __device__ __forceinline__ void drain(const LinArgs& p, const Column& c, uint32_t tmem_lane, int part, int m0, int j,
+                                        int lane) {
+    const int i_end = j < p.N ? min(p.M, m0 + p.bn) : 0;
+    for (int g = part; g * 16 < p.bn; g += PARTS) {
+      const int i0 = m0 + g * 16;
+      if (i0 >= p.M) break;
+      uint32_t r[16], next[16];
+      float next_as;
+      tmem_ld16(tmem_lane + g * 16, r);
+      fetch(p, c, i0 + PARTS * 16, i_end, lane, next, next_as);
+      tmem_wait_ld();
+      float v[16], a[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) v[t] = sum_of<KIND>(r[t]);
+      if (KIND != LIN_F16) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) a[t] = __shfl_sync(0xffffffffu, as, t);
+      }
+      finish<16>(p, c, v, a, res, i0, 1, i_end);
+#pragma unroll
+      for (int t = 0; t < 16; ++t) res[t] = next[t];
+      as = next_as;
+    }
+  }
+};
 
 // ------------------------------------------------------------------ rows of A that no TMA box fits
 // kLoadWarps warps write the token operand of a stage themselves, in the
@@ -330,7 +363,7 @@ __device__ __forceinline__ void tile_at(const LinArgs& p, int t, int& tm, int& t
 }
 
 template <int KIND, bool PAIR, bool ATMA>
-__global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)), 1)
+__global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps)), 1)
     k_linear_tiles(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, int* __restrict__ err) {
   static_assert(ATMA || !PAIR, "rows without a TMA box are loaded by single CTAs");
@@ -351,7 +384,7 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&b->acc_full[i], 1);
-      mbar_init(&b->acc_empty[i], P * kEpiWarps);
+      mbar_init(&b->acc_empty[i], P * kTileEpi);
     }
     mbar_init(&b->exit_bar, 1);
     b->abort_flag = 0;
@@ -464,8 +497,8 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
         }
       }
     }
-  } else if (warp < 2 + kEpiWarps) {
-    const int q = warp & 3, half = (warp - 2) >> 2;
+  } else if (warp < 2 + kTileEpi) {
+    const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t acce0 = PAIR ? mapa_shared(&b->acc_empty[0], 0) : 0u;
     griddep_wait();
     int it = 0;
@@ -474,17 +507,15 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
       tile_at(p, t, tm, tn);
       const int m0 = tm * p.bn;
       const int j = (tn * P + rank) * kCols + q * 32 + lane;
-      const bool in = j < p.N;
-      const float ws = column_scale(p, j, in);
-      const float bs = p.bias != nullptr && in ? p.bias[j] : 0.0f;
-      uint32_t res[16];
-      if (p.residual != nullptr) load_residual<16>(p, m0 + half * 16, 1, in ? min(p.M, m0 + p.bn) : 0, j, res);
+      const Column c = column_of(p, j);
+      TileShare<KIND, kTileEpi / 4> share;
+      share.begin(p, c, part, m0, j, lane);
       const int buf = it & 1;
       const bool ok = mbar_wait(&b->acc_full[buf], (it >> 1) & 1u, &b->abort_flag, err);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      drain_tile<KIND>(p, tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * 256), half, m0, j,
-                       ws, bs, res);
+      share.drain(p, c, tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * 256), part, m0, j,
+                  lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -494,7 +525,7 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
     }
   } else {
     griddep_wait();
-    const int w = warp - 2 - kEpiWarps;
+    const int w = warp - 2 - kTileEpi;
     RingPos at;
     bool ok = true;
     for (int t = first; t < tiles && ok; t += walkers) {
@@ -550,7 +581,7 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 }
 
 template <int KIND, bool ATMA>
-__global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)), 2)
+__global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)), 2)
     k_linear_split(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, uint32_t tmem_cols, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
@@ -629,9 +660,9 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
         if (kc + 1 == kb1 - kb0) mma_commit(&b->acc_full[0]);
       }
     }
-  } else if (warp >= 2 + kEpiWarps) {
+  } else if (warp >= 2 + kSplitEpi) {
     griddep_wait();
-    const int w = warp - 2 - kEpiWarps;
+    const int w = warp - 2 - kSplitEpi;
     RingPos at;
     for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
       const int s = at.s;
@@ -644,25 +675,24 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
     }
   }
 
-  const bool epi = warp >= 2 && warp < 2 + kEpiWarps;
+  const bool epi = warp >= 2 && warp < 2 + kSplitEpi;
   const int q = warp & 3, half = (warp - 2) >> 2;
   const int col = q * 32 + lane;
   const int j = tn * kCols + col;
   const bool in = j < p.N;
   const int tokens = min(p.bn, p.M - m0);
-  float ws = 0.0f, bs = 0.0f;
+  Column c = {};
   if (epi) {
     griddep_wait();
-    ws = column_scale(p, j, in);
-    bs = p.bias != nullptr && in ? p.bias[j] : 0.0f;
+    c = column_of(p, j);
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     if (p.split == 1) {
-      uint32_t res[16];
-      if (p.residual != nullptr) load_residual<16>(p, m0 + half * 16, 1, in ? m0 + tokens : 0, j, res);
+      TileShare<KIND, kSplitEpi / 4> share;
+      share.begin(p, c, half, m0, j, lane);
       const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
-        drain_tile<KIND>(p, lane_base, half, m0, j, ws, bs, res);
+        share.drain(p, c, lane_base, half, m0, j, lane);
       }
     } else {
       const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
@@ -671,12 +701,12 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
         // takes the partial sums, [token][column]
         tc_fence_after();
         uint32_t* part = reinterpret_cast<uint32_t*>(ring);
-        for (int c = half; c * 16 < tokens; c += 2) {
+        for (int g = half; g * 16 < tokens; g += 2) {
           uint32_t r[16];
-          tmem_ld16(lane_base + c * 16, r);
+          tmem_ld16(lane_base + g * 16, r);
           tmem_wait_ld();
 #pragma unroll
-          for (int t = 0; t < 16; ++t) part[(c * 16 + t) * kCols + col] = r[t];
+          for (int t = 0; t < 16; ++t) part[(g * 16 + t) * kCols + col] = r[t];
         }
       }
     }
@@ -691,20 +721,23 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
       const uint32_t own = smem_addr(ring) + static_cast<uint32_t>(col * 4);
       uint32_t peer[kMaxSplit];
 #pragma unroll
-      for (int c = 0; c < kMaxSplit; ++c)
-        if (c < p.split) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[c]) : "r"(own), "r"(c));
+      for (int x = 0; x < kMaxSplit; ++x)
+        if (x < p.split) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[x]) : "r"(own), "r"(x));
       constexpr int U = 4;
+      const int i_end = in ? m0 + hi : 0;
       for (int i = lo + half; i < hi; i += 2 * U) {
         uint32_t res[U];
-        const int i_end = in ? m0 + hi : 0;
-        if (p.residual != nullptr) load_residual<U>(p, m0 + i, 2, i_end, j, res);
+        load_residual<U>(p, c, m0 + i, 2, i_end, res);
+        float as[U];
+#pragma unroll
+        for (int t = 0; t < U; ++t) as[t] = p.a_scale != nullptr ? p.a_scale[m0 + min(i + 2 * t, hi - 1)] : 1.0f;
         uint32_t acc[U] = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int c = 0; c < kMaxSplit; ++c)
-          if (c < p.split) {
+        for (int x = 0; x < kMaxSplit; ++x)
+          if (x < p.split) {
             uint32_t part[U];
 #pragma unroll
-            for (int t = 0; t < U; ++t) part[t] = ld_cluster(peer[c] + static_cast<uint32_t>(min(i + 2 * t, hi - 1) * kCols * 4));
+            for (int t = 0; t < U; ++t) part[t] = ld_cluster(peer[x] + static_cast<uint32_t>(min(i + 2 * t, hi - 1) * kCols * 4));
 #pragma unroll
             for (int t = 0; t < U; ++t)
               acc[t] = KIND == LIN_I8 ? acc[t] + part[t] : __float_as_uint(__uint_as_float(acc[t]) + __uint_as_float(part[t]));
@@ -712,7 +745,7 @@ __global__ void __launch_bounds__(64 + 32 * (kEpiWarps + (ATMA ? 0 : kLoadWarps)
         float v[U];
 #pragma unroll
         for (int t = 0; t < U; ++t) v[t] = sum_of<KIND>(acc[t]);
-        finish<U>(p, v, res, m0 + i, 2, i_end, j, ws, bs);
+        finish<U>(p, c, v, as, res, m0 + i, 2, i_end);
       }
     }
     __syncwarp();
@@ -826,7 +859,7 @@ int launch_tiles(osc_ctx* ctx, const LinPlan& pl, bool atma, const CUtensorMap& 
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, ctx->num_sms / per) * per));
-  cfg.blockDim = dim3(64 + 32 * (kEpiWarps + (atma ? 0 : kLoadWarps)));
+  cfg.blockDim = dim3(64 + 32 * (kTileEpi + (atma ? 0 : kLoadWarps)));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
@@ -854,7 +887,7 @@ int launch_split(osc_ctx* ctx, bool atma, const CUtensorMap& mW, const CUtensorM
   while (cols < static_cast<uint32_t>(p.bn)) cols *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * p.split));
-  cfg.blockDim = dim3(64 + 32 * (kEpiWarps + (atma ? 0 : kLoadWarps)));
+  cfg.blockDim = dim3(64 + 32 * (kSplitEpi + (atma ? 0 : kLoadWarps)));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
@@ -1024,9 +1057,9 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   p.act = act;
   p.out = out_dtype;
   p.residual = residual;
-  p.ldr = ldr;
+  p.ldr_bytes = ldr * o;
   p.y = y;
-  p.ldy = ldy;
+  p.ldy_bytes = ldy * o;
   p.a = static_cast<const uint8_t*>(a);
   p.lda_bytes = lda * e;
 
