@@ -58,6 +58,26 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// Two FP32 lanes in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -78,11 +98,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // below 2^8, exact in FP32 sums, no overflow in FP16), which after the first
 // tiles hardly happens.
 constexpr int kKeys = 128;
-constexpr int kWinThreads = 64 + 256;
+constexpr int kWinThreads = 128 + 256;  // producer, an MMA warp per tile, one idle; two softmax warpgroups
 constexpr float kLazy = 8.0f;
 
 struct WinBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full;
+  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -148,16 +168,16 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   const int hk = blockIdx.y, b = blockIdx.z;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bar->q_full, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->q_full[i], 1);
       mbar_init(&bar->k_full[i], 1);
-      mbar_init(&bar->k_empty[i], 1);
+      mbar_init(&bar->k_empty[i], 2);
       mbar_init(&bar->v_full[i], 1);
-      mbar_init(&bar->v_empty[i], 1);
+      mbar_init(&bar->v_empty[i], 2);
       mbar_init(&bar->s_full[i], 1);
       mbar_init(&bar->p_ready[i], 4);
+      mbar_init(&bar->o_full[i], 1);
     }
-    mbar_init(&bar->o_full, 1);
     bar->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch(&mQ);
@@ -187,102 +207,109 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     span.n = span.sink_tiles + both.hi / kKeys - span.lo_tile + 1;
   }
 
-  // The producer and the MMA warp walk their loops as whole warps; one lane issues.
+  // The producer and the MMA warps walk their loops as whole warps; one lane issues.
   auto wait = [&](uint64_t* m, uint32_t parity) {
     const bool ok = mbar_wait(m, parity, &bar->abort_flag, err);
     return __all_sync(0xffffffffu, ok) != 0;
   };
   if (warp == 0) {
-    if (span.n > 0) {
-      const int tiles_q = t0 + p.tokens < p.T ? 2 : 1;
-      const uint32_t box = static_cast<uint32_t>(p.tokens * p.G * 128);
-      if (elect_one()) {
-        mbar_arrive_expect_tx(&bar->q_full, tiles_q * Cfg::CH * box);
-        for (int w = 0; w < tiles_q; ++w)
-          for (int c = 0; c < Cfg::CH; ++c)
-            tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full, c * 64, hk * p.G, t0 + w * p.tokens, b);
+    const uint32_t box = static_cast<uint32_t>(p.tokens * p.G * 128);
+    auto load_q = [&](int w) {
+      if (rows[w].lo <= rows[w].hi && elect_one()) {
+        mbar_arrive_expect_tx(&bar->q_full[w], Cfg::CH * box);
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full[w], c * 64, hk * p.G, t0 + w * p.tokens, b);
       }
-      for (int i = 0; i < span.n; ++i) {
-        const int s = i & 1;
-        const uint32_t free = ((i >> 1) & 1u) ^ 1u;
-        const int j0 = span.at(i) * kKeys;
-        if (!wait(&bar->k_empty[s], free)) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
-          for (int c = 0; c < Cfg::CH; ++c)
-            tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
-        }
-        if (!wait(&bar->v_empty[s], free)) break;
-        if (elect_one()) {
-          mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
-          for (int c = 0; c < Cfg::CH; ++c)
-            tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
-        }
+    };
+    for (int i = 0; i < span.n; ++i) {
+      const int s = i & 1;
+      const uint32_t free = ((i >> 1) & 1u) ^ 1u;
+      const int j0 = span.at(i) * kKeys;
+      if (!wait(&bar->k_empty[s], free)) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
+      }
+      if (i == 0) {
+        load_q(0);
+        load_q(1);
+      }
+      if (!wait(&bar->v_empty[s], free)) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c)
+          tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
       }
     }
-  } else if (warp == 1) {
-    // (all lanes clear the V rows behind the length)
+  } else if (warp < 3) {
+    // one tile's products: S of key tile i + 1 follows P V of key tile i (P lies
+    // in S's columns, and the tensor cores take one thread's products in order)
+    const int w = warp - 1;
+    const Rows mine = w == 0 ? rows[0] : rows[1];
     constexpr uint32_t fmt = BF16 ? 1u : 0u;
     constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) |
                                  (static_cast<uint32_t>(128 >> 4) << 24);
     constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) |
                                  (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-    bool ok = span.n > 0 && wait(&bar->q_full, 0);
-    uint32_t seen[2] = {0u, 0u};  // PV products issued per tile
-    auto scores = [&](int w, int i) {
+    const uint32_t s_at = tmem + static_cast<uint32_t>(w * kKeys), o_at = tmem + 256u + static_cast<uint32_t>(w * 128);
+    const uint64_t dq = sdesc_kmajor_sw128(smem_addr(sq + w * Cfg::TILE)), dk0 = sdesc_kmajor_sw128(smem_addr(sk));
+    const uint64_t dv0 = sdesc_mn16(smem_addr(sv), kKeys * 128);
+    constexpr uint64_t kStage = Cfg::TILE >> 4, kColumn = (kKeys * 128) >> 4;
+    auto scores = [&](int s, bool real) {
       if (elect_one()) {
-        const uint32_t q0 = smem_addr(sq + w * Cfg::TILE), k0 = smem_addr(sk + (i & 1) * Cfg::TILE);
-        for (int c = 0; c < Cfg::CH; ++c) {
-          const uint64_t dq = sdesc_kmajor_sw128(q0 + c * kKeys * 128), dk = sdesc_kmajor_sw128(k0 + c * kKeys * 128);
+        if (real) {
+          const uint64_t dk = dk0 + (s != 0 ? kStage : 0);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f16_ss(tmem + static_cast<uint32_t>(w * kKeys), dq + kk * 2, dk + kk * 2, idesc_s, (c | kk) != 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {  // 16 of D: 32 bytes of a 128-byte column
+            const uint64_t off = (kk >> 2) * kColumn + (kk & 3) * 2;
+            mma_f16_ss(s_at, dq + off, dk + off, idesc_s, kk != 0 ? 1u : 0u);
+          }
+          mma_commit(&bar->s_full[w]);
         }
-        mma_commit(&bar->s_full[w]);
+        mma_commit(&bar->k_empty[s]);
       }
     };
-    if (ok && (ok = wait(&bar->k_full[0], 0))) {
-      tc_fence_after();
-      for (int w = 0; w < 2; ++w)
-        if (needs(p, rows[w], span.at(0) * kKeys)) scores(w, 0);
-      if (elect_one()) mma_commit(&bar->k_empty[0]);
-      for (int i = 0; i < span.n && ok; ++i) {
-        const int s = i & 1, j0 = span.at(i) * kKeys;
-        if (!(ok = wait(&bar->v_full[s], (i >> 1) & 1u))) break;
-        if (j0 + kKeys > len) {
-          // V rows behind the length: whatever the cache holds there must not meet P's zeros
-          for (int x = (len - j0) * 8 + lane; x < kKeys * 8; x += 32)
-            for (int c = 0; c < Cfg::CH; ++c)
-              *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_async_smem();
-          __syncwarp();
-        }
-        const bool more = i + 1 < span.n;
-        if (more && !(ok = wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u))) break;
-        for (int w = 0; w < 2 && ok; ++w) {
-          if (needs(p, rows[w], j0)) {
-            if (!(ok = wait(&bar->p_ready[w], seen[w] & 1u))) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t dv = sdesc_mn16(smem_addr(sv + s * Cfg::TILE), kKeys * 128);
-#pragma unroll
-              for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-                mma_f16_ts(tmem + 256u + static_cast<uint32_t>(w * 128), tmem + static_cast<uint32_t>(w * kKeys + kk * 8),
-                           dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o, seen[w] != 0 || kk != 0 ? 1u : 0u);
-            }
-            ++seen[w];
-          }
-          if (more && needs(p, rows[w], span.at(i + 1) * kKeys)) scores(w, i + 1);
-        }
-        if (ok && elect_one()) {
-          mma_commit(&bar->v_empty[s]);
-          if (more) mma_commit(&bar->k_empty[s ^ 1]);
-        }
+    bool ok = span.n > 0;
+    bool now = ok && needs(p, mine, span.at(0) * kKeys);
+    uint32_t done = 0;  // products with V so far
+    if (ok && mine.lo <= mine.hi) ok = wait(&bar->q_full[w], 0);
+    ok = ok && wait(&bar->k_full[0], 0);
+    if (ok) scores(0, now);
+    for (int i = 0; i < span.n && ok; ++i) {
+      const int s = i & 1, j0 = span.at(i) * kKeys;
+      const bool more = i + 1 < span.n;
+      const bool next = more && needs(p, mine, span.at(i + 1) * kKeys);
+      if (!(ok = wait(&bar->v_full[s], (i >> 1) & 1u))) break;
+      if (j0 + kKeys > len) {
+        // V rows behind the length: whatever the cache holds there must not
+        // meet P's zeros (both MMA warps write the same zeros)
+        for (int x = (len - j0) * 8 + lane; x < kKeys * 8; x += 32)
+          for (int c = 0; c < Cfg::CH; ++c)
+            *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
+        __syncwarp();
       }
-      if (ok && elect_one()) mma_commit(&bar->o_full);
+      if (more && !(ok = wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u))) break;
+      if (now && !(ok = wait(&bar->p_ready[w], done & 1u))) break;
+      tc_fence_after();
+      if (elect_one()) {
+        if (now) {
+          const uint64_t dv = dv0 + (s != 0 ? kStage : 0);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+            mma_f16_ts(o_at, s_at + static_cast<uint32_t>(kk * 8), dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o,
+                       done != 0 || kk != 0 ? 1u : 0u);
+        }
+        mma_commit(&bar->v_empty[s]);
+      }
+      if (more) scores(s ^ 1, next);
+      if (now) ++done;
+      now = next;
     }
-  } else {
-    const int w = (warp - 2) >> 2, q = warp & 3;
+    if (ok && span.n > 0 && elect_one()) mma_commit(&bar->o_full[w]);
+  } else if (warp >= 4) {
+    const int w = (warp - 4) >> 2, q = warp & 3;
     const int r = q * 32 + lane;                     // row of the tile
     const int t = t0 + w * p.tokens + r / p.G;       // its token
     const int head = hk * p.G + r % p.G;
@@ -291,48 +318,78 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     const bool live = mine && pos >= 0 && pos < len;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const uint32_t s_at = lane_base + static_cast<uint32_t>(w * kKeys), o_at = lane_base + 256u + static_cast<uint32_t>(w * 128);
-    float m = -INFINITY, l = 0.0f;
+    const Rows rows_w = w == 0 ? rows[0] : rows[1];
+    float m = 0.0f, l = 0.0f;
     uint32_t count = 0;
     bool ok = true;
     for (int i = 0; i < span.n && ok; ++i) {
       const int j0 = span.at(i) * kKeys;
-      if (!needs(p, rows[w], j0)) continue;
+      if (!needs(p, rows_w, j0)) continue;
       ok = mbar_wait(&bar->s_full[w], count & 1u, &bar->abort_flag, err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld32(s_at + g * 32, s[g]);
-      tmem_wait_ld();
       // keys [j0 + from, j0 + to] and those below `sunk` are seen
-      const bool whole = j0 + kKeys - 1 <= rows[w].lo && (j0 > rows[w].hi - p.window || j0 + kKeys <= p.sinks) &&
-                         rows[w].lo == first + t0 + w * p.tokens;  // no row before position 0
-      if (!whole) {
-        const int to = live ? pos - j0 : -1;
-        const int from = pos >= p.window ? pos - p.window + 1 - j0 : -j0;
-        const int sunk = p.sinks - j0;
+      const bool whole = j0 + kKeys - 1 <= rows_w.lo && (j0 > rows_w.hi - p.window || j0 + kKeys <= p.sinks) &&
+                         rows_w.lo == first + t0 + w * p.tokens;  // no row before position 0
+      // the keys of 32-key group g that this row sees, a bit each
+      const int to = live ? pos - j0 : -1;
+      const int from = pos >= p.window ? pos - p.window + 1 - j0 : -j0;
+      const int sunk = p.sinks - j0;
+      auto seen_of = [&](int g) {
+        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // keys 0 .. n - 1
+        return below(to + 1 - g * 32) & (~below(from - g * 32) | below(sunk - g * 32));
+      };
+      auto mask = [&](uint32_t (&s)[32], int g) {
+        if (whole) return;
+        const uint32_t seen = seen_of(g);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int x = 0; x < 32; ++x)
+          if ((seen & (1u << x)) == 0u) s[x] = 0xff800000u;  // -inf
+      };
+      // some row of the tile sees some key of the group (the others' probabilities are 0 without a look)
+      auto wanted = [&](int g) {
+        const int g0 = j0 + g * 32;
+        return g0 <= rows_w.hi && (g0 + 31 > rows_w.lo - p.window || g0 < p.sinks);
+      };
+      // The probabilities are taken relative to the maximum so far (0 before a
+      // row's first key) while this tile's own is still being found; should that
+      // be more than 2^8 above it, or a row's first keys all below it, the
+      // maximum moves and the sweep is repeated: S is intact until P is stored.
+      uint32_t pk[64];
+      float2 sum;
+      for (;;) {
+        const float2 mul = make_float2(p.scale2, p.scale2), off = make_float2(-m, -m);
+        float top = -INFINITY;
+        sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int j = g * 32 + x;
-            if (!(j <= to && (j >= from || j < sunk))) s[g][x] = 0xff800000u;  // -inf
+        for (int g = 0; g < 4; ++g) {
+          if (wanted(g)) {
+            uint32_t s[32];
+            tmem_ld32(s_at + g * 32, s);
+            tmem_wait_ld();
+            mask(s, g);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const float2 a = make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1]));
+              top = fmaxf(top, fmaxf(a.x, a.y));
+              const float2 y = fma2(a, mul, off);
+              const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+              sum = add2(sum, e);
+              pk[g * 16 + x] = pack2<BF16>(e.x, e.y);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) pk[g * 16 + x] = 0u;
           }
-      }
-      float top[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        top[g] = __uint_as_float(s[g][0]);
-#pragma unroll
-        for (int x = 1; x < 32; ++x) top[g] = fmaxf(top[g], __uint_as_float(s[g][x]));
-      }
-      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
-      if (__any_sync(0xffffffffu, peak > m + kLazy)) {  // the first tile of a row among them (m = -inf)
-        const float next = fmaxf(m, peak);
-        const float alpha = next == -INFINITY ? 1.0f : exp2_fast(m - next);
+        }
+        const float peak = top * p.scale2;
+        const bool low = l == 0.0f && peak < m && peak > -INFINITY;
+        if (!__any_sync(0xffffffffu, low || peak > m + kLazy)) break;
+        const float up = low ? peak : fmaxf(m, peak);
+        const float alpha = l > 0.0f ? exp2_fast(m - up) : 1.0f;  // O is zero before a row's first key
         l *= alpha;
-        m = next;
+        m = up;
         if (count > 0) {
           // the scores' commit came after the last P V of this tile: O is at rest
 #pragma unroll
@@ -346,22 +403,14 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           }
         }
       }
-      const float base = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      l += sum.x + sum.y;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
+        uint32_t half[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const int j = h * 64 + 2 * x;
-          const float e0 = exp2_fast(fmaf(__uint_as_float(s[j >> 5][j & 31]), p.scale2, -base));
-          const float e1 = exp2_fast(fmaf(__uint_as_float(s[j >> 5][(j & 31) + 1]), p.scale2, -base));
-          sum[x & 3] += e0 + e1;
-          pk[x] = pack2<BF16>(e0, e1);
-        }
-        tmem_st32(s_at + h * 32, pk);
+        for (int x = 0; x < 32; ++x) half[x] = pk[h * 32 + x];
+        tmem_st32(s_at + h * 32, half);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -369,7 +418,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       ++count;
     }
     if (ok && count > 0) {
-      ok = mbar_wait(&bar->o_full, 0, &bar->abort_flag, err);
+      ok = mbar_wait(&bar->o_full[w], 0, &bar->abort_flag, err);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
