@@ -39,6 +39,7 @@ struct WinArgs {
   int window, sinks;
   float scale2;       // scale * log2(e): softmax in powers of two
   int tokens;         // tokens of a 128-row tile (k_window_tiles)
+  int token_tiles, items;
   int split;          // CTAs that share a row tile's keys (k_window_rows)
   int row_tiles;
 };
@@ -87,22 +88,30 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // ------------------------------------------------------------------ many rows
-// A CTA takes two tiles of 128 rows (2 * tokens consecutive tokens of one
-// key/value head's group) and walks the 128-key tiles that either sees: first
-// the tiles of the sinks, then those of the window. Per tile, S = Q K^T (both
-// from shared memory) goes to TMEM, a thread of the tile's softmax warpgroup
-// reads its row's 128 scores, writes exp2 of them back over S as 16-bit P, and
-// O += P V takes P from TMEM and V as it lies, [key][d] (MN-major). While one
-// tile's scores are in the softmax the tensor cores work on the other's.
-// O is rescaled only when a row's maximum has grown by more than 2^8 (P stays
-// below 2^8, exact in FP32 sums, no overflow in FP16), which after the first
-// tiles hardly happens.
+// Persistent CTAs walk the row tiles: 128 rows (128 / G consecutive tokens of
+// one key/value head's group) against the 128-key tiles that some row sees,
+// first those of the sinks, then those of the window. Per key tile ("step")
+//   MMA warps      one for S = Q K^T, into one of two S buffers, so the softmax
+//                  always has the next scores; one for O += P V, with P from
+//                  TMEM and V as it lies, [key][d] (MN-major). (A single warp
+//                  spends more cycles in its waits than its products take.)
+//   softmax warps  two threads a row, one for the keys 0 .. 63 of every tile, one
+//                  for 64 .. 127, each with a running maximum, sum and O of its
+//                  own that meet once, at the row tile's end: two warps of an SM
+//                  quadrant that need not wait for one another keep the
+//                  special-function unit busy through each other's pauses
+//   producer warps one for Q and K, one for V, two TMA stages each
+// The result goes out by TMA from the Q buffer that it replaces. The
+// special-function units bound it: 128 x 128 exponentials are 1024 cycles of an
+// SM, as are the two products (16 MMAs of 64).
 constexpr int kKeys = 128;
-constexpr int kWinThreads = 128 + 256;  // producer, an MMA warp per tile, one idle; two softmax warpgroups
-constexpr float kLazy = 8.0f;
+constexpr int kWinThreads = 384;  // Q and K producer, S, V producer, P V; 8 softmax warps
+constexpr float kLazy = 8.0f;     // O is rescaled when a maximum has grown by more than 2^8: P stays
+                                  // below that, far from overflow in FP16
 
 struct WinBars {
-  uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_ready[2], o_full, o_empty;
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -111,25 +120,82 @@ template <int D>
 struct WinCfg {
   static constexpr int CH = D / 64;                    // 128-byte columns of a row
   static constexpr int TILE = CH * kKeys * 128;        // a [128][D] tile
-  static constexpr int SMEM = 1024 + 6 * TILE + 512;   // two Q tiles, two stages of K and V
+  static constexpr int BARS = 6 * TILE;                // after two stages of Q, K and V
+  static constexpr int EXCHANGE = BARS + 512;          // maximum and sum: [2 halves][128 rows]
+  static constexpr int SMEM = 1024 + EXCHANGE + 2 * 128 * 8;
 };
+static_assert(sizeof(WinBars) <= 512, "barriers fit");
 
-struct Span {  // the key tiles of a CTA, in order
-  int sink_tiles, lo_tile, n;
-  __device__ __forceinline__ int at(int i) const { return i < sink_tiles ? i : lo_tile + i - sink_tiles; }
+// A row tile: which rows, which key tiles. Every role derives the same from the
+// same item number.
+struct Item {
+  int b, hk, t0;       // sequence, key/value head, first token
+  int first, len;      // position of query 0, the sequence's length
+  int lo, hi;          // live positions of its rows (none: lo > hi)
+  int sink_tiles, lo_tile, n;  // key tiles: sinks', then from lo_tile on; how many
+  __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : lo_tile + i - sink_tiles) * kKeys; }
 };
-
-struct Rows {  // live positions of a 128-row tile: none if lo > hi
-  int lo, hi;
-};
-
-__device__ __forceinline__ Rows live_rows(const WinArgs& p, int first, int len, int t0, int tokens) {
-  return {max(first + t0, 0), min(min(first + t0 + tokens, first + p.T) - 1, len - 1)};
+__device__ __forceinline__ Item item_at(const WinArgs& p, int x) {
+  Item w;
+  const int per = p.HK * p.B;
+  const int tile = x / per, rest = x - tile * per;
+  w.t0 = (p.token_tiles - 1 - tile) * p.tokens;  // late tokens see the most keys of a prompt: they come first
+  w.b = rest / p.HK;
+  w.hk = rest - w.b * p.HK;
+  place_of(p, w.b, w.first, w.len);
+  w.lo = max(w.first + w.t0, 0);
+  w.hi = min(w.first + min(w.t0 + p.tokens, p.T), w.len) - 1;
+  w.sink_tiles = w.lo_tile = w.n = 0;
+  if (w.lo <= w.hi) {
+    w.lo_tile = (w.lo >= p.window ? w.lo - p.window + 1 : 0) / kKeys;
+    w.sink_tiles = min((min(p.sinks, w.hi + 1) + kKeys - 1) / kKeys, w.lo_tile);
+    w.n = w.sink_tiles + w.hi / kKeys - w.lo_tile + 1;
+  }
+  return w;
 }
-// Some row of the tile sees some key of [j0, j0 + 128).
-__device__ __forceinline__ bool needs(const WinArgs& p, const Rows& r, int j0) {
-  return r.lo <= r.hi && j0 <= r.hi && (j0 + kKeys - 1 > r.lo - p.window || j0 < p.sinks);
+// Some row sees some key of the 32 from g0 on. (The others' probabilities are 0 without a look.)
+__device__ __forceinline__ bool wanted(const WinArgs& p, const Item& w, int g0) {
+  return g0 <= w.hi && (g0 + 31 > w.lo - p.window || g0 < p.sinks);
 }
+
+// Some row sees some key of half `part` of the tile at j0.
+__device__ __forceinline__ bool half_wanted(const WinArgs& p, const Item& w, int j0, int part) {
+  return wanted(p, w, j0 + part * 64) || wanted(p, w, j0 + part * 64 + 32);
+}
+
+// Walks the steps of a CTA's items in order.
+struct Steps {
+  Item w;
+  int x, i;        // item, key tile
+  uint32_t item;   // items with keys so far
+  uint32_t step;   // steps so far
+  bool more;
+  __device__ __forceinline__ void seek(const WinArgs& p) {
+    more = false;
+    for (; x < p.items; x += static_cast<int>(gridDim.x)) {
+      w = item_at(p, x);
+      if (w.n > 0) {
+        more = true;
+        break;
+      }
+    }
+  }
+  __device__ __forceinline__ void start(const WinArgs& p) {
+    x = static_cast<int>(blockIdx.x);
+    i = 0;
+    item = step = 0;
+    seek(p);
+  }
+  __device__ __forceinline__ void next(const WinArgs& p) {
+    ++step;
+    if (++i == w.n) {
+      i = 0;
+      ++item;
+      x += static_cast<int>(gridDim.x);
+      seek(p);
+    }
+  }
+};
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -151,33 +217,51 @@ __device__ __forceinline__ uint64_t sdesc_mn16(uint32_t saddr, uint32_t lbo) {
          (static_cast<uint64_t>(2u) << 61);
 }
 
+// The two warps of 32 rows (named barriers 1 .. 4); all softmax warps (5).
+__device__ __forceinline__ void rows_meet(int q) { asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory"); }
+__device__ __forceinline__ void softmax_meet() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_addr(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+// 32 TMEM lanes x 64 columns.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(r);
+  uint32_t(&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(r + 32);
+  tmem_ld32(taddr, a);
+  tmem_ld32(taddr + 32, b);
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kWinThreads, 1)
     k_window_tiles(const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mK,
-                   const __grid_constant__ CUtensorMap mV, const __grid_constant__ WinArgs p, int* __restrict__ err) {
+                   const __grid_constant__ CUtensorMap mV, const __grid_constant__ CUtensorMap mO,
+                   const __grid_constant__ WinArgs p, int* __restrict__ err) {
   using Cfg = WinCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
   uint8_t* sk = smem + 2 * Cfg::TILE;
   uint8_t* sv = smem + 4 * Cfg::TILE;
-  WinBars* bar = reinterpret_cast<WinBars*>(smem + 6 * Cfg::TILE);
+  WinBars* bar = reinterpret_cast<WinBars*>(smem + Cfg::BARS);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // late tokens see the most keys of a prompt: they start first
-  const int t0 = (static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x)) * 2 * p.tokens;
-  const int hk = blockIdx.y, b = blockIdx.z;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar->q_full[i], 1);
+      mbar_init(&bar->q_empty[i], 1);
       mbar_init(&bar->k_full[i], 1);
-      mbar_init(&bar->k_empty[i], 2);
+      mbar_init(&bar->k_empty[i], 1);
       mbar_init(&bar->v_full[i], 1);
-      mbar_init(&bar->v_empty[i], 2);
+      mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 1);
-      mbar_init(&bar->p_ready[i], 4);
-      mbar_init(&bar->o_full[i], 1);
+      mbar_init(&bar->p_ready[i], 8);
     }
+    mbar_init(&bar->o_full, 1);
+    mbar_init(&bar->o_empty, 8);
     bar->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch(&mQ);
@@ -195,257 +279,291 @@ __global__ void __launch_bounds__(kWinThreads, 1)
   griddep_launch();
   griddep_wait();
 
-  int first, len;
-  place_of(p, b, first, len);
-  const Rows rows[2] = {live_rows(p, first, len, t0, p.tokens), live_rows(p, first, len, t0 + p.tokens, p.tokens)};
-  const Rows both = live_rows(p, first, len, t0, 2 * p.tokens);
-  Span span{0, 0, 0};
-  if (both.lo <= both.hi) {
-    const int lo = both.lo >= p.window ? both.lo - p.window + 1 : 0;
-    span.lo_tile = lo / kKeys;
-    span.sink_tiles = min((min(p.sinks, both.hi + 1) + kKeys - 1) / kKeys, span.lo_tile);
-    span.n = span.sink_tiles + both.hi / kKeys - span.lo_tile + 1;
-  }
-
-  // The producer and the MMA warps walk their loops as whole warps; one lane issues.
+  constexpr uint32_t kFmt = BF16 ? 1u : 0u;
+  constexpr uint64_t kStage = Cfg::TILE >> 4;  // in a descriptor's units
+  // Producers and MMA warps walk their loops as whole warps; one lane issues.
   auto wait = [&](uint64_t* m, uint32_t parity) {
-    const bool ok = mbar_wait(m, parity, &bar->abort_flag, err);
+    const bool ok = mbar_wait(m, parity & 1u, &bar->abort_flag, err);
     return __all_sync(0xffffffffu, ok) != 0;
   };
   if (warp == 0) {
     const uint32_t box = static_cast<uint32_t>(p.tokens * p.G * 128);
-    auto load_q = [&](int w) {
-      if (rows[w].lo <= rows[w].hi && elect_one()) {
-        mbar_arrive_expect_tx(&bar->q_full[w], Cfg::CH * box);
-        for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sq + w * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full[w], c * 64, hk * p.G, t0 + w * p.tokens, b);
+    Steps at;
+    for (at.start(p); at.more; at.next(p)) {
+      if (at.i == 0) {
+        const int u = at.item & 1;
+        if (!wait(&bar->q_empty[u], (at.item >> 1) ^ 1u)) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&bar->q_full[u], Cfg::CH * box);
+          for (int c = 0; c < Cfg::CH; ++c)
+            tma_load_4d(sq + u * Cfg::TILE + c * kKeys * 128, &mQ, &bar->q_full[u], c * 64, at.w.hk * p.G, at.w.t0, at.w.b);
+        }
       }
-    };
-    for (int i = 0; i < span.n; ++i) {
-      const int s = i & 1;
-      const uint32_t free = ((i >> 1) & 1u) ^ 1u;
-      const int j0 = span.at(i) * kKeys;
-      if (!wait(&bar->k_empty[s], free)) break;
+      const int s = at.step & 1;
+      if (!wait(&bar->k_empty[s], (at.step >> 1) ^ 1u)) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&bar->k_full[s], Cfg::TILE);
         for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, j0, hk, b);
+          tma_load_4d(sk + s * Cfg::TILE + c * kKeys * 128, &mK, &bar->k_full[s], c * 64, at.w.key0(at.i), at.w.hk, at.w.b);
       }
-      if (i == 0) {
-        load_q(0);
-        load_q(1);
-      }
-      if (!wait(&bar->v_empty[s], free)) break;
+    }
+  } else if (warp == 2) {
+    Steps at;
+    for (at.start(p); at.more; at.next(p)) {
+      const int s = at.step & 1;
+      if (!wait(&bar->v_empty[s], (at.step >> 1) ^ 1u)) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&bar->v_full[s], Cfg::TILE);
         for (int c = 0; c < Cfg::CH; ++c)
-          tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, j0, hk, b);
+          tma_load_4d(sv + s * Cfg::TILE + c * kKeys * 128, &mV, &bar->v_full[s], c * 64, at.w.key0(at.i), at.w.hk, at.w.b);
       }
     }
-  } else if (warp < 3) {
-    // one tile's products: S of key tile i + 1 follows P V of key tile i (P lies
-    // in S's columns, and the tensor cores take one thread's products in order)
-    const int w = warp - 1;
-    const Rows mine = w == 0 ? rows[0] : rows[1];
-    constexpr uint32_t fmt = BF16 ? 1u : 0u;
-    constexpr uint32_t idesc_s = (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) |
-                                 (static_cast<uint32_t>(128 >> 4) << 24);
-    constexpr uint32_t idesc_o = (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 16) |
-                                 (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-    const uint32_t s_at = tmem + static_cast<uint32_t>(w * kKeys), o_at = tmem + 256u + static_cast<uint32_t>(w * 128);
-    const uint64_t dq = sdesc_kmajor_sw128(smem_addr(sq + w * Cfg::TILE)), dk0 = sdesc_kmajor_sw128(smem_addr(sk));
-    const uint64_t dv0 = sdesc_mn16(smem_addr(sv), kKeys * 128);
-    constexpr uint64_t kStage = Cfg::TILE >> 4, kColumn = (kKeys * 128) >> 4;
-    auto scores = [&](int s, bool real) {
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (static_cast<uint32_t>(kKeys >> 3) << 17) |
+                               (static_cast<uint32_t>(128 >> 4) << 24);
+    const uint64_t dq0 = sdesc_kmajor_sw128(smem_addr(sq)), dk0 = sdesc_kmajor_sw128(smem_addr(sk));
+    Steps at;
+    for (at.start(p); at.more; at.next(p)) {
+      const int s = at.step & 1, u = at.item & 1;
+      if (at.i == 0 && !wait(&bar->q_full[u], at.item >> 1)) break;
+      if (!wait(&bar->k_full[s], at.step >> 1)) break;
+      // P of the step before last lies in these columns until its product is done
+      if (!wait(&bar->v_empty[s], (at.step >> 1) ^ 1u)) break;
+      tc_fence_after();
       if (elect_one()) {
-        if (real) {
-          const uint64_t dk = dk0 + (s != 0 ? kStage : 0);
+        const uint64_t dq = dq0 + (u != 0 ? kStage : 0), dk = dk0 + (s != 0 ? kStage : 0);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {  // 16 of D: 32 bytes of a 128-byte column
-            const uint64_t off = (kk >> 2) * kColumn + (kk & 3) * 2;
-            mma_f16_ss(s_at, dq + off, dk + off, idesc_s, kk != 0 ? 1u : 0u);
-          }
-          mma_commit(&bar->s_full[w]);
+        for (int kk = 0; kk < D / 16; ++kk) {  // 16 of D: 32 bytes of a 128-byte column
+          const uint64_t off = (kk >> 2) * ((kKeys * 128) >> 4) + (kk & 3) * 2;
+          mma_f16_ss(tmem + static_cast<uint32_t>(s * kKeys), dq + off, dk + off, idesc, kk != 0 ? 1u : 0u);
         }
+        mma_commit(&bar->s_full[s]);
         mma_commit(&bar->k_empty[s]);
       }
-    };
-    bool ok = span.n > 0;
-    bool now = ok && needs(p, mine, span.at(0) * kKeys);
-    uint32_t done = 0;  // products with V so far
-    if (ok && mine.lo <= mine.hi) ok = wait(&bar->q_full[w], 0);
-    ok = ok && wait(&bar->k_full[0], 0);
-    if (ok) scores(0, now);
-    for (int i = 0; i < span.n && ok; ++i) {
-      const int s = i & 1, j0 = span.at(i) * kKeys;
-      const bool more = i + 1 < span.n;
-      const bool next = more && needs(p, mine, span.at(i + 1) * kKeys);
-      if (!(ok = wait(&bar->v_full[s], (i >> 1) & 1u))) break;
-      if (j0 + kKeys > len) {
-        // V rows behind the length: whatever the cache holds there must not
-        // meet P's zeros (both MMA warps write the same zeros)
-        for (int x = (len - j0) * 8 + lane; x < kKeys * 8; x += 32)
+    }
+  } else if (warp == 3) {
+    constexpr uint32_t idesc = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) |
+                               (static_cast<uint32_t>(128 >> 4) << 24);
+    const uint64_t dv0 = sdesc_mn16(smem_addr(sv), kKeys * 128);
+    bool begun[2] = {false, false};  // this item's O of each half has been written
+    Steps at;
+    for (at.start(p); at.more; at.next(p)) {
+      const int s = at.step & 1, j0 = at.w.key0(at.i);
+      if (!wait(&bar->v_full[s], at.step >> 1)) break;
+      if (j0 + kKeys > at.w.len) {
+        // V rows behind the length: whatever the cache holds there must not meet P's zeros
+        for (int x = (at.w.len - j0) * 8 + lane; x < kKeys * 8; x += 32)
           for (int c = 0; c < Cfg::CH; ++c)
             *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_async_smem();
         __syncwarp();
       }
-      if (more && !(ok = wait(&bar->k_full[s ^ 1], ((i + 1) >> 1) & 1u))) break;
-      if (now && !(ok = wait(&bar->p_ready[w], done & 1u))) break;
+      if (at.i == 0) {
+        begun[0] = begun[1] = false;
+        if (!wait(&bar->o_empty, at.item ^ 1u)) break;
+      }
+      const bool half[2] = {half_wanted(p, at.w, j0, 0), half_wanted(p, at.w, j0, 1)};
+      if (!wait(&bar->p_ready[s], at.step >> 1)) break;
       tc_fence_after();
       if (elect_one()) {
-        if (now) {
-          const uint64_t dv = dv0 + (s != 0 ? kStage : 0);
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-            mma_f16_ts(o_at, s_at + static_cast<uint32_t>(kk * 8), dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_o,
-                       done != 0 || kk != 0 ? 1u : 0u);
+        for (int part = 0; part < 2; ++part) {
+          if (!half[part]) continue;
+          const uint64_t dv = dv0 + (s != 0 ? kStage : 0) + static_cast<uint64_t>(part * (64 * 128 >> 4));
+          const uint32_t o_at = tmem + 256u + static_cast<uint32_t>(part * 128);
+          const uint32_t p_at = tmem + static_cast<uint32_t>(s * kKeys + part * 64);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+            mma_f16_ts(o_at, p_at + static_cast<uint32_t>(kk * 8), dv + static_cast<uint64_t>(kk * (2048 >> 4)), idesc,
+                       begun[part] || kk != 0 ? 1u : 0u);
         }
         mma_commit(&bar->v_empty[s]);
+        if (at.i + 1 == at.w.n) mma_commit(&bar->o_full);
       }
-      if (more) scores(s ^ 1, next);
-      if (now) ++done;
-      now = next;
+      begun[0] = begun[0] || half[0];
+      begun[1] = begun[1] || half[1];
     }
-    if (ok && span.n > 0 && elect_one()) mma_commit(&bar->o_full[w]);
   } else if (warp >= 4) {
-    const int w = (warp - 4) >> 2, q = warp & 3;
-    const int r = q * 32 + lane;                     // row of the tile
-    const int t = t0 + w * p.tokens + r / p.G;       // its token
-    const int head = hk * p.G + r % p.G;
-    const bool mine = r < p.tokens * p.G && t < p.T;
-    const int pos = first + t;
-    const bool live = mine && pos >= 0 && pos < len;
+    const int part = (warp - 4) >> 2, q = warp & 3;
+    const int r = q * 32 + lane;  // row of the tile
+    const int row_token = r / p.G;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t s_at = lane_base + static_cast<uint32_t>(w * kKeys), o_at = lane_base + 256u + static_cast<uint32_t>(w * 128);
-    const Rows rows_w = w == 0 ? rows[0] : rows[1];
-    float m = 0.0f, l = 0.0f;
-    uint32_t count = 0;
-    bool ok = true;
-    for (int i = 0; i < span.n && ok; ++i) {
-      const int j0 = span.at(i) * kKeys;
-      if (!needs(p, rows_w, j0)) continue;
-      ok = mbar_wait(&bar->s_full[w], count & 1u, &bar->abort_flag, err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      // keys [j0 + from, j0 + to] and those below `sunk` are seen
-      const bool whole = j0 + kKeys - 1 <= rows_w.lo && (j0 > rows_w.hi - p.window || j0 + kKeys <= p.sinks) &&
-                         rows_w.lo == first + t0 + w * p.tokens;  // no row before position 0
-      // the keys of 32-key group g that this row sees, a bit each
-      const int to = live ? pos - j0 : -1;
-      const int from = pos >= p.window ? pos - p.window + 1 - j0 : -j0;
-      const int sunk = p.sinks - j0;
-      auto seen_of = [&](int g) {
-        auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // keys 0 .. n - 1
-        return below(to + 1 - g * 32) & (~below(from - g * 32) | below(sunk - g * 32));
-      };
-      auto mask = [&](uint32_t (&s)[32], int g) {
-        if (whole) return;
-        const uint32_t seen = seen_of(g);
-#pragma unroll
-        for (int x = 0; x < 32; ++x)
-          if ((seen & (1u << x)) == 0u) s[x] = 0xff800000u;  // -inf
-      };
-      // some row of the tile sees some key of the group (the others' probabilities are 0 without a look)
-      auto wanted = [&](int g) {
-        const int g0 = j0 + g * 32;
-        return g0 <= rows_w.hi && (g0 + 31 > rows_w.lo - p.window || g0 < p.sinks);
-      };
-      // The probabilities are taken relative to the maximum so far (0 before a
-      // row's first key) while this tile's own is still being found; should that
-      // be more than 2^8 above it, or a row's first keys all below it, the
-      // maximum moves and the sweep is repeated: S is intact until P is stored.
-      uint32_t pk[64];
-      float2 sum;
-      for (;;) {
-        const float2 mul = make_float2(p.scale2, p.scale2), off = make_float2(-m, -m);
-        float top = -INFINITY;
-        sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (wanted(g)) {
-            uint32_t s[32];
-            tmem_ld32(s_at + g * 32, s);
+    const uint32_t o_own = lane_base + 256u + static_cast<uint32_t>(part * 128);
+    float2* exchange = reinterpret_cast<float2*>(smem + Cfg::EXCHANGE) + r;
+    uint32_t item = 0, step = 0;
+    bool ok = true;       // after a wait that ran out the meetings go on, over whatever TMEM holds, and nothing is stored
+    int unreleased = -1;  // Q buffer that still holds a result on its way out
+    auto release = [&]() {  // warp 4, lane by election: the thread that issued the stores
+      if (unreleased >= 0 && warp == 4 && elect_one()) {
+        bulk_wait_read_all();
+        mbar_arrive(&bar->q_empty[unreleased]);
+      }
+      unreleased = -1;
+    };
+    for (int x = static_cast<int>(blockIdx.x); x < p.items; x += static_cast<int>(gridDim.x)) {
+      const Item w = item_at(p, x);
+      const int t = w.t0 + row_token, pos = w.first + t;
+      const bool mine = r < p.tokens * p.G && t < p.T;
+      const bool live = mine && pos >= 0 && pos < w.len;
+      float m = 0.0f, l = 0.0f;
+      bool seen = false;     // the row has had a key of this half
+      int had = 0;           // steps of this item that wanted this half
+      uint32_t s[64];
+      bool loaded = false;   // the scores of the step at hand are on their way to s
+      for (int i = 0; i < w.n; ++i, ++step) {
+        const int j0 = w.key0(i);
+        const uint32_t s_at = lane_base + static_cast<uint32_t>((step & 1u) * kKeys + part * 64);
+        // both halves take part in every step: the scores after next wait for both
+        if (!loaded) {
+          if (ok) ok = wait(&bar->s_full[step & 1u], step >> 1);
+          tc_fence_after();
+        }
+        if (half_wanted(p, w, j0, part)) {
+          if (!loaded) tmem_ld64(s_at, s);
+          loaded = false;
+          // every row sees every key of the half
+          const int h0 = j0 + part * 64;
+          const bool whole = h0 + 63 <= w.lo && (h0 > w.hi - p.window || h0 + 64 <= p.sinks) && w.lo == w.first + w.t0;
+          // The probabilities are taken relative to the maximum so far (0 before a
+          // row's first key) while this tile's own is still being found; should that
+          // be more than 2^8 above it, or a row's first keys all below it, the
+          // maximum moves and the sweep is repeated: S is intact until P is stored.
+          uint32_t pk[32];
+          float2 sum;
+          for (int again = 0; again < 3; ++again) {  // the second sweep passes
+            const float2 mul = make_float2(p.scale2, p.scale2), off = make_float2(-m, -m);
+            float top = -INFINITY;
+            sum = make_float2(0.0f, 0.0f);
             tmem_wait_ld();
-            mask(s, g);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const float2 a = make_float2(__uint_as_float(s[2 * x]), __uint_as_float(s[2 * x + 1]));
-              top = fmaxf(top, fmaxf(a.x, a.y));
-              const float2 y = fma2(a, mul, off);
-              const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-              sum = add2(sum, e);
-              pk[g * 16 + x] = pack2<BF16>(e.x, e.y);
+            for (int h = 0; h < 2; ++h) {
+              const int g0 = h0 + h * 32;
+              if (wanted(p, w, g0)) {
+                if (!whole) {
+                  // a bit for each key that this row sees: those up to its own position, from the window's start or among the sinks
+                  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // keys 0 .. n - 1
+                  const int to = live ? pos - g0 : -1;
+                  const int from = pos >= p.window ? pos - p.window + 1 - g0 : 0;
+                  const uint32_t bits = below(to + 1) & (~below(from) | below(p.sinks - g0));
+#pragma unroll
+                  for (int y = 0; y < 32; ++y)
+                    if ((bits & (1u << y)) == 0u) s[h * 32 + y] = 0xff800000u;  // -inf
+                }
+#pragma unroll
+                for (int y = 0; y < 16; ++y) {
+                  const float2 a = make_float2(__uint_as_float(s[h * 32 + 2 * y]), __uint_as_float(s[h * 32 + 2 * y + 1]));
+                  top = fmaxf(top, fmaxf(a.x, a.y));
+                  const float2 z = fma2(a, mul, off);
+                  const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+                  sum = add2(sum, e);
+                  pk[h * 16 + y] = pack2<BF16>(e.x, e.y);
+                }
+              } else {
+#pragma unroll
+                for (int y = 0; y < 16; ++y) pk[h * 16 + y] = 0u;
+              }
             }
-          } else {
+            const float peak = top * p.scale2;
+            const bool low = !seen && peak < m && peak > -INFINITY;
+            if (!__any_sync(0xffffffffu, low || peak > m + kLazy)) {
+              seen = seen || peak > -INFINITY;
+              break;
+            }
+            const float up = low ? peak : fmaxf(m, peak);
+            const float alpha = seen ? exp2_fast(m - up) : 1.0f;  // O is zero before a row's first key
+            l *= alpha;
+            m = up;
+            if (had > 0) {
+              // O is at rest once the last step's product is done: this step's waits for P
+              const uint32_t last = step - 1u;
+              if (ok) ok = wait(&bar->v_empty[last & 1u], last >> 1);
+              tc_fence_after();
 #pragma unroll
-            for (int x = 0; x < 16; ++x) pk[g * 16 + x] = 0u;
+              for (int g = 0; g < D / 32; ++g) {
+                uint32_t o[32];
+                tmem_ld32(o_own + g * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+                tmem_st32(o_own + g * 32, o);
+              }
+            }
+            tmem_ld64(s_at, s);
           }
-        }
-        const float peak = top * p.scale2;
-        const bool low = l == 0.0f && peak < m && peak > -INFINITY;
-        if (!__any_sync(0xffffffffu, low || peak > m + kLazy)) break;
-        const float up = low ? peak : fmaxf(m, peak);
-        const float alpha = l > 0.0f ? exp2_fast(m - up) : 1.0f;  // O is zero before a row's first key
-        l *= alpha;
-        m = up;
-        if (count > 0) {
-          // the scores' commit came after the last P V of this tile: O is at rest
-#pragma unroll
-          for (int g = 0; g < D / 32; ++g) {
-            uint32_t o[32];
-            tmem_ld32(o_at + g * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * alpha);
-            tmem_st32(o_at + g * 32, o);
+          l += sum.x + sum.y;
+          tmem_st32(s_at, pk);
+          ++had;
+          if (i + 1 < w.n && half_wanted(p, w, w.key0(i + 1), part)) {
+            const uint32_t next = step + 1u;
+            if (ok) ok = wait(&bar->s_full[next & 1u], next >> 1);
+            tc_fence_after();
+            tmem_ld64(lane_base + static_cast<uint32_t>((next & 1u) * kKeys + part * 64), s);
+            loaded = true;
           }
+          tmem_wait_st();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->p_ready[step & 1u]);
+        if (i == 0) release();
       }
-      l += sum.x + sum.y;
+      // the row tile is done: join the halves, through the Q buffer, out
+      if (w.n > 0) {
+        exchange[part * 128] = make_float2(had > 0 ? m : -INFINITY, l);
+        rows_meet(q);
+        const float2 his = exchange[(part ^ 1) * 128];
+        if (ok) ok = wait(&bar->o_full, item);
+        tc_fence_after();
+        // weights of the halves' O; a half without a key has l = 0
+        const float top = l > 0.0f ? (his.y > 0.0f ? fmaxf(m, his.x) : m) : his.x;
+        const float mine_w = l > 0.0f ? exp2_fast(m - top) : 0.0f, his_w = his.y > 0.0f ? exp2_fast(his.x - top) : 0.0f;
+        const float total = l * mine_w + his.y * his_w;
+        const float inv = live && total > 0.0f ? 1.0f / total : 0.0f;
+        const float f_mine = mine_w * inv, f_his = his_w * inv;
+        const uint32_t o_his = lane_base + 256u + static_cast<uint32_t>((part ^ 1) * 128);
+        uint8_t* stage = sq + (item & 1u) * Cfg::TILE;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t half[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) half[x] = pk[h * 32 + x];
-        tmem_st32(s_at + h * 32, half);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->p_ready[w]);
-      ++count;
-    }
-    if (ok && count > 0) {
-      ok = mbar_wait(&bar->o_full[w], 0, &bar->abort_flag, err);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    if (ok) {
-      const float inv = live && l > 0.0f ? 1.0f / l : 0.0f;
-      uint16_t* dst = static_cast<uint16_t*>(p.out) + b * p.o_b + static_cast<long long>(t) * p.o_t + head * p.o_h;
-#pragma unroll
-      for (int g = 0; g < D / 32; ++g) {
-        uint32_t o[32];
-        if (count > 0) {
-          tmem_ld32(o_at + g * 32, o);
+        for (int g = 0; g < D / 32; ++g) {
+          const int c0 = part * (D / 2) + g * 16;  // this thread's columns of the result
+          uint32_t a[16], c[16];
+          tmem_ld16(o_own + static_cast<uint32_t>(c0), a);
+          tmem_ld16(o_his + static_cast<uint32_t>(c0), c);
           tmem_wait_ld();
-        }
-        if (mine) {
+          float o[16];
 #pragma unroll
-          for (int x = 0; x < 32; x += 8) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (live)
-              v = make_uint4(pack2<BF16>(__uint_as_float(o[x]) * inv, __uint_as_float(o[x + 1]) * inv),
-                             pack2<BF16>(__uint_as_float(o[x + 2]) * inv, __uint_as_float(o[x + 3]) * inv),
-                             pack2<BF16>(__uint_as_float(o[x + 4]) * inv, __uint_as_float(o[x + 5]) * inv),
-                             pack2<BF16>(__uint_as_float(o[x + 6]) * inv, __uint_as_float(o[x + 7]) * inv));
-            *reinterpret_cast<uint4*>(dst + g * 32 + x) = v;
+          for (int y = 0; y < 16; ++y) {
+            // selected, not multiplied away: a half without a product was never written
+            const float own = f_mine > 0.0f ? __uint_as_float(a[y]) * f_mine : 0.0f;
+            o[y] = f_his > 0.0f ? fmaf(__uint_as_float(c[y]), f_his, own) : own;
           }
+          const int col = (c0 >> 6) * kKeys * 128, chunk0 = (c0 & 63) >> 3;
+#pragma unroll
+          for (int y = 0; y < 16; y += 8)
+            *reinterpret_cast<uint4*>(stage + col + r * 128 + (((chunk0 + (y >> 3)) ^ (r & 7)) << 4)) =
+                make_uint4(pack2<BF16>(o[y], o[y + 1]), pack2<BF16>(o[y + 2], o[y + 3]), pack2<BF16>(o[y + 4], o[y + 5]),
+                           pack2<BF16>(o[y + 6], o[y + 7]));
         }
+        tc_fence_before();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar->o_empty);
+        release();  // (an item of one step that this half did not want)
+        softmax_meet();
+        if (warp == 4 && elect_one()) {
+          if (ok)
+            for (int c = 0; c < Cfg::CH; ++c)
+              tma_store_4d(&mO, stage + c * kKeys * 128, c * 64, w.hk * p.G, w.t0, w.b);
+          bulk_commit();
+        }
+        unreleased = static_cast<int>(item & 1u);
+        ++item;
+      } else if (mine) {  // padding alone
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + w.b * p.o_b + static_cast<long long>(t) * p.o_t +
+                        (w.hk * p.G + r % p.G) * p.o_h + part * (D / 2);
+        for (int y = 0; y < D / 2; y += 8) *reinterpret_cast<uint4*>(dst + y) = make_uint4(0u, 0u, 0u, 0u);
       }
     }
+    if (warp == 4 && elect_one()) bulk_wait_all();
     tc_fence_before();
   }
   __syncwarp();
@@ -756,7 +874,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) k_window_rows(const __grid_con
 template <int D, bool BF16>
 int launch_tiles(osc_ctx* ctx, const WinArgs& p) {
   using Cfg = WinCfg<D>;
-  CUtensorMap mQ, mK, mV;
+  CUtensorMap mQ, mK, mV, mO;
   const uint32_t box_q[4] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tokens), 1};
   const uint32_t box_k[4] = {64, kKeys, 1, 1};
   const uint64_t one = D * 2;  // a stride for axes of length one
@@ -765,14 +883,15 @@ int launch_tiles(osc_ctx* ctx, const WinArgs& p) {
   const uint64_t sq[3] = {stride(p.q_h, p.H), stride(p.q_t, p.T), stride(p.q_b, p.B)};
   const uint64_t dk[4] = {D, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.HK), static_cast<uint64_t>(p.B)};
   const uint64_t sk[3] = {stride(p.k_s, p.S), stride(p.k_h, p.HK), stride(p.k_b, p.B)};
+  const uint64_t so[3] = {stride(p.o_h, p.H), stride(p.o_t, p.T), stride(p.o_b, p.B)};
   const uint64_t sv[3] = {stride(p.v_s, p.S), stride(p.v_h, p.HK), stride(p.v_b, p.B)};
   const auto type = CU_TENSOR_MAP_DATA_TYPE_UINT16;
   OSC_TRY(encode_tiled(&mQ, type, 4, p.q, dq, sq, box_q, CU_TENSOR_MAP_SWIZZLE_128B));
   OSC_TRY(encode_tiled(&mK, type, 4, p.k, dk, sk, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
   OSC_TRY(encode_tiled(&mV, type, 4, p.v, dk, sv, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
+  OSC_TRY(encode_tiled(&mO, type, 4, p.out, dq, so, box_q, CU_TENSOR_MAP_SWIZZLE_128B));
   OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(k_window_tiles<D, BF16>), Cfg::SMEM));
-  const dim3 grid((p.T + 2 * p.tokens - 1) / (2 * p.tokens), p.HK, p.B);
-  return launch_pdl(ctx, k_window_tiles<D, BF16>, grid, dim3(kWinThreads), Cfg::SMEM, "k_window_tiles", mQ, mK, mV, p,
+  return launch_pdl(ctx, k_window_tiles<D, BF16>, dim3(std::min(p.items, ctx->num_sms)), dim3(kWinThreads), Cfg::SMEM, "k_window_tiles", mQ, mK, mV, mO, p,
                     ctx->d_err);
 }
 
@@ -813,6 +932,10 @@ int launch(osc_ctx* ctx, WinArgs& p) {
     return launch_rows<D, BF16>(ctx, p);
   }
   p.tokens = 128 / p.G;
+  p.token_tiles = (p.T + p.tokens - 1) / p.tokens;
+  const long long items = static_cast<long long>(p.token_tiles) * p.HK * p.B;
+  if (items >= (1ll << 30)) return fail(OSC_EINVAL, "osc_attention_window: %lld row tiles are too many", items);
+  p.items = static_cast<int>(items);
   return launch_tiles<D, BF16>(ctx, p);
 }
 
