@@ -133,6 +133,7 @@ struct Item {
   int first, len;      // position of query 0, the sequence's length
   int lo, hi;          // live positions of its rows (none: lo > hi)
   int sink_tiles, lo_tile, n;  // key tiles: sinks', then from lo_tile on; how many
+  int plain_lo, plain_hi;      // every row sees every key of the tiles that start in [plain_lo, plain_hi]
   __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : lo_tile + i - sink_tiles) * kKeys; }
 };
 __device__ __forceinline__ Item item_at(const WinArgs& p, int x) {
@@ -151,16 +152,13 @@ __device__ __forceinline__ Item item_at(const WinArgs& p, int x) {
     w.sink_tiles = min((min(p.sinks, w.hi + 1) + kKeys - 1) / kKeys, w.lo_tile);
     w.n = w.sink_tiles + w.hi / kKeys - w.lo_tile + 1;
   }
+  w.plain_lo = w.hi >= p.window ? w.hi - p.window + 1 : 0;
+  w.plain_hi = w.lo == w.first + w.t0 ? w.lo - kKeys + 1 : -1;  // (a row before position 0 sees nothing)
   return w;
 }
-// Some row sees some key of the 32 from g0 on. (The others' probabilities are 0 without a look.)
-__device__ __forceinline__ bool wanted(const WinArgs& p, const Item& w, int g0) {
-  return g0 <= w.hi && (g0 + 31 > w.lo - p.window || g0 < p.sinks);
-}
-
-// Some row sees some key of half `part` of the tile at j0.
-__device__ __forceinline__ bool half_wanted(const WinArgs& p, const Item& w, int j0, int part) {
-  return wanted(p, w, j0 + part * 64) || wanted(p, w, j0 + part * 64 + 32);
+// Some row sees some key of the 64 from h0 on.
+__device__ __forceinline__ bool wanted(const WinArgs& p, const Item& w, int h0) {
+  return h0 <= w.hi && (h0 + 63 > w.lo - p.window || h0 < p.sinks);
 }
 
 // Walks the steps of a CTA's items in order.
@@ -362,7 +360,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         begun[0] = begun[1] = false;
         if (!wait(&bar->o_empty, at.item ^ 1u)) break;
       }
-      const bool half[2] = {half_wanted(p, at.w, j0, 0), half_wanted(p, at.w, j0, 1)};
+      const bool half[2] = {wanted(p, at.w, j0), wanted(p, at.w, j0 + 64)};
       if (!wait(&bar->p_ready[s], at.step >> 1)) break;
       tc_fence_after();
       if (elect_one()) {
@@ -413,17 +411,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       for (int i = 0; i < w.n; ++i, ++step) {
         const int j0 = w.key0(i);
         const uint32_t s_at = lane_base + static_cast<uint32_t>((step & 1u) * kKeys + part * 64);
+        const bool plain = j0 >= w.plain_lo && j0 <= w.plain_hi;
         // both halves take part in every step: the scores after next wait for both
         if (!loaded) {
           if (ok) ok = wait(&bar->s_full[step & 1u], step >> 1);
           tc_fence_after();
         }
-        if (half_wanted(p, w, j0, part)) {
+        if (plain || wanted(p, w, j0 + part * 64)) {
           if (!loaded) tmem_ld64(s_at, s);
           loaded = false;
-          // every row sees every key of the half
-          const int h0 = j0 + part * 64;
-          const bool whole = h0 + 63 <= w.lo && (h0 > w.hi - p.window || h0 + 64 <= p.sinks) && w.lo == w.first + w.t0;
           // The probabilities are taken relative to the maximum so far (0 before a
           // row's first key) while this tile's own is still being found; should that
           // be more than 2^8 above it, or a row's first keys all below it, the
@@ -431,37 +427,32 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           uint32_t pk[32];
           float2 sum;
           for (int again = 0; again < 3; ++again) {  // the second sweep passes
+            tmem_wait_ld(s);
+            if (!plain) {
+              // a bit for each key that this row sees: those up to its own position, from the window's start or among the sinks
+              auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // keys 0 .. n - 1
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int g0 = j0 + part * 64 + h * 32;
+                const int to = live ? pos - g0 : -1;
+                const int from = pos >= p.window ? pos - p.window + 1 - g0 : 0;
+                const uint32_t bits = below(to + 1) & (~below(from) | below(p.sinks - g0));
+#pragma unroll
+                for (int y = 0; y < 32; ++y)
+                  if ((bits & (1u << y)) == 0u) s[h * 32 + y] = 0xff800000u;  // -inf
+              }
+            }
             const float2 mul = make_float2(p.scale2, p.scale2), off = make_float2(-m, -m);
             float top = -INFINITY;
             sum = make_float2(0.0f, 0.0f);
-            tmem_wait_ld();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int g0 = h0 + h * 32;
-              if (wanted(p, w, g0)) {
-                if (!whole) {
-                  // a bit for each key that this row sees: those up to its own position, from the window's start or among the sinks
-                  auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };  // keys 0 .. n - 1
-                  const int to = live ? pos - g0 : -1;
-                  const int from = pos >= p.window ? pos - p.window + 1 - g0 : 0;
-                  const uint32_t bits = below(to + 1) & (~below(from) | below(p.sinks - g0));
-#pragma unroll
-                  for (int y = 0; y < 32; ++y)
-                    if ((bits & (1u << y)) == 0u) s[h * 32 + y] = 0xff800000u;  // -inf
-                }
-#pragma unroll
-                for (int y = 0; y < 16; ++y) {
-                  const float2 a = make_float2(__uint_as_float(s[h * 32 + 2 * y]), __uint_as_float(s[h * 32 + 2 * y + 1]));
-                  top = fmaxf(top, fmaxf(a.x, a.y));
-                  const float2 z = fma2(a, mul, off);
-                  const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
-                  sum = add2(sum, e);
-                  pk[h * 16 + y] = pack2<BF16>(e.x, e.y);
-                }
-              } else {
-#pragma unroll
-                for (int y = 0; y < 16; ++y) pk[h * 16 + y] = 0u;
-              }
+            for (int y = 0; y < 32; ++y) {
+              const float2 a = make_float2(__uint_as_float(s[2 * y]), __uint_as_float(s[2 * y + 1]));
+              top = fmaxf(top, fmaxf(a.x, a.y));
+              const float2 z = fma2(a, mul, off);
+              const float2 e = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+              sum = add2(sum, e);
+              pk[y] = pack2<BF16>(e.x, e.y);
             }
             const float peak = top * p.scale2;
             const bool low = !seen && peak < m && peak > -INFINITY;
@@ -482,7 +473,7 @@ __global__ void __launch_bounds__(kWinThreads, 1)
               for (int g = 0; g < D / 32; ++g) {
                 uint32_t o[32];
                 tmem_ld32(o_own + g * 32, o);
-                tmem_wait_ld();
+                tmem_wait_ld(o);
 #pragma unroll
                 for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
                 tmem_st32(o_own + g * 32, o);
@@ -493,13 +484,6 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           l += sum.x + sum.y;
           tmem_st32(s_at, pk);
           ++had;
-          if (i + 1 < w.n && half_wanted(p, w, w.key0(i + 1), part)) {
-            const uint32_t next = step + 1u;
-            if (ok) ok = wait(&bar->s_full[next & 1u], next >> 1);
-            tc_fence_after();
-            tmem_ld64(lane_base + static_cast<uint32_t>((next & 1u) * kKeys + part * 64), s);
-            loaded = true;
-          }
           tmem_wait_st();
         }
         tc_fence_before();
@@ -528,7 +512,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
           uint32_t a[16], c[16];
           tmem_ld16(o_own + static_cast<uint32_t>(c0), a);
           tmem_ld16(o_his + static_cast<uint32_t>(c0), c);
-          tmem_wait_ld();
+          tmem_wait_ld(a);
+          tmem_wait_ld(c);
           float o[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {

@@ -294,7 +294,7 @@ struct TileShare {
       float next_as;
       tmem_ld16(tmem_lane + g * 16, r);
       fetch(p, c, i0 + PARTS * 16, i_end, lane, next, next_as);
-      tmem_wait_ld();
+      tmem_wait_ld(r);
       float v[16], a[16];
 #pragma unroll
       for (int t = 0; t < 16; ++t) v[t] = sum_of<KIND>(r[t]);
@@ -704,7 +704,7 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
         for (int g = half; g * 16 < tokens; g += 2) {
           uint32_t r[16];
           tmem_ld16(lane_base + g * 16, r);
-          tmem_wait_ld();
+          tmem_wait_ld(r);
 #pragma unroll
           for (int t = 0; t < 16; ++t) part[(g * 16 + t) * kCols + col] = r[t];
         }

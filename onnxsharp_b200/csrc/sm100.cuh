@@ -255,6 +255,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The same, with the loaded registers held back: arithmetic on a load's
+// registers is no memory access, so nothing else keeps the compiler from moving
+// it in front of the wait, where the values may not have arrived.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[N]) {
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 
 // 32 TMEM lanes x 32 consecutive 32-bit columns from registers: thread i of
 // the warp writes lane (base_lane + i). tmem_wait_st() before the values are
