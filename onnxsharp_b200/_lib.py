@@ -35,16 +35,21 @@ ACT_FAST = 16  # OR into conv2d_direct's activation: hardware ex2/rcp Sigmoid/Si
 
 # element types (enum osc_dtype)
 F32, F16, BF16, S8, E4M3 = 0, 1, 2, 3, 4
-_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int8": S8,
-           "torch.float8_e4m3fn": E4M3}
+_dtypes: dict = {}
 
 
 def dtype_code(dtype) -> int:
     """enum osc_dtype of a torch dtype."""
-    try:
-        return _DTYPES[str(dtype)]
-    except KeyError:
-        raise TypeError(f"{dtype} is not float32, float16, bfloat16, int8 or float8_e4m3fn") from None
+    code = _dtypes.get(dtype)
+    if code is None:
+        if not _dtypes:
+            import torch
+
+            _dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: S8,
+                            torch.float8_e4m3fn: E4M3})
+            return dtype_code(dtype)
+        raise TypeError(f"{dtype} is not float32, float16, bfloat16, int8 or float8_e4m3fn")
+    return code
 
 
 class OscError(RuntimeError):

@@ -93,46 +93,60 @@ def layernorm(ctx, x, gamma, beta, eps, y, inner=None):
     return y
 
 
-def _rows(name, t, ctx, like=None):
-    """(row pitch, rows, columns) of a [..., columns] device tensor whose rows follow one another at one pitch."""
-    if not t.is_cuda or t.device.index != ctx.device:
-        raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise ValueError(f"{name} has no columns: {tuple(t.shape)}")
-    if like is not None and t.shape != like.shape:
-        raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(like.shape)}")
-    cols = int(t.shape[-1])
-    if t.dim() == 1 or t.is_contiguous():
-        if t.stride(-1) != 1 and cols > 1:
-            raise ValueError(f"{name}: elements of a row must be adjacent")
-        return cols, t.numel() // cols, cols
-    ok = t.stride(-1) == 1 or cols == 1
-    for d in range(t.dim() - 2):  # leading dimensions fold into one run of rows
-        ok = ok and (t.shape[d] == 1 or t.stride(d) == t.stride(d + 1) * t.shape[d + 1])
-    if not ok or (t.shape[-2] > 1 and t.stride(-2) < cols):
+def _row_pitch(name, t, cols):
+    """Row pitch of a [..., cols] tensor whose rows are dense and follow one another at one pitch."""
+    shape, stride = t.shape, t.stride()
+    ok = stride[-1] == 1 or cols == 1
+    for d in range(len(shape) - 2):  # leading dimensions fold into one run of rows
+        ok = ok and (shape[d] == 1 or stride[d] == stride[d + 1] * shape[d + 1])
+    pitch = stride[-2] if len(shape) > 1 and shape[-2] > 1 else next((s for n, s in zip(shape[-3::-1], stride[-3::-1])
+                                                                       if n > 1), cols)
+    if not ok or pitch < cols:
         raise ValueError(f"{name}: rows must be dense and follow one another at one pitch")
-    return max(int(t.stride(-2)), cols), t.numel() // cols, cols
+    return pitch
+
+
+def _rows_like(name, t, device, shape, dtype):
+    """Row pitch of a tensor that has to match x (dtype None: any)."""
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the context on cuda:{device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, x is {dtype}")
+    return shape[-1] if t.is_contiguous() else _row_pitch(name, t, shape[-1])
+
+
+def _adjacent(name, t, device, n, dtype):
+    if t.get_device() != device or t.numel() != n or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{name} must be {n} adjacent {dtype} values on cuda:{device}")
+    return t.data_ptr()
 
 
 def _rmsnorm(ctx, x, gamma, eps, residual, sum_out, y, q, scales):
-    ld, rows, cols = _rows("x", x, ctx)
-    pitch = {"residual": 0, "sum_out": 0, "y": 0, "q": 0}
-    for name, t in (("residual", residual), ("sum_out", sum_out), ("y", y), ("q", q)):
-        if t is not None:
-            pitch[name] = _rows(name, t, ctx, x)[0]
-            if name != "q" and t.dtype != x.dtype:
-                raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
+    shape, dtype, device = x.shape, x.dtype, ctx.device
+    if len(shape) == 0 or shape[-1] == 0:
+        raise ValueError(f"x has no columns: {tuple(shape)}")
+    cols = shape[-1]
+    rows = x.numel() // cols
+    ld, ld_r, ld_s, ld_y, ld_q = _rows_like("x", x, device, shape, dtype), 0, 0, 0, 0
+    r = s = o = c = f = g = None
+    if residual is not None:
+        ld_r, r = _rows_like("residual", residual, device, shape, dtype), residual.data_ptr()
+    if sum_out is not None:
+        ld_s, s = _rows_like("sum_out", sum_out, device, shape, dtype), sum_out.data_ptr()
+    if y is not None:
+        ld_y, o = _rows_like("y", y, device, shape, dtype), y.data_ptr()
+    if q is not None:
+        ld_q, c = _rows_like("q", q, device, shape, None), q.data_ptr()
     if gamma is not None:
-        _rows("gamma", gamma, ctx)
-        if gamma.dtype != x.dtype or gamma.numel() != cols or not gamma.is_contiguous():
-            raise ValueError(f"gamma must be {cols} adjacent {x.dtype} values")
+        g = _adjacent("gamma", gamma, device, cols, dtype)
     if scales is not None:
-        _rows("scales", scales, ctx)
-        if str(scales.dtype) != "torch.float32" or scales.numel() != rows or not scales.is_contiguous():
-            raise ValueError(f"scales must be {rows} adjacent float32 values")
-    call("osc_rmsnorm", ctx.handle, _lib.dtype_code(x.dtype), ptr(x), ld, ptr(residual), pitch["residual"], rows, cols,
-         ptr(gamma), float(eps), ptr(sum_out), pitch["sum_out"], ptr(y), pitch["y"],
-         0 if q is None else _lib.dtype_code(q.dtype), ptr(q), pitch["q"], ptr(scales))
+        import torch
+
+        f = _adjacent("scales", scales, device, rows, torch.float32)
+    call("osc_rmsnorm", ctx.handle, _lib.dtype_code(dtype), x.data_ptr(), ld, r, ld_r, rows, cols, g, eps, s, ld_s, o, ld_y,
+         0 if q is None else _lib.dtype_code(q.dtype), c, ld_q, f)
 
 
 def rmsnorm(ctx, x, gamma, eps, y, residual=None, sum_out=None):

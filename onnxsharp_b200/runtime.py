@@ -326,25 +326,29 @@ class LinearWeights:
         self._finalizer = weakref.finalize(self, _lib.load().osc_linear_weights_free, h)
 
 
-def _pitch(name: str, t, ctx: Context, rows: int, cols: int) -> int:
-    """Row pitch of a [rows, cols] device tensor with adjacent elements."""
-    if not t.is_cuda or t.device.index != ctx.device:
+def _pitch(name: str, t, ctx: Context, shape: tuple) -> int:
+    """Row pitch of a device matrix of that shape with dense rows."""
+    if t.get_device() != ctx.device:
         raise ValueError(f"linear: {name} is on {t.device}, the context on cuda:{ctx.device}")
-    if tuple(t.shape) != (rows, cols):
-        raise ValueError(f"linear: {name} is {tuple(t.shape)}, expected {(rows, cols)}")
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    if t.shape != shape:
+        raise ValueError(f"linear: {name} is {tuple(t.shape)}, expected {shape}")
+    rows, cols = shape
+    if t.is_contiguous():
+        return cols
+    pitch, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and pitch < cols):
         raise ValueError(f"linear: the rows of {name} must be dense")
-    return max(int(t.stride(0)), cols) if rows > 1 else cols
+    return pitch if rows > 1 else cols
 
 
-def _vector(name: str, t, ctx: Context, *sizes: int):
+def _vector(name: str, t, ctx: Context, n: int, also: int = 0):
     if t is None:
         return None
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise ValueError(f"linear: {name} is on {t.device}, the context on cuda:{ctx.device}")
-    if str(t.dtype) != "torch.float32" or t.numel() not in sizes or not t.is_contiguous():
-        raise ValueError(f"linear: {name} must be {' or '.join(map(str, sizes))} adjacent float32 values")
-    return ptr(t)
+    if _lib.dtype_code(t.dtype) != _lib.F32 or t.numel() not in (n, also or n) or not t.is_contiguous():
+        raise ValueError(f"linear: {name} must be {n}{f' or {also}' if also else ''} adjacent float32 values")
+    return t.data_ptr()
 
 
 def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NONE, residual=None, a_scale=None,
@@ -353,27 +357,29 @@ def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NON
     a [m, k] has w's type and may be a pitched view; a_scale [m], w_scale [n] or [1] (8-bit types) and bias [n] are
     float32. The result is float32, float16 or bfloat16: out's, the residual's, out_dtype, else a's type (8-bit: float32).
     out may be the residual itself."""
-    import torch
-
     if a.dim() != 2:
         raise ValueError(f"linear: a is {tuple(a.shape)}, expected (m, {w.k})")
-    m = int(a.shape[0])
+    m, n = a.shape[0], w.n
     if a.dtype != w.dtype:
         raise TypeError(f"linear: a is {a.dtype}, the weights are {w.dtype}")
+    lda = _pitch("a", a, ctx, (m, w.k))
     if out is None:
+        import torch
+
         if out_dtype is None:
             coded = a.dtype in (torch.int8, torch.float8_e4m3fn)
             out_dtype = residual.dtype if residual is not None else torch.float32 if coded else a.dtype
-        out = torch.empty((m, w.n), dtype=out_dtype, device=a.device)
+        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"linear: out is {out.dtype}, not {out_dtype}")
-    if residual is not None and residual.dtype != out.dtype:
-        raise TypeError(f"linear: the residual is {residual.dtype}, the result {out.dtype}")
-    lda, ldy = _pitch("a", a, ctx, m, w.k), _pitch("out", out, ctx, m, w.n)
-    ldr = 0 if residual is None else _pitch("residual", residual, ctx, m, w.n)
-    call("osc_linear", ctx.handle, ptr(a), m, lda, w.handle, _vector("a_scale", a_scale, ctx, m),
-         _vector("w_scale", w_scale, ctx, 1, w.n), 0 if w_scale is None else int(w_scale.numel()),
-         _vector("bias", bias, ctx, w.n), int(act), ptr(residual), ldr, _lib.dtype_code(out.dtype), ptr(out), ldy)
+    ldy, ldr = _pitch("out", out, ctx, (m, n)), 0
+    if residual is not None:
+        if residual.dtype != out.dtype:
+            raise TypeError(f"linear: the residual is {residual.dtype}, the result {out.dtype}")
+        ldr = _pitch("residual", residual, ctx, (m, n))
+    call("osc_linear", ctx.handle, a.data_ptr(), m, lda, w.handle, _vector("a_scale", a_scale, ctx, m),
+         _vector("w_scale", w_scale, ctx, n, 1), 0 if w_scale is None else w_scale.numel(), _vector("bias", bias, ctx, n),
+         act, ptr(residual), ldr, _lib.dtype_code(out.dtype), out.data_ptr(), ldy)
     return out
 
 
@@ -410,31 +416,34 @@ def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int |
     first `sinks`. Padding queries (outside 0 .. lengths - 1) give zeros."""
     import torch
 
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"attention_window: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    B, T, H, D = (int(x) for x in q.shape)
-    S, HK = int(k.shape[1]), int(k.shape[2])
+    shape, keys, dtype, device = q.shape, k.shape, q.dtype, ctx.device
+    if len(shape) != 4 or len(keys) != 4 or v.shape != keys or shape[0] != keys[0] or shape[3] != keys[3]:
+        raise ValueError(f"attention_window: q {tuple(shape)}, k {tuple(keys)}, v {tuple(v.shape)}")
+    (B, T, H, D), (_, S, HK, _) = shape, keys
     if out is None:
-        out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-    if out.shape != q.shape:
-        raise ValueError(f"attention_window: out is {tuple(out.shape)}, q {tuple(q.shape)}")
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        if not t.is_cuda or t.device.index != ctx.device:
-            raise ValueError(f"attention_window: {name} is on {t.device}, the context on cuda:{ctx.device}")
-        if t.dtype != q.dtype:
-            raise TypeError(f"attention_window: {name} is {t.dtype}, q is {q.dtype}")
-        if t.stride(3) != 1:
-            raise ValueError(f"attention_window: the last axis of {name} must be dense")
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape:
+        raise ValueError(f"attention_window: out is {tuple(out.shape)}, q {tuple(shape)}")
+    strides = []
+    for t in (q, k, v, out):
+        if t.get_device() != device:
+            raise ValueError(f"attention_window: a tensor is on {t.device}, the context on cuda:{device}")
+        if t.dtype != dtype:
+            raise TypeError(f"attention_window: one tensor is {t.dtype}, q is {dtype}")
+        s = t.stride()
+        if s[3] != 1:
+            raise ValueError("attention_window: the last axis of q, k, v and out must be dense")
+        strides += s[:3]
     for name, t in (("lengths", lengths), ("starts", starts)):
-        if t is not None and (not t.is_cuda or t.device.index != ctx.device or t.dtype != torch.int32
-                              or t.numel() != B or not t.is_contiguous()):
-            raise ValueError(f"attention_window: {name} must be {B} adjacent int32 values on cuda:{ctx.device}")
-    if lengths is None:
-        raise ValueError("attention_window: lengths are needed")
-    st = [(C.c_longlong * 3)(*t.stride()[:3]) for t in (q, k, v, out)]
-    call("osc_attention_window", ctx.handle, _lib.dtype_code(q.dtype), ptr(q), st[0], ptr(k), st[1], ptr(v), st[2],
-         ptr(lengths), ptr(starts), B, T, S, H, HK, D, 2**31 - 1 if window is None else int(window), int(sinks),
-         float(scale), ptr(out), st[3])
+        if t is None:
+            if name == "lengths":
+                raise ValueError("attention_window: lengths are needed")
+        elif t.get_device() != device or t.dtype != torch.int32 or t.numel() != B or not t.is_contiguous():
+            raise ValueError(f"attention_window: {name} must be {B} adjacent int32 values on cuda:{device}")
+    st = (C.c_longlong * 12)(*strides)
+    call("osc_attention_window", ctx.handle, _lib.dtype_code(dtype), q.data_ptr(), st, k.data_ptr(), C.byref(st, 24),
+         v.data_ptr(), C.byref(st, 48), lengths.data_ptr(), None if starts is None else starts.data_ptr(), B, T, S, H, HK, D,
+         2**31 - 1 if window is None else window, sinks, scale, out.data_ptr(), C.byref(st, 72))
     return out
 
 

@@ -227,7 +227,7 @@ def test_refusals(ctx):
         attention_window(ctx, torch.zeros(2 * 3 * 4 * 64 + 1, dtype=q.dtype, device="cuda")[1:].view(2, 3, 4, 64), k, v, n, 1.0)
     with pytest.raises(OscError, match="dtype"):
         attention_window(ctx, q.float(), k.float(), v.float(), n, 1.0)
-    with pytest.raises(TypeError, match="k is"):
+    with pytest.raises(TypeError, match="one tensor is"):
         attention_window(ctx, q, k.half(), v, n, 1.0)
     with pytest.raises(ValueError, match="lengths"):
         attention_window(ctx, q, k, v, n.long(), 1.0)
