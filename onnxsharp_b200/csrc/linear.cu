@@ -50,16 +50,17 @@ constexpr int kKB = 128;                 // bytes of K in a block: one swizzle r
 constexpr int kWBytes = kCols * kKB;     // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kTileEpi = 16;             // epilogue warps of k_linear_tiles
-constexpr int kSplitEpi = 8;             // of k_linear_split: two CTAs share an SM
+constexpr int kSplitEpi = 4;             // of k_linear_split: several CTAs share an SM
 constexpr int kLoadWarps = 4;            // rows of A that no TMA box fits
 constexpr int kSmemTail = 512;           // barriers
 constexpr int kSmemOne = 232448 - 1024;  // one CTA per SM: the ring and the tail
-constexpr int kSmemTwo = 115712 - 1024;  // two CTAs per SM
+constexpr int kSmemSm = 233472;          // of an SM, 1 KB of every CTA's the system's
 constexpr int kMaxSplit = 8;             // portable cluster size
 
 struct LinArgs {
   int M, N, num_kb, last_steps;  // last_steps: 32-byte K steps of the last block
   int bn;                        // tokens of a tile
+  int kbs;                       // k-blocks of a ring stage
   int stages, stage_bytes;
   int tiles_m, tiles_n;          // token tiles, column tiles (of 256 for a CTA pair)
   int split;                     // CTAs that share a tile's K
@@ -420,12 +421,14 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
     bool waited = false;
     int pre = 0;  // weight blocks issued before the previous kernel was waited for, not yet joined by their tokens
     bool ok = true;
-    auto load_w = [&](int s, int row) {
+    auto load_w = [&](int s, int row, int blocks) {
       if (elect_one()) {
         uint8_t* st = ring + s * p.stage_bytes;
-        if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * (kWBytes + (ATMA ? arows * kKB : 0)));
-        if (PAIR) tma_load_2d_pair(st, &mW, full0 + static_cast<uint32_t>(s * 8), 0, row);
-        else tma_load_2d(st, &mW, &b->full[s], 0, row);
+        if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * blocks * (kWBytes + (ATMA ? arows * kKB : 0)));
+        for (int y = 0; y < blocks; ++y) {
+          if (PAIR) tma_load_2d_pair(st + y * kWBytes, &mW, full0 + static_cast<uint32_t>(s * 8), 0, row + y * kCols);
+          else tma_load_2d(st + y * kWBytes, &mW, &b->full[s], 0, row + y * kCols);
+        }
       }
     };
     for (int t = first; t < tiles && ok; t += walkers) {
@@ -435,24 +438,26 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
       if (!waited) {
         // the weights were laid out before this launch was made: their first
         // blocks travel while the previous kernel on the stream drains
-        pre = min(p.stages, p.num_kb);
-        for (int kb = 0; kb < pre; ++kb) load_w(kb, w_row + kb * kCols);
+        for (int kb = 0; pre < p.stages && kb < p.num_kb; kb += p.kbs, ++pre)
+          load_w(pre, w_row + kb * kCols, min(p.kbs, p.num_kb - kb));
         griddep_wait();
         waited = true;
       }
-      for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
-        const int s = at.s;
+      for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
+        const int s = at.s, blocks = min(p.kbs, p.num_kb - kb);
         if (pre > 0) {
           --pre;
         } else {
           ok = wait(&b->empty[s], at.phase ^ 1u);
           if (!ok) break;
-          load_w(s, w_row + kb * kCols);
+          load_w(s, w_row + kb * kCols, blocks);
         }
         if (ATMA && elect_one()) {
-          uint8_t* st = ring + s * p.stage_bytes + kWBytes;
-          if (PAIR) tma_load_2d_pair(st, &mA, full0 + static_cast<uint32_t>(s * 8), kb * kKB, a_row);
-          else tma_load_2d(st, &mA, &b->full[s], kb * kKB, a_row);
+          uint8_t* st = ring + s * p.stage_bytes + p.kbs * kWBytes;
+          for (int y = 0; y < blocks; ++y) {
+            if (PAIR) tma_load_2d_pair(st + y * arows * kKB, &mA, full0 + static_cast<uint32_t>(s * 8), (kb + y) * kKB, a_row);
+            else tma_load_2d(st + y * arows * kKB, &mA, &b->full[s], (kb + y) * kKB, a_row);
+          }
         }
       }
     }
@@ -476,23 +481,26 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
         if (!wait(&b->acc_empty[buf], ((it >> 1) & 1u) ^ 1u)) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(buf * 256);
-        for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
-          const int s = at.s;
+        for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
+          const int s = at.s, blocks = min(p.kbs, p.num_kb - kb);
           ok = wait(&b->full[s], at.phase);
           if (!ok) break;
           const uint32_t base = smem_addr(ring + s * p.stage_bytes);
-          const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
-          const int steps = kb + 1 == p.num_kb ? p.last_steps : 4;
+          const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + p.kbs * kWBytes);
           if (elect_one()) {
+            for (int y = 0; y < blocks; ++y) {
+              const uint64_t dw = dw0 + static_cast<uint64_t>(y * (kWBytes >> 4)), da = da0 + static_cast<uint64_t>(y * (arows * kKB >> 4));
+              const int steps = kb + y + 1 == p.num_kb ? p.last_steps : 4;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              if (kk < steps) {
-                const uint64_t off = static_cast<uint64_t>(kk * 2);  // 32 bytes of K
-                if (PAIR) mma_two<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-                else mma_one<KIND>(d, dw + off, da + off, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-              }
+              for (int kk = 0; kk < 4; ++kk)
+                if (kk < steps) {
+                  const uint64_t off = static_cast<uint64_t>(kk * 2);  // 32 bytes of K
+                  if (PAIR) mma_two<KIND>(d, dw + off, da + off, p.idesc, (kb | y | kk) != 0 ? 1u : 0u);
+                  else mma_one<KIND>(d, dw + off, da + off, p.idesc, (kb | y | kk) != 0 ? 1u : 0u);
+                }
+            }
             commit(&b->empty[s]);
-            if (kb + 1 == p.num_kb) commit(&b->acc_full[buf]);
+            if (kb + p.kbs >= p.num_kb) commit(&b->acc_full[buf]);
           }
         }
       }
@@ -531,12 +539,13 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
     for (int t = first; t < tiles && ok; t += walkers) {
       int tm, tn;
       tile_at(p, t, tm, tn);
-      for (int kb = 0; kb < p.num_kb; ++kb, at.next(p.stages)) {
+      for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
         const int s = at.s;
         ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        load_rows(p, ring + s * p.stage_bytes + kWBytes, tm * p.bn, arows, kb, w, lane);
+        for (int y = 0; y < min(p.kbs, p.num_kb - kb); ++y)
+          load_rows(p, ring + s * p.stage_bytes + p.kbs * kWBytes + y * arows * kKB, tm * p.bn, arows, kb + y, w, lane);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&b->full[s]);
@@ -581,7 +590,7 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 }
 
 template <int KIND, bool ATMA>
-__global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)), 2)
+__global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)), ATMA ? 4 : 2)
     k_linear_split(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, uint32_t tmem_cols, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
   const int tile = static_cast<int>(blockIdx.x) / p.split;
   const int tm = tile / p.tiles_n, tn = tile - tm * p.tiles_n;
   const int kb0 = static_cast<int>(static_cast<long long>(rank) * p.num_kb / p.split);
-  const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * p.num_kb / p.split);
+  const int kbn = static_cast<int>(static_cast<long long>(rank + 1) * p.num_kb / p.split) - kb0;  // this CTA's k-blocks
   const int m0 = tm * p.bn;
 
   if (threadIdx.x == 0) {
@@ -621,54 +630,65 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
     return __all_sync(0xffffffffu, ok) != 0;
   };
   if (warp == 0) {
-    const int pre = min(p.stages, kb1 - kb0);
     const int w_row = (tn * p.num_kb + kb0) * kCols;
     auto load_w = [&](int s, int kc) {
       if (elect_one()) {
-        mbar_arrive_expect_tx(&b->full[s], kWBytes + (ATMA ? p.bn * kKB : 0));
-        tma_load_2d(ring + s * p.stage_bytes, &mW, &b->full[s], 0, w_row + kc * kCols);
+        const int blocks = min(p.kbs, kbn - kc);
+        mbar_arrive_expect_tx(&b->full[s], blocks * (kWBytes + (ATMA ? p.bn * kKB : 0)));
+        for (int y = 0; y < blocks; ++y)
+          tma_load_2d(ring + s * p.stage_bytes + y * kWBytes, &mW, &b->full[s], 0, w_row + (kc + y) * kCols);
       }
     };
-    for (int kc = 0; kc < pre; ++kc) load_w(kc, kc);  // laid out before this launch was made
+    // the weights were laid out before this launch was made: the first blocks
+    // land while the previous kernel on the stream drains
+    int pre = 0;
+    for (int kc = 0; pre < p.stages && kc < kbn; kc += p.kbs, ++pre) load_w(pre, kc);
     griddep_wait();
     RingPos at;
-    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
+    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
       const int s = at.s;
-      if (kc >= pre) {
+      if (pre > 0) {
+        --pre;
+      } else {
         if (!wait(&b->empty[s], at.phase ^ 1u)) break;
         load_w(s, kc);
       }
       if (ATMA && elect_one())
-        tma_load_2d(ring + s * p.stage_bytes + kWBytes, &mA, &b->full[s], (kb0 + kc) * kKB, m0);
+        for (int y = 0; y < min(p.kbs, kbn - kc); ++y)
+          tma_load_2d(ring + s * p.stage_bytes + p.kbs * kWBytes + y * p.bn * kKB, &mA, &b->full[s], (kb0 + kc + y) * kKB, m0);
     }
   } else if (warp == 1) {
     RingPos at;
-    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
-      const int s = at.s;
+    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
+      const int s = at.s, blocks = min(p.kbs, kbn - kc);
       if (!wait(&b->full[s], at.phase)) break;
       const uint32_t base = smem_addr(ring + s * p.stage_bytes);
-      const uint64_t dw = sdesc_kmajor_sw128(base), da = sdesc_kmajor_sw128(base + kWBytes);
-      const int steps = kb0 + kc + 1 == p.num_kb ? p.last_steps : 4;
+      const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + p.kbs * kWBytes);
       if (elect_one()) {
+        for (int y = 0; y < blocks; ++y) {
+          const uint64_t dw = dw0 + static_cast<uint64_t>(y * (kWBytes >> 4)), da = da0 + static_cast<uint64_t>(y * (p.bn * kKB >> 4));
+          const int steps = kb0 + kc + y + 1 == p.num_kb ? p.last_steps : 4;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          if (kk < steps) {
-            const uint64_t off = static_cast<uint64_t>(kk * 2);
-            mma_one<KIND>(tmem, dw + off, da + off, p.idesc, (kc | kk) != 0 ? 1u : 0u);
-          }
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < steps) {
+              const uint64_t off = static_cast<uint64_t>(kk * 2);
+              mma_one<KIND>(tmem, dw + off, da + off, p.idesc, (kc | y | kk) != 0 ? 1u : 0u);
+            }
+        }
         mma_commit(&b->empty[s]);
-        if (kc + 1 == kb1 - kb0) mma_commit(&b->acc_full[0]);
+        if (kc + p.kbs >= kbn) mma_commit(&b->acc_full[0]);
       }
     }
   } else if (warp >= 2 + kSplitEpi) {
     griddep_wait();
     const int w = warp - 2 - kSplitEpi;
     RingPos at;
-    for (int kc = 0; kc < kb1 - kb0; ++kc, at.next(p.stages)) {
+    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
       const int s = at.s;
       const bool ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
       if (!__all_sync(0xffffffffu, ok)) break;
-      load_rows(p, ring + s * p.stage_bytes + kWBytes, m0, p.bn, kb0 + kc, w, lane);
+      for (int y = 0; y < min(p.kbs, kbn - kc); ++y)
+        load_rows(p, ring + s * p.stage_bytes + p.kbs * kWBytes + y * p.bn * kKB, m0, p.bn, kb0 + kc + y, w, lane);
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b->full[s]);
@@ -676,7 +696,8 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
   }
 
   const bool epi = warp >= 2 && warp < 2 + kSplitEpi;
-  const int q = warp & 3, half = (warp - 2) >> 2;
+  const int q = warp & 3, part = (warp - 2) >> 2;
+  constexpr int kParts = kSplitEpi / 4;
   const int col = q * 32 + lane;
   const int j = tn * kCols + col;
   const bool in = j < p.N;
@@ -688,11 +709,11 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(q * 32) << 16);
     if (p.split == 1) {
       TileShare<KIND, kSplitEpi / 4> share;
-      share.begin(p, c, half, m0, j, lane);
+      share.begin(p, c, part, m0, j, lane);
       const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
-        share.drain(p, c, lane_base, half, m0, j, lane);
+        share.drain(p, c, lane_base, part, m0, j, lane);
       }
     } else {
       const bool ok = mbar_wait(&b->acc_full[0], 0, &b->abort_flag, err);
@@ -700,52 +721,60 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
         // every block of this CTA has been multiplied: the ring is free and
         // takes the partial sums, [token][column]
         tc_fence_after();
-        uint32_t* part = reinterpret_cast<uint32_t*>(ring);
-        for (int g = half; g * 16 < tokens; g += 2) {
+        uint32_t* sums = reinterpret_cast<uint32_t*>(ring);
+        for (int g = part; g * 16 < tokens; g += kParts) {
           uint32_t r[16];
           tmem_ld16(lane_base + g * 16, r);
           tmem_wait_ld(r);
 #pragma unroll
-          for (int t = 0; t < 16; ++t) part[(g * 16 + t) * kCols + col] = r[t];
+          for (int t = 0; t < 16; ++t) sums[(g * 16 + t) * kCols + col] = r[t];
         }
       }
     }
     tc_fence_before();
   }
   if (p.split > 1) {
+    constexpr int U = 4;
+    const int slice = (tokens + p.split - 1) / p.split;
+    const int lo = rank * slice, hi = min(tokens, lo + slice);
+    const int i_end = in ? m0 + hi : 0;
+    // what the first tokens need beside the sums travels while the CTAs meet
+    uint32_t res[U];
+    float as[U];
+    auto fetch = [&](int i) {
+      load_residual<U>(p, c, m0 + i, kParts, i_end, res);
+#pragma unroll
+      for (int t = 0; t < U; ++t)
+        as[t] = p.a_scale != nullptr && i + kParts * t < hi ? p.a_scale[m0 + i + kParts * t] : 1.0f;
+    };
+    if (epi) fetch(lo + part);
     __syncwarp();
     cluster_sync_all();
     if (epi) {
-      const int slice = (tokens + p.split - 1) / p.split;
-      const int lo = rank * slice, hi = min(tokens, lo + slice);
       const uint32_t own = smem_addr(ring) + static_cast<uint32_t>(col * 4);
       uint32_t peer[kMaxSplit];
 #pragma unroll
       for (int x = 0; x < kMaxSplit; ++x)
         if (x < p.split) asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(peer[x]) : "r"(own), "r"(x));
-      constexpr int U = 4;
-      const int i_end = in ? m0 + hi : 0;
-      for (int i = lo + half; i < hi; i += 2 * U) {
-        uint32_t res[U];
-        load_residual<U>(p, c, m0 + i, 2, i_end, res);
-        float as[U];
+      for (int i = lo + part; i < hi; i += kParts * U) {
+        // every CTA's part is on its way before the first is added
+        uint32_t sums[kMaxSplit][U];
 #pragma unroll
-        for (int t = 0; t < U; ++t) as[t] = p.a_scale != nullptr ? p.a_scale[m0 + min(i + 2 * t, hi - 1)] : 1.0f;
+        for (int x = 0; x < kMaxSplit; ++x)
+#pragma unroll
+          for (int t = 0; t < U; ++t)
+            sums[x][t] = x < p.split && i + kParts * t < hi ? ld_cluster(peer[x] + static_cast<uint32_t>((i + kParts * t) * kCols * 4)) : 0u;
         uint32_t acc[U] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int x = 0; x < kMaxSplit; ++x)
-          if (x < p.split) {
-            uint32_t part[U];
 #pragma unroll
-            for (int t = 0; t < U; ++t) part[t] = ld_cluster(peer[x] + static_cast<uint32_t>(min(i + 2 * t, hi - 1) * kCols * 4));
-#pragma unroll
-            for (int t = 0; t < U; ++t)
-              acc[t] = KIND == LIN_I8 ? acc[t] + part[t] : __float_as_uint(__uint_as_float(acc[t]) + __uint_as_float(part[t]));
-          }
+          for (int t = 0; t < U; ++t)
+            acc[t] = KIND == LIN_I8 ? acc[t] + sums[x][t] : __float_as_uint(__uint_as_float(acc[t]) + __uint_as_float(sums[x][t]));
         float v[U];
 #pragma unroll
         for (int t = 0; t < U; ++t) v[t] = sum_of<KIND>(acc[t]);
-        finish<U>(p, c, v, as, res, m0 + i, 2, i_end);
+        finish<U>(p, c, v, as, res, m0 + i, kParts, i_end);
+        if (i + kParts * U < hi) fetch(i + kParts * U);
       }
     }
     __syncwarp();
@@ -807,6 +836,8 @@ struct LinPlan {
   bool split_kernel;
   bool pair;
   int bn, split;
+  int per_sm;  // CTAs of k_linear_split that an SM's shared memory is cut for
+  int kbs;     // k-blocks of a ring stage
 };
 
 int div_up(int a, int b) { return (a + b - 1) / b; }
@@ -830,7 +861,7 @@ LinPlan choose(int num_sms, int m, int n, int num_kb, bool atma) {
       if (split > num_kb) break;
       const double waves = std::ceil(tiles * split / (2 * num_sms));
       const double kb = div_up(num_kb, split);
-      consider({true, false, bn, split},
+      consider({true, false, bn, split, 2, 2},
                waves * (kb * std::max(2 * 4 * std::max(50.0, bn / 2.0), 2 * (kWBytes + bn * kKB) / 40.0) + 1500 + 10 * bn) + (split > 1 ? 1500 : 0));
     }
   }
@@ -841,7 +872,7 @@ LinPlan choose(int num_sms, int m, int n, int num_kb, bool atma) {
       const double tiles = static_cast<double>(div_up(cols, pair ? 2 : 1)) * div_up(m, bn);
       const double waves = std::ceil(tiles / (num_sms / (pair ? 2 : 1)));
       const double bytes = kWBytes + static_cast<double>(bn) * kKB / (pair ? 2 : 1);
-      consider({false, pair != 0, bn, 1},
+      consider({false, pair != 0, bn, 1, 1, 2},
                waves * num_kb * std::max(4 * std::max(50.0, bn / 2.0), bytes / 60.0) + 2500 + 20.0 * bn);
     }
   }
@@ -1042,8 +1073,9 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   p.bn = pl.bn;
   p.split = pl.split;
   const int arows = pl.pair ? pl.bn / 2 : pl.bn;
-  p.stage_bytes = kWBytes + arows * kKB;
-  p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemTwo : kSmemOne) - kSmemTail) / p.stage_bytes);
+  p.kbs = pl.kbs;
+  p.stage_bytes = p.kbs * (kWBytes + arows * kKB);
+  p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemSm / pl.per_sm - 2048 : kSmemOne) - kSmemTail) / p.stage_bytes);
   p.tiles_m = div_up(m, pl.bn);
   p.tiles_n = div_up(w->n, pl.pair ? 2 * kCols : kCols);
   if (static_cast<long long>(p.tiles_m) * p.tiles_n * pl.split >= (1ll << 31) || m > (1 << 30))
