@@ -379,14 +379,14 @@ OSC_API int osc_linear_prepack(osc_ctx* ctx, int dtype, const void* w, int k, in
 OSC_API int osc_linear_weights_free(osc_linear_weights* w);
 
 /* m >= 0 (0: nothing is done). lda, ldr, ldy: row pitches in elements (0 =
- * dense), of any alignment; rows that are 16-byte aligned travel by TMA. The
+ * dense), of any alignment; rows of a that do not start on 16-byte boundaries
+ * are first copied to a temporary, allocated and freed in stream order. The
  * scales (8-bit types only) and the bias are FP32 and may be NULL: a_scale [m]
  * (what osc_rmsnorm writes), w_scale n_scale entries (1 or n), bias [n].
  * out_dtype: OSC_F32, OSC_F16 or OSC_BF16, also the residual's type. act: any
  * osc_act up to OSC_ACT_GELU_TANH. residual may be NULL, and may be y itself
- * (same pointer and pitch); no other argument may overlap y. Uses no scratch
- * memory, so calls on different streams or in different graphs share nothing
- * but the weights. */
+ * (same pointer and pitch); no other argument may overlap y. Calls on different
+ * streams or in different graphs share nothing but the weights. */
 OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const osc_linear_weights* w,
                        const float* a_scale, const float* w_scale, int n_scale, const float* bias, int act,
                        const void* residual, long long ldr, int out_dtype, void* y, long long ldy);

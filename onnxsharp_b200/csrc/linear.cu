@@ -51,7 +51,6 @@ constexpr int kWBytes = kCols * kKB;     // 16 KB
 constexpr int kMaxStages = 8;
 constexpr int kTileEpi = 16;             // epilogue warps of k_linear_tiles
 constexpr int kSplitEpi = 4;             // of k_linear_split: several CTAs share an SM
-constexpr int kLoadWarps = 4;            // rows of A that no TMA box fits
 constexpr int kSmemTail = 512;           // barriers
 constexpr int kSmemOne = 232448 - 1024;  // one CTA per SM: the ring and the tail
 constexpr int kSmemSm = 233472;          // of an SM, 1 KB of every CTA's the system's
@@ -75,9 +74,6 @@ struct LinArgs {
   long long ldr_bytes;
   void* y;
   long long ldy_bytes;
-  const uint8_t* a;              // for rows that no TMA box fits
-  long long lda_bytes;
-  int k_bytes;
 };
 
 struct LinBars {
@@ -312,39 +308,42 @@ struct TileShare {
 };
 
 // ------------------------------------------------------------------ rows of A that no TMA box fits
-// kLoadWarps warps write the token operand of a stage themselves, in the
-// layout the 128-byte-swizzled TMA box would have: a lane takes four bytes of a
-// row from the one or two aligned words that hold them (each holds a byte of
-// the row, so neither lies outside the tensor's allocation), bytes past K and
-// rows past M are zeros.
-__device__ __forceinline__ void load_rows(const LinArgs& p, uint8_t* dst, int row0, int rows, int kb, int w, int lane) {
-  const int off = kb * kKB + lane * 4;
-  const int valid = min(4, p.k_bytes - off);  // <= 0: nothing of the row here
-  constexpr int U = 8;
-  for (int r0 = w; r0 < rows; r0 += kLoadWarps * U) {
-    uint32_t w0[U], w1[U], sh[U];
+// Rows at any pitch and alignment -> rows of whole 16-byte pieces, 16-byte
+// aligned, zeros past k_bytes. A thread puts one piece together from the one or
+// two aligned ones that hold it (each holds a byte of the row, so neither lies
+// outside the tensor's allocation). 2000 x 2001 bf16 by 2048 columns takes 21 us
+// with this copy; loader warps inside the product, which fetched such rows for
+// every column tile again, took 95.
+__global__ void k_linear_rows(const uint8_t* __restrict__ a, int m, int k_bytes, long long lda_bytes, int pieces,
+                              uint8_t* __restrict__ out) {
+  griddep_launch();
+  griddep_wait();
+  const long long total = static_cast<long long>(m) * pieces;
+  for (long long x = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; x < total;
+       x += static_cast<long long>(gridDim.x) * blockDim.x) {
+    const long long i = x / pieces;
+    const int off = static_cast<int>(x - i * pieces) * 16, valid = min(16, k_bytes - off);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a + i * lda_bytes + off);
+    const uint32_t s = static_cast<uint32_t>(at & 15u), q = s >> 2, bits = 8u * (s & 3u);
+    const uint4* piece = reinterpret_cast<const uint4*>(at - s);
+    const uint4 lo = piece[0];
+    const uint4 hi = static_cast<int>(s) + valid > 16 ? piece[1] : make_uint4(0u, 0u, 0u, 0u);
+    // the five words from the q-th of the eight on
+    const uint32_t x0 = q < 2 ? (q == 0 ? lo.x : lo.y) : (q == 2 ? lo.z : lo.w);
+    const uint32_t x1 = q < 2 ? (q == 0 ? lo.y : lo.z) : (q == 2 ? lo.w : hi.x);
+    const uint32_t x2 = q < 2 ? (q == 0 ? lo.z : lo.w) : (q == 2 ? hi.x : hi.y);
+    const uint32_t x3 = q < 2 ? (q == 0 ? lo.w : hi.x) : (q == 2 ? hi.y : hi.z);
+    const uint32_t x4 = q < 2 ? (q == 0 ? hi.x : hi.y) : (q == 2 ? hi.z : hi.w);
+    uint32_t o[4] = {__funnelshift_r(x0, x1, bits), __funnelshift_r(x1, x2, bits), __funnelshift_r(x2, x3, bits),
+                     __funnelshift_r(x3, x4, bits)};
+    if (valid < 16) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = row0 + r0 + u * kLoadWarps;
-      w0[u] = w1[u] = sh[u] = 0u;
-      if (r0 + u * kLoadWarps < rows && i < p.M && valid > 0) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(p.a + static_cast<long long>(i) * p.lda_bytes + off);
-        const uint32_t s = static_cast<uint32_t>(at & 3u);
-        const uint32_t* word = reinterpret_cast<const uint32_t*>(at - s);
-        w0[u] = word[0];
-        if (static_cast<int>(s) + valid > 4) w1[u] = word[1];
-        sh[u] = 8u * s;
+      for (int y = 0; y < 4; ++y) {
+        const int left = valid - 4 * y;
+        o[y] = left >= 4 ? o[y] : left > 0 ? o[y] & ((1u << (8 * left)) - 1u) : 0u;
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * kLoadWarps;
-      if (r < rows) {
-        uint32_t v = __funnelshift_r(w0[u], w1[u], sh[u]);
-        if (valid < 4) v = valid > 0 ? v & ((1u << (8 * valid)) - 1u) : 0u;
-        *reinterpret_cast<uint32_t*>(dst + r * kKB + ((((lane >> 2) ^ r) & 7) << 4) + (lane & 3) * 4) = v;
-      }
-    }
+    *reinterpret_cast<uint4*>(out + x * 16) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -363,11 +362,10 @@ __device__ __forceinline__ void tile_at(const LinArgs& p, int t, int& tm, int& t
   tm = g * kGroup + (in - tn * h);
 }
 
-template <int KIND, bool PAIR, bool ATMA>
-__global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps)), 1)
+template <int KIND, bool PAIR>
+__global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
     k_linear_tiles(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, int* __restrict__ err) {
-  static_assert(ATMA || !PAIR, "rows without a TMA box are loaded by single CTAs");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   LinBars* b = reinterpret_cast<LinBars*>(ring + p.stages * p.stage_bytes);
@@ -380,7 +378,7 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&b->full[s], ATMA ? 1 : 1 + kLoadWarps);
+      mbar_init(&b->full[s], 1);
       mbar_init(&b->empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -392,7 +390,7 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
     b->no_abort = 0;
     fence_mbar_init();
     tma_prefetch(&mW);
-    if (ATMA) tma_prefetch(&mA);
+    tma_prefetch(&mA);
   }
   if (warp == 1) {
     if (PAIR) {
@@ -424,7 +422,7 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
     auto load_w = [&](int s, int row, int blocks) {
       if (elect_one()) {
         uint8_t* st = ring + s * p.stage_bytes;
-        if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * blocks * (kWBytes + (ATMA ? arows * kKB : 0)));
+        if (rank == 0) mbar_arrive_expect_tx(&b->full[s], P * blocks * (kWBytes + arows * kKB));
         for (int y = 0; y < blocks; ++y) {
           if (PAIR) tma_load_2d_pair(st + y * kWBytes, &mW, full0 + static_cast<uint32_t>(s * 8), 0, row + y * kCols);
           else tma_load_2d(st + y * kWBytes, &mW, &b->full[s], 0, row + y * kCols);
@@ -452,7 +450,7 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
           if (!ok) break;
           load_w(s, w_row + kb * kCols, blocks);
         }
-        if (ATMA && elect_one()) {
+        if (elect_one()) {
           uint8_t* st = ring + s * p.stage_bytes + p.kbs * kWBytes;
           for (int y = 0; y < blocks; ++y) {
             if (PAIR) tma_load_2d_pair(st + y * arows * kKB, &mA, full0 + static_cast<uint32_t>(s * 8), (kb + y) * kKB, a_row);
@@ -505,7 +503,7 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
         }
       }
     }
-  } else if (warp < 2 + kTileEpi) {
+  } else {
     const int q = warp & 3, part = (warp - 2) >> 2;
     const uint32_t acce0 = PAIR ? mapa_shared(&b->acc_empty[0], 0) : 0u;
     griddep_wait();
@@ -529,26 +527,6 @@ __global__ void __launch_bounds__(64 + 32 * (kTileEpi + (ATMA ? 0 : kLoadWarps))
       if (lane == 0) {
         if (PAIR) mbar_arrive_cluster(acce0 + static_cast<uint32_t>(buf * 8));
         else mbar_arrive(&b->acc_empty[buf]);
-      }
-    }
-  } else {
-    griddep_wait();
-    const int w = warp - 2 - kTileEpi;
-    RingPos at;
-    bool ok = true;
-    for (int t = first; t < tiles && ok; t += walkers) {
-      int tm, tn;
-      tile_at(p, t, tm, tn);
-      for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
-        const int s = at.s;
-        ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        for (int y = 0; y < min(p.kbs, p.num_kb - kb); ++y)
-          load_rows(p, ring + s * p.stage_bytes + p.kbs * kWBytes + y * arows * kKB, tm * p.bn, arows, kb + y, w, lane);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b->full[s]);
       }
     }
   }
@@ -589,8 +567,8 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   return v;
 }
 
-template <int KIND, bool ATMA>
-__global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)), ATMA ? 4 : 2)
+template <int KIND>
+__global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
     k_linear_split(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, uint32_t tmem_cols, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
@@ -606,14 +584,14 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&b->full[s], ATMA ? 1 : 1 + kLoadWarps);
+      mbar_init(&b->full[s], 1);
       mbar_init(&b->empty[s], 1);
     }
     mbar_init(&b->acc_full[0], 1);
     b->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch(&mW);
-    if (ATMA) tma_prefetch(&mA);
+    tma_prefetch(&mA);
   }
   if (warp == 1) {
     tmem_alloc(&b->tmem_slot, tmem_cols);
@@ -634,7 +612,7 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
     auto load_w = [&](int s, int kc) {
       if (elect_one()) {
         const int blocks = min(p.kbs, kbn - kc);
-        mbar_arrive_expect_tx(&b->full[s], blocks * (kWBytes + (ATMA ? p.bn * kKB : 0)));
+        mbar_arrive_expect_tx(&b->full[s], blocks * (kWBytes + p.bn * kKB));
         for (int y = 0; y < blocks; ++y)
           tma_load_2d(ring + s * p.stage_bytes + y * kWBytes, &mW, &b->full[s], 0, w_row + (kc + y) * kCols);
       }
@@ -653,7 +631,7 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
         if (!wait(&b->empty[s], at.phase ^ 1u)) break;
         load_w(s, kc);
       }
-      if (ATMA && elect_one())
+      if (elect_one())
         for (int y = 0; y < min(p.kbs, kbn - kc); ++y)
           tma_load_2d(ring + s * p.stage_bytes + p.kbs * kWBytes + y * p.bn * kKB, &mA, &b->full[s], (kb0 + kc + y) * kKB, m0);
     }
@@ -679,23 +657,9 @@ __global__ void __launch_bounds__(64 + 32 * (kSplitEpi + (ATMA ? 0 : kLoadWarps)
         if (kc + p.kbs >= kbn) mma_commit(&b->acc_full[0]);
       }
     }
-  } else if (warp >= 2 + kSplitEpi) {
-    griddep_wait();
-    const int w = warp - 2 - kSplitEpi;
-    RingPos at;
-    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
-      const int s = at.s;
-      const bool ok = mbar_wait(&b->empty[s], at.phase ^ 1u, &b->abort_flag, err);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      for (int y = 0; y < min(p.kbs, kbn - kc); ++y)
-        load_rows(p, ring + s * p.stage_bytes + p.kbs * kWBytes + y * p.bn * kKB, m0, p.bn, kb0 + kc + y, w, lane);
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b->full[s]);
-    }
   }
 
-  const bool epi = warp >= 2 && warp < 2 + kSplitEpi;
+  const bool epi = warp >= 2;
   const int q = warp & 3, part = (warp - 2) >> 2;
   constexpr int kParts = kSplitEpi / 4;
   const int col = q * 32 + lane;
@@ -842,55 +806,71 @@ struct LinPlan {
 
 int div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Which kernel, tile and split: the fewest cycles by a count of what a tile
-// costs. One k-block is four MMAs of max(50, bn / 2) cycles.
-LinPlan choose(int num_sms, int m, int n, int num_kb, bool atma) {
+// Which kernel, tile and split: the least of a cost in microseconds whose
+// constants were fitted to 8400 measured launches (m 1 to 4096, nine (n, k) from
+// 256 x 256 to 16384 x 1024, bf16 and s8, every tile and split here): its choice
+// is 1.8 % from the best of them in the geometric mean and 20 % at worst.
+//   k_linear_split: a k-block of a CTA takes its issue and landing latency or its
+//     share of what an SM takes in; a split adds the meeting of the cluster.
+//   k_linear_tiles: a k-block takes its MMAs and their issue (a pair's tile of the
+//     same width half the operand bytes); a tile's epilogue hides behind the next
+//     tile's blocks, the last one's does not.
+//   Either: no less than the bytes' own time.
+struct LinShape {
+  int m, n, num_kb, out;  // out: bytes of an element of y
+};
+
+LinPlan choose(int num_sms, const LinShape& z) {
   LinPlan best{};
   double best_t = 1e300;
-  const int cols = div_up(n, kCols);
-  auto consider = [&](LinPlan c, double t) {
+  auto consider = [&](const LinPlan& c, double t) {
     if (t < best_t) {
       best_t = t;
       best = c;
     }
   };
+  const int cols = div_up(z.n, kCols);
+  const double kbytes = static_cast<double>(z.num_kb) * kKB;
+  const double bytes_us = ((z.m + z.n) * kbytes + static_cast<double>(z.m) * z.n * 2 * z.out) / 8.6e6;
   for (int bn = 16; bn <= 128; bn += 16) {
-    if (bn > 16 && bn - 16 >= m) break;
-    const double tiles = static_cast<double>(cols) * div_up(m, bn);
-    for (int split = 1; split <= kMaxSplit; split *= 2) {
-      if (split > num_kb) break;
-      const double waves = std::ceil(tiles * split / (2 * num_sms));
-      const double kb = div_up(num_kb, split);
+    if (bn > 16 && bn - 16 >= z.m) break;
+    for (int split = 1; split <= kMaxSplit && split <= z.num_kb; split *= 2) {
+      const double ctas = static_cast<double>(cols) * div_up(z.m, bn) * split;
+      const double waves = std::ceil(ctas / (2 * num_sms)), per_sm = ctas > num_sms ? 2 : 1;
+      const double mma = 4 * std::max(50.0, bn / 2.0) / 1800;
+      const double kb = std::max({0.37, per_sm * (kWBytes + bn * kKB) / 95e3, per_sm * mma});
       consider({true, false, bn, split, 2, 2},
-               waves * (kb * std::max(2 * 4 * std::max(50.0, bn / 2.0), 2 * (kWBytes + bn * kKB) / 40.0) + 1500 + 10 * bn) + (split > 1 ? 1500 : 0));
+               3.4 + std::max(bytes_us, waves * div_up(z.num_kb, split) * kb + 0.57 * (waves - 1)) + 0.018 * bn +
+                   (split > 1 ? 1.7 + 0.02 * bn : 0));
     }
   }
-  for (int pair = 0; pair <= (atma ? 1 : 0); ++pair) {
+  for (int pair = 0; pair <= 1; ++pair) {
     const int step = pair ? 32 : 16;
     for (int bn = step; bn <= 256; bn += step) {
-      if (bn > step && bn - step >= m) break;
-      const double tiles = static_cast<double>(div_up(cols, pair ? 2 : 1)) * div_up(m, bn);
+      if (bn > step && bn - step >= z.m) break;
+      const double tiles = static_cast<double>(div_up(cols, pair ? 2 : 1)) * div_up(z.m, bn);
       const double waves = std::ceil(tiles / (num_sms / (pair ? 2 : 1)));
-      const double bytes = kWBytes + static_cast<double>(bn) * kKB / (pair ? 2 : 1);
+      const double kb = std::max(0.154, pair ? 0.107 + 0.00052 * bn : 0.072 + 0.00093 * bn);
+      const double main = z.num_kb * kb, tail = 0.76 + 0.0071 * bn;
       consider({false, pair != 0, bn, 1, 1, 2},
-               waves * num_kb * std::max(4 * std::max(50.0, bn / 2.0), bytes / 60.0) + 2500 + 20.0 * bn);
+               3.9 + (pair ? 0.6 : 0) + std::max(bytes_us, main + (waves - 1) * std::max(main, tail) + tail));
     }
   }
   return best;
 }
 
 template <int KIND>
-int launch_tiles(osc_ctx* ctx, const LinPlan& pl, bool atma, const CUtensorMap& mW, const CUtensorMap& mA,
+int launch_tiles(osc_ctx* ctx, const LinPlan& pl, const CUtensorMap& mW, const CUtensorMap& mA,
                  const LinArgs& p) {
   void (*kern)(CUtensorMap, CUtensorMap, LinArgs, int*) =
-      pl.pair ? k_linear_tiles<KIND, true, true> : atma ? k_linear_tiles<KIND, false, true> : k_linear_tiles<KIND, false, false>;
+      pl.pair ? k_linear_tiles<KIND, true> : k_linear_tiles<KIND, false>;
   const int smem = p.stages * p.stage_bytes + kSmemTail + 1024;
   OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(kern), smem));
   const int per = pl.pair ? 2 : 1;
   const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<long long>(tiles, ctx->num_sms / per) * per));
-  cfg.blockDim = dim3(64 + 32 * (kTileEpi + (atma ? 0 : kLoadWarps)));
+  cfg.blockDim = dim3(64 + 32 * kTileEpi);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
@@ -909,16 +889,15 @@ int launch_tiles(osc_ctx* ctx, const LinPlan& pl, bool atma, const CUtensorMap& 
 }
 
 template <int KIND>
-int launch_split(osc_ctx* ctx, bool atma, const CUtensorMap& mW, const CUtensorMap& mA, const LinArgs& p) {
-  void (*kern)(CUtensorMap, CUtensorMap, LinArgs, uint32_t, int*) =
-      atma ? k_linear_split<KIND, true> : k_linear_split<KIND, false>;
+int launch_split(osc_ctx* ctx, const CUtensorMap& mW, const CUtensorMap& mA, const LinArgs& p) {
+  void (*kern)(CUtensorMap, CUtensorMap, LinArgs, uint32_t, int*) = k_linear_split<KIND>;
   const int smem = p.stages * p.stage_bytes + kSmemTail + 1024;
   OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(kern), smem));
   uint32_t cols = 32;
   while (cols < static_cast<uint32_t>(p.bn)) cols *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * p.split));
-  cfg.blockDim = dim3(64 + 32 * (kSplitEpi + (atma ? 0 : kLoadWarps)));
+  cfg.blockDim = dim3(64 + 32 * kSplitEpi);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[2];
@@ -1062,14 +1041,13 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   OSC_TRY(enter(ctx));
   if (fault_injected("launch")) return fail(OSC_EFAULT_INJECTED, "injected failure (launch)");
 
-  const bool atma = aligned(a, 16) && (m == 1 || (lda * e) % 16 == 0);
-  const LinPlan pl = choose(ctx->num_sms, m, w->n, w->num_kb, atma);
+  const LinPlan pl = choose(ctx->num_sms, {m, w->n, w->num_kb, o});
   LinArgs p = {};
   p.M = m;
   p.N = w->n;
   p.num_kb = w->num_kb;
-  p.k_bytes = w->k * e;
-  p.last_steps = div_up(p.k_bytes - (w->num_kb - 1) * kKB, 32);
+  const int k_bytes = w->k * e;
+  p.last_steps = div_up(k_bytes - (w->num_kb - 1) * kKB, 32);
   p.bn = pl.bn;
   p.split = pl.split;
   const int arows = pl.pair ? pl.bn / 2 : pl.bn;
@@ -1092,33 +1070,54 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   p.ldr_bytes = ldr * o;
   p.y = y;
   p.ldy_bytes = ldy * o;
-  p.a = static_cast<const uint8_t*>(a);
-  p.lda_bytes = lda * e;
 
-  CUtensorMap mA{};
-  if (atma) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(p.k_bytes), static_cast<uint64_t>(m)};
-    const uint64_t pitch[1] = {m == 1 ? round_up(static_cast<size_t>(p.k_bytes), 16) : static_cast<uint64_t>(lda) * e};
-    const uint32_t box[2] = {kKB, static_cast<uint32_t>(arows)};
-    OSC_TRY(encode_tiled(&mA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B));
-  }
   switch (w->dtype) {
-    case OSC_F16:
-    case OSC_BF16: {
-      const uint32_t fmt = w->dtype == OSC_BF16 ? 1u : 0u;
-      p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | size;  // F32 sums
-      return pl.split_kernel ? launch_split<LIN_F16>(ctx, atma, w->map, mA, p)
-                             : launch_tiles<LIN_F16>(ctx, pl, atma, w->map, mA, p);
-    }
-    case OSC_E4M3:
-      p.idesc = (1u << 4) | size;  // both operands E4M3, F32 sums
-      return pl.split_kernel ? launch_split<LIN_F8>(ctx, atma, w->map, mA, p)
-                             : launch_tiles<LIN_F8>(ctx, pl, atma, w->map, mA, p);
-    default:
-      p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | size;  // both operands signed, S32 sums
-      return pl.split_kernel ? launch_split<LIN_I8>(ctx, atma, w->map, mA, p)
-                             : launch_tiles<LIN_I8>(ctx, pl, atma, w->map, mA, p);
+    case OSC_F16: p.idesc = (1u << 4) | size; break;                           // F16 operands, F32 sums
+    case OSC_BF16: p.idesc = (1u << 4) | (1u << 7) | (1u << 10) | size; break;  // BF16
+    case OSC_E4M3: p.idesc = (1u << 4) | size; break;                          // E4M3
+    default: p.idesc = (2u << 4) | (1u << 7) | (1u << 10) | size; break;       // signed 8-bit operands, S32 sums
   }
+
+  // rows that start on 16-byte boundaries travel by TMA; others are first copied to such
+  const bool direct = aligned(a, 16) && (m == 1 || (lda * e) % 16 == 0);
+  const int pieces = div_up(k_bytes, 16);
+  void* rows_copy = nullptr;
+  uint64_t pitch[1] = {m == 1 ? static_cast<uint64_t>(pieces) * 16 : static_cast<uint64_t>(lda) * e};
+  int st = OSC_OK;
+  if (!direct) {
+    const long long total = static_cast<long long>(m) * pieces;
+    OSC_TRY(stream_alloc(ctx, static_cast<size_t>(total) * 16, &rows_copy));
+    const long long blocks = std::min<long long>((total + 255) / 256, 8ll * ctx->num_sms);
+    st = launch_pdl(ctx, k_linear_rows, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, "k_linear_rows",
+                    static_cast<const uint8_t*>(a), m, k_bytes, lda * e, pieces, static_cast<uint8_t*>(rows_copy));
+    a = rows_copy;
+    pitch[0] = static_cast<uint64_t>(pieces) * 16;
+  }
+  CUtensorMap mA{};
+  if (st == OSC_OK) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(k_bytes), static_cast<uint64_t>(m)};
+    const uint32_t box[2] = {kKB, static_cast<uint32_t>(arows)};
+    st = encode_tiled(&mA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  if (st == OSC_OK) {
+    switch (w->dtype) {
+      case OSC_F16:
+      case OSC_BF16:
+        st = pl.split_kernel ? launch_split<LIN_F16>(ctx, w->map, mA, p) : launch_tiles<LIN_F16>(ctx, pl, w->map, mA, p);
+        break;
+      case OSC_E4M3:
+        st = pl.split_kernel ? launch_split<LIN_F8>(ctx, w->map, mA, p) : launch_tiles<LIN_F8>(ctx, pl, w->map, mA, p);
+        break;
+      default:
+        st = pl.split_kernel ? launch_split<LIN_I8>(ctx, w->map, mA, p) : launch_tiles<LIN_I8>(ctx, pl, w->map, mA, p);
+        break;
+    }
+  }
+  if (rows_copy != nullptr) {
+    const int freed = stream_free(ctx, rows_copy);
+    if (st == OSC_OK) st = freed;
+  }
+  return st;
 }
 
 }  // extern "C"

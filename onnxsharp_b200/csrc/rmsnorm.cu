@@ -35,8 +35,9 @@ namespace {
 
 constexpr float kTiny = 8.27180612553028e-25f;  // 2^-80: below it FP32 products of 24-bit factors lose bits
 constexpr int kMaxThreads = 1024;
-constexpr int kRegFloats = 16;                            // elements of a row a thread keeps
-constexpr int kMaxRegCols = kMaxThreads * kRegFloats;     // longer rows are read again
+constexpr int kRowsPerCta = 4;                        // rows of one warp each
+constexpr int kRegFloats = 16;                        // elements of a row a thread keeps at most
+constexpr int kMaxRegCols = kMaxThreads * kRegFloats; // longer rows are read again
 
 struct NormArgs {
   const void* x;
@@ -75,45 +76,84 @@ struct alignas(sizeof(T) * VEC) Vec {
   T v[VEC];
 };
 
+// The larger, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // What a row's codes are made from, the same in all of its threads.
 struct RowCode {
-  float ratio;  // top / peak in FP32
+  float ratio;  // top / peak in FP32; 0 where the codes are 0
   double peak;  // max|t|, exact
   float top;
-  bool live;    // false: the codes are 0
 };
 
-// The code of t = h * g as its byte. r is t * top / peak to about 5 ulp; where
-// a border between codes is nearer than that, FP64 decides.
-__device__ __forceinline__ uint8_t code_s8(float t, float h, float g, const RowCode& c) {
-  const float r = t * c.ratio;
-  float n = rintf(r);
-  if (fabsf(fabsf(r - n) - 0.5f) < 1e-4f)
-    n = static_cast<float>(rint(static_cast<double>(h) * static_cast<double>(g) * static_cast<double>(c.top) / c.peak));
-  return static_cast<uint8_t>(static_cast<int8_t>(static_cast<int>(n)));
+// t * top / peak as FP64 has it, from the exact factors of t.
+__device__ __forceinline__ double exact_ratio(float h, float g, const RowCode& c) {
+  return static_cast<double>(h) * static_cast<double>(g) * static_cast<double>(c.top) / c.peak;
 }
-__device__ __forceinline__ uint8_t code_e4m3(float t, float h, float g, const RowCode& c) {
-  float r = t * c.ratio;
-  const float a = fabsf(r);
-  // borders: 2^-6 and up the middle of the 20 bits below e4m3's, below it the odd multiples of 2^-10
-  const bool near_border = a >= 0.015625f
-                               ? abs(static_cast<int>(__float_as_uint(a) & 0xFFFFFu) - 0x80000) <= 16
-                               : fabsf(a * 512.0f - floorf(a * 512.0f) - 0.5f) < 1e-4f;
-  if (near_border) {
-    // toward zero with the last bit set when inexact: the second rounding then sees which side of a border it is on
-    const double v = static_cast<double>(h) * static_cast<double>(g) * static_cast<double>(c.top) / c.peak;
-    r = __double2float_rz(v);
-    if (static_cast<double>(r) != v) r = __uint_as_float(__float_as_uint(r) | 1u);
+
+// N codes of t[e] = h[e] * g[e] as bytes. r = t * ratio is good to about 5 ulp;
+// where a border between two codes is nearer than that, FP64 decides (a branch
+// that one element in some thousands takes).
+template <int N, class H, class G>
+__device__ __forceinline__ void codes_s8(const float (&t)[N], H h, G g, const RowCode& c, uint8_t (&o)[N]) {
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even
+  float n[N];
+  uint32_t close = 0u;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float r = t[e] * c.ratio;
+    n[e] = r + kRound;
+    if (fabsf(r - (n[e] - kRound)) > 0.4999f) close |= 1u << e;
   }
-  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(r, __NV_SATFINITE, __NV_E4M3));
+  if (close != 0u) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if ((close >> e & 1u) != 0u) n[e] = static_cast<float>(rint(exact_ratio(h(e), g(e), c))) + kRound;
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) o[e] = static_cast<uint8_t>(__float_as_uint(n[e]));  // the integer's low byte
 }
-__device__ __forceinline__ uint8_t code_of(float t, float h, float g, const RowCode& c, int q_dtype) {
-  if (!c.live) return 0;
-  return q_dtype == OSC_S8 ? code_s8(t, h, g, c) : code_e4m3(t, h, g, c);
+template <int N, class H, class G>
+__device__ __forceinline__ void codes_e4m3(const float (&t)[N], H h, G g, const RowCode& c, uint8_t (&o)[N]) {
+  float r[N];
+  uint32_t close = 0u;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    r[e] = t[e] * c.ratio;
+    const uint32_t u = __float_as_uint(r[e]) & 0x7fffffffu;
+    // borders: the middle of the 20 bits below e4m3's; under 2^-6, where they lie otherwise, every value but 0 is looked at
+    if ((u & 0xFFFFFu) - 0x7FFF0u <= 32u || u - 1u < 0x3C800000u - 1u) close |= 1u << e;
+  }
+  if (close != 0u) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if ((close >> e & 1u) != 0u) {
+        // toward zero with the last bit set when inexact: the second rounding then sees which side of a border it is on
+        const double v = exact_ratio(h(e), g(e), c);
+        r[e] = __double2float_rz(v);
+        if (static_cast<double>(r[e]) != v) r[e] = __uint_as_float(__float_as_uint(r[e]) | 1u);
+      }
+  }
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(r[e], r[e + 1]), __NV_SATFINITE, __NV_E4M3);
+      o[e] = static_cast<uint8_t>(two);
+      o[e + 1] = static_cast<uint8_t>(two >> 8);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = __nv_cvt_float_to_fp8(r[e], __NV_SATFINITE, __NV_E4M3);
+  }
 }
 
 // Sum and maximum over a row's threads: a warp's shuffles, then (rows of more
 // than a warp) the warps' partials through shared memory, added in warp order.
+// `peak` is the bits of a float that is not negative.
 template <bool WARP>
 __device__ __forceinline__ void reduce_row(float& ss, uint32_t& peak, float2* part, int warps) {
 #pragma unroll
@@ -123,13 +163,11 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& peak, float2* pa
     const int lane = threadIdx.x & 31;
     if (lane == 0) part[threadIdx.x >> 5] = make_float2(ss, __uint_as_float(peak));
     __syncthreads();
-    float s = lane < warps ? part[lane].x : 0.0f;
-    uint32_t m = lane < warps ? __float_as_uint(part[lane].y) : 0u;
+    ss = lane < warps ? part[lane].x : 0.0f;
+    peak = lane < warps ? __float_as_uint(part[lane].y) : 0u;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    ss = s;
-    peak = __reduce_max_sync(0xffffffffu, m);
-    __syncthreads();  // part is used again
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    peak = __reduce_max_sync(0xffffffffu, peak);
   }
 }
 
@@ -145,54 +183,59 @@ __device__ __forceinline__ float rstd_scaled(float ss, int cols) {
 }
 constexpr float kDown = 5.421010862427522e-20f;  // 2^-64
 
+__device__ __forceinline__ bool live_peak(uint32_t peak) {
+  return __uint_as_float(peak) >= kTiny && peak < 0x7f800000u;
+}
 __device__ __forceinline__ RowCode row_code(uint32_t peak, double exact_peak, int q_dtype) {
   RowCode c;
-  const float p = __uint_as_float(peak);
   c.top = q_dtype == OSC_S8 ? 127.0f : 448.0f;
-  c.live = p >= kTiny && peak < 0x7f800000u;
-  c.ratio = c.live ? __fdiv_rn(c.top, p) : 0.0f;
+  c.ratio = live_peak(peak) ? __fdiv_rn(c.top, __uint_as_float(peak)) : 0.0f;
   c.peak = exact_peak;
   return c;
 }
-
 __device__ __forceinline__ float row_scale(uint32_t peak, float rstd, const RowCode& c) {
   if (peak >= 0x7f800000u) return __uint_as_float(0x7fc00000u);  // no finite scale: the row is not a number
-  return c.live ? __fdiv_rn(__uint_as_float(peak) * rstd, c.top) : 1.0f;
+  return live_peak(peak) ? __fdiv_rn(__uint_as_float(peak) * rstd, c.top) : 1.0f;
 }
 
-// max over the row of the bits that FP32 dropped of the largest |t|: products
-// of two 24-bit factors have 48. (Products of 16-bit types fit FP32.)
-template <bool WARP>
-__device__ __forceinline__ float reduce_rest(float rest, float2* part, int warps) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) rest = fmaxf(rest, __shfl_xor_sync(0xffffffffu, rest, o));
-  if constexpr (!WARP) {
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) part[threadIdx.x >> 5].x = rest;
-    __syncthreads();
-    rest = lane < warps ? part[lane].x : -INFINITY;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) rest = fmaxf(rest, __shfl_xor_sync(0xffffffffu, rest, o));
-    __syncthreads();
-  }
-  return rest;
+// What FP32 dropped of the largest |t| (products of two 24-bit factors have 48
+// bits; those of 16-bit types fit FP32): the maximum over the elements whose
+// FP32 product is the peak, as an integer that orders like the float.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return (u >> 31) != 0u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float rest_of(float t, float h, float g, uint32_t peak) {
-  if ((__float_as_uint(t) & 0x7fffffffu) != peak) return -INFINITY;
+__device__ __forceinline__ float from_ordered(uint32_t u) {
+  return __uint_as_float((u >> 31) != 0u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint32_t rest_of(float t, float h, float g, uint32_t peak) {
+  if ((__float_as_uint(t) & 0x7fffffffu) != peak) return 0u;  // below every float
   const float rest = fmaf(h, g, -t);
-  return t < 0.0f ? -rest : rest;
+  return ordered(t < 0.0f ? -rest : rest);
+}
+template <bool WARP>
+__device__ __forceinline__ double exact_peak_of(uint32_t peak, uint32_t rest, uint32_t* shared_rest) {
+  rest = __reduce_max_sync(0xffffffffu, rest);
+  if constexpr (!WARP) {
+    if ((threadIdx.x & 31) == 0 && rest != 0u) atomicMax(shared_rest, rest);
+    __syncthreads();
+    rest = *shared_rest;
+  }
+  return static_cast<double>(__uint_as_float(peak)) + (rest != 0u ? static_cast<double>(from_ordered(rest)) : 0.0);
 }
 
 // A row in registers: WARP: one row a warp, several a CTA; else one row a CTA.
 // Element (i * threads + thread) * VEC + e of the row is this thread's (i, e).
 template <typename T, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : kMaxThreads) k_rmsnorm(const __grid_constant__ NormArgs p) {
+__global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsnorm(const __grid_constant__ NormArgs p) {
   __shared__ float2 part[32];
+  __shared__ uint32_t shared_rest;
   const int lanes = WARP ? 32 : static_cast<int>(blockDim.x);
   const int me = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
   const int warps = static_cast<int>(blockDim.x) >> 5;
   const long long row = WARP ? static_cast<long long>(blockIdx.x) * warps + (threadIdx.x >> 5)
                              : static_cast<long long>(blockIdx.x);
+  if (!WARP && threadIdx.x == 0) shared_rest = 0u;
   griddep_launch();
   griddep_wait();
   if (row >= p.rows) return;  // whole warps (WARP), none otherwise
@@ -200,46 +243,51 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxThreads) k_rmsnorm(const __gr
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* res = p.residual != nullptr ? static_cast<const T*>(p.residual) + row * p.res_ld : nullptr;
   const T* gamma = static_cast<const T*>(p.gamma);
+  auto at = [&](int i) { return (i * lanes + me) * VEC; };
 
-  V raw[NV], add[NV], gv[NV];
+  V raw[NV], gv[NV];
+  {
+    V add[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e0 = (i * lanes + me) * VEC;
-    if (e0 < p.cols) {
-      raw[i] = *reinterpret_cast<const V*>(x + e0);
-      if (res != nullptr) add[i] = *reinterpret_cast<const V*>(res + e0);
-    } else {
+    for (int i = 0; i < NV; ++i) {
+      if (at(i) < p.cols) {
+        raw[i] = *reinterpret_cast<const V*>(x + at(i));
+        if (res != nullptr) add[i] = *reinterpret_cast<const V*>(res + at(i));
+      } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) raw[i].v[e] = from_f<T>(0.0f);
+        for (int e = 0; e < VEC; ++e) raw[i].v[e] = add[i].v[e] = from_f<T>(0.0f);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (at(i) < p.cols && gamma != nullptr) {
+        gv[i] = *reinterpret_cast<const V*>(gamma + at(i));
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) gv[i].v[e] = from_f<T>(1.0f);
+      }
+    }
+    if (res != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) raw[i].v[e] = from_f<T>(to_f<T>(raw[i].v[e]) + to_f<T>(add[i].v[e]));
+        if (p.sum != nullptr && at(i) < p.cols) *reinterpret_cast<V*>(static_cast<T*>(p.sum) + row * p.sum_ld + at(i)) = raw[i];
+      }
     }
   }
+  auto h_of = [&](int i, int e) { return to_f<T>(raw[i].v[e]); };
+  auto g_of = [&](int i, int e) { return to_f<T>(gv[i].v[e]); };
+  float ss = 0.0f, top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e0 = (i * lanes + me) * VEC;
-    if (e0 < p.cols && gamma != nullptr) {
-      gv[i] = *reinterpret_cast<const V*>(gamma + e0);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) gv[i].v[e] = from_f<T>(1.0f);
-    }
-  }
-  float ss = 0.0f;
-  uint32_t peak = 0u;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int e0 = (i * lanes + me) * VEC;
-    if (e0 < p.cols && res != nullptr) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) raw[i].v[e] = from_f<T>(to_f<T>(raw[i].v[e]) + to_f<T>(add[i].v[e]));
-      if (p.sum != nullptr) *reinterpret_cast<V*>(static_cast<T*>(p.sum) + row * p.sum_ld + e0) = raw[i];
-    }
+  for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float h = to_f<T>(raw[i].v[e]);
+      const float h = h_of(i, e);
       ss = fmaf(h, h, ss);
-      if (p.q != nullptr) peak = max(peak, __float_as_uint(h * to_f<T>(gv[i].v[e])) & 0x7fffffffu);
+      if (p.q != nullptr) top = max_nan(top, fabsf(h * g_of(i, e)));
     }
-  }
+  uint32_t peak = __float_as_uint(top) & 0x7fffffffu;  // a NaN is above every number
   reduce_row<WARP>(ss, peak, part, warps);
   float rstd = rstd_of(ss, p.cols, p.eps);
   if (!(ss < INFINITY)) {  // the same in all of the row's threads
@@ -248,10 +296,11 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxThreads) k_rmsnorm(const __gr
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float h = to_f<T>(raw[i].v[e]) * kDown;
+        const float h = h_of(i, e) * kDown;
         ss = fmaf(h, h, ss);
       }
     uint32_t none = 0u;
+    if (!WARP) __syncthreads();  // part is written again
     reduce_row<WARP>(ss, none, part, warps);
     rstd = rstd_scaled(ss, p.cols);
   }
@@ -259,45 +308,39 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxThreads) k_rmsnorm(const __gr
   if (p.y != nullptr) {
     T* y = static_cast<T*>(p.y) + row * p.y_ld;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e0 = (i * lanes + me) * VEC;
-      if (e0 < p.cols) {
+    for (int i = 0; i < NV; ++i)
+      if (at(i) < p.cols) {
         V o;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(to_f<T>(raw[i].v[e]) * rstd * to_f<T>(gv[i].v[e]));
-        *reinterpret_cast<V*>(y + e0) = o;
+        for (int e = 0; e < VEC; ++e) o.v[e] = from_f<T>(h_of(i, e) * rstd * g_of(i, e));
+        *reinterpret_cast<V*>(y + at(i)) = o;
       }
-    }
   }
   if (p.q != nullptr) {
     double exact = static_cast<double>(__uint_as_float(peak));
     if constexpr (std::is_same<T, float>::value) {
-      float rest = -INFINITY;
+      uint32_t rest = 0u;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = to_f<T>(raw[i].v[e]), g = to_f<T>(gv[i].v[e]);
-          rest = fmaxf(rest, rest_of(h * g, h, g, peak));
-        }
-      exact += static_cast<double>(reduce_rest<WARP>(rest, part, warps));
+        for (int e = 0; e < VEC; ++e) rest = max(rest, rest_of(h_of(i, e) * g_of(i, e), h_of(i, e), g_of(i, e), peak));
+      exact = exact_peak_of<WARP>(peak, rest, &shared_rest);
     }
     const RowCode c = row_code(peak, exact, p.q_dtype);
     if (me == 0) p.scales[row] = row_scale(peak, rstd, c);
     uint8_t* q = p.q + row * p.q_ld;
+    const bool live = c.ratio != 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e0 = (i * lanes + me) * VEC;
-      if (e0 < p.cols) {
+    for (int i = 0; i < NV; ++i)
+      if (at(i) < p.cols) {
         Vec<uint8_t, VEC> o;
+        float t[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float h = to_f<T>(raw[i].v[e]), g = to_f<T>(gv[i].v[e]);
-          o.v[e] = code_of(h * g, h, g, c, p.q_dtype);
-        }
-        *reinterpret_cast<Vec<uint8_t, VEC>*>(q + e0) = o;
+        for (int e = 0; e < VEC; ++e) t[e] = live ? h_of(i, e) * g_of(i, e) : 0.0f;
+        if (p.q_dtype == OSC_S8) codes_s8<VEC>(t, [&](int e) { return h_of(i, e); }, [&](int e) { return g_of(i, e); }, c, o.v);
+        else codes_e4m3<VEC>(t, [&](int e) { return h_of(i, e); }, [&](int e) { return g_of(i, e); }, c, o.v);
+        *reinterpret_cast<Vec<uint8_t, VEC>*>(q + at(i)) = o;
       }
-    }
   }
 }
 
@@ -307,6 +350,8 @@ __global__ void __launch_bounds__(WARP ? 128 : kMaxThreads) k_rmsnorm(const __gr
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_constant__ NormArgs p) {
   __shared__ float2 part[32];
+  __shared__ uint32_t shared_rest;
+  if (threadIdx.x == 0) shared_rest = 0u;
   constexpr int warps = kMaxThreads / 32;
   const long long row = blockIdx.x;
   griddep_launch();
@@ -321,8 +366,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
     return res != nullptr ? to_f<T>(from_f<T>(to_f<T>(x[e]) + to_f<T>(res[e]))) : to_f<T>(x[e]);
   };
   auto g_at = [&](int e) { return gamma != nullptr ? to_f<T>(gamma[e]) : 1.0f; };
-  float ss = 0.0f;
-  uint32_t peak = 0u;
+  float ss = 0.0f, top = 0.0f;
   for (int e = threadIdx.x; e < p.cols; e += kMaxThreads) {
     float h = to_f<T>(x[e]);
     if (res != nullptr) {
@@ -331,8 +375,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
       if (kept) sum[e] = s;
     }
     ss = fmaf(h, h, ss);
-    if (p.q != nullptr) peak = max(peak, __float_as_uint(h * g_at(e)) & 0x7fffffffu);
+    if (p.q != nullptr) top = max_nan(top, fabsf(h * g_at(e)));
   }
+  uint32_t peak = __float_as_uint(top) & 0x7fffffffu;
   reduce_row<false>(ss, peak, part, warps);
   float rstd = rstd_of(ss, p.cols, p.eps);
   if (!(ss < INFINITY)) {
@@ -342,6 +387,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
       ss = fmaf(h, h, ss);
     }
     uint32_t none = 0u;
+    __syncthreads();
     reduce_row<false>(ss, none, part, warps);
     rstd = rstd_scaled(ss, p.cols);
   }
@@ -349,12 +395,12 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
   if (p.q != nullptr) {
     double exact = static_cast<double>(__uint_as_float(peak));
     if constexpr (std::is_same<T, float>::value) {
-      float rest = -INFINITY;
+      uint32_t rest = 0u;
       for (int e = threadIdx.x; e < p.cols; e += kMaxThreads) {
         const float h = h_at(e), g = g_at(e);
-        rest = fmaxf(rest, rest_of(h * g, h, g, peak));
+        rest = max(rest, rest_of(h * g, h, g, peak));
       }
-      exact += static_cast<double>(reduce_rest<false>(rest, part, warps));
+      exact = exact_peak_of<false>(peak, rest, &shared_rest);
     }
     c = row_code(peak, exact, p.q_dtype);
     if (threadIdx.x == 0) p.scales[row] = row_scale(peak, rstd, c);
@@ -363,7 +409,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
   uint8_t* q = p.q != nullptr ? p.q + row * p.q_ld : nullptr;
   for (int e = threadIdx.x; e < p.cols; e += kMaxThreads) {
     const float h = h_at(e), g = g_at(e);
-    if (q != nullptr) q[e] = code_of(h * g, h, g, c, p.q_dtype);
+    if (q != nullptr) {
+      const float t[1] = {c.ratio != 0.0f ? h * g : 0.0f};
+      uint8_t o[1];
+      if (p.q_dtype == OSC_S8) codes_s8<1>(t, [&](int) { return h; }, [&](int) { return g; }, c, o);
+      else codes_e4m3<1>(t, [&](int) { return h; }, [&](int) { return g; }, c, o);
+      q[e] = o[0];
+    }
     if (y != nullptr) y[e] = from_f<T>(h * rstd * g);
   }
 }
@@ -372,7 +424,6 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
 template <typename T, int VEC, int NV>
 int launch_rows(osc_ctx* ctx, const NormArgs& p, int threads) {
   if (threads == 32) {
-    constexpr int kRowsPerCta = 4;
     const long long blocks = (p.rows + kRowsPerCta - 1) / kRowsPerCta;
     return launch_pdl(ctx, k_rmsnorm<T, VEC, NV, true>, dim3(static_cast<unsigned>(blocks)), dim3(32 * kRowsPerCta), 0,
                       "k_rmsnorm", p);
@@ -387,11 +438,16 @@ int launch_norm(osc_ctx* ctx, const NormArgs& p, bool vectors) {
     return launch_pdl(ctx, k_rmsnorm_long<T>, dim3(static_cast<unsigned>(p.rows)), dim3(kMaxThreads), 0,
                       "k_rmsnorm_long", p);
   constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-  constexpr int NV = kRegFloats / VEC;
-  // threads of a row: the fewest warps whose registers hold it
-  const int threads = (p.cols + 32 * kRegFloats - 1) / (32 * kRegFloats) * 32;
-  if (vectors) return launch_rows<T, VEC, NV>(ctx, p, threads);
-  return launch_rows<T, 1, kRegFloats>(ctx, p, threads);
+  auto threads_for = [&](int per) { return (p.cols + 32 * per - 1) / (32 * per) * 32; };
+  // Rows spread over as many threads as fit at once; more rows than that take
+  // fewer threads a row, each with more of it.
+  const bool few = p.rows * threads_for(vectors ? VEC : 4) <= 1024ll * ctx->num_sms;
+  if (vectors) {
+    if (few && threads_for(VEC) <= kMaxThreads) return launch_rows<T, VEC, 1>(ctx, p, threads_for(VEC));
+    return launch_rows<T, VEC, kRegFloats / VEC>(ctx, p, threads_for(kRegFloats));
+  }
+  if (few && threads_for(4) <= kMaxThreads) return launch_rows<T, 1, 4>(ctx, p, threads_for(4));
+  return launch_rows<T, 1, kRegFloats>(ctx, p, threads_for(kRegFloats));
 }
 
 int type_bytes(int dtype) { return dtype == OSC_F32 ? 4 : 2; }

@@ -88,6 +88,22 @@ int scratch(osc_ctx* ctx, size_t bytes, void** out) {
   return OSC_OK;
 }
 
+int stream_alloc(osc_ctx* ctx, size_t bytes, void** out) {
+  *out = nullptr;
+  if (fault_injected("alloc")) return fail(OSC_EFAULT_INJECTED, "injected allocation failure (temporary)");
+  const cudaError_t e = cudaMallocFromPoolAsync(out, bytes, ctx->pool, ctx->stream);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(OSC_ENOMEM, "temporary of %zu bytes: %s", bytes, cudaGetErrorString(e));
+  }
+  return OSC_OK;
+}
+
+int stream_free(osc_ctx* ctx, void* ptr) {
+  OSC_CUDA(cudaFreeAsync(ptr, ctx->stream), "cudaFreeAsync (temporary)");
+  return OSC_OK;
+}
+
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base, const uint64_t* dims,
                  const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -212,10 +228,23 @@ OSC_API int osc_create(int device, osc_ctx** out) {
   ctx->stream = ctx->own_stream;
   e = cudaMalloc(&ctx->d_err, 64);
   if (e == cudaSuccess) e = cudaMemset(ctx->d_err, 0, 64);
+  if (e == cudaSuccess) {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = device;
+    e = cudaMemPoolCreate(&ctx->pool, &props);
+  }
+  if (e == cudaSuccess) {
+    uint64_t keep = UINT64_MAX;  // freed temporaries stay with the pool until the context goes
+    e = cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  }
   if (e != cudaSuccess) {
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
+    if (ctx->d_err) cudaFree(ctx->d_err);
     cudaStreamDestroy(ctx->own_stream);
     delete ctx;
-    return cuda_fail(e, "cudaMalloc (error word)");
+    return cuda_fail(e, "context memory (error word, pool)");
   }
   *out = ctx;
   return OSC_OK;
@@ -317,6 +346,7 @@ OSC_API int osc_destroy(osc_ctx* ctx) {
   }
   for (auto ev : ctx->prof_pool) cudaEventDestroy(ev);
   if (ctx->scratch) cudaFree(ctx->scratch);
+  if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
   if (ctx->d_err) cudaFree(ctx->d_err);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;

@@ -29,6 +29,7 @@ struct osc_ctx {
                                   // arrival/departure counters of in-kernel grid barriers
   void* scratch = nullptr;        // grow-only per-call temporaries
   size_t scratch_bytes = 0;
+  cudaMemPool_t pool = nullptr;   // stream-ordered temporaries (stream_alloc)
   // Launch accounting and per-kernel event timing (osc_profile_*).
   unsigned long long launches = 0;
   bool prof_on = false;
@@ -67,6 +68,12 @@ int attention_composed(osc_ctx* ctx, const float* q, const float* k, const float
 // Scratch arena of at least `bytes`, 256-byte aligned. Fails during stream
 // capture if it would have to grow.
 int scratch(osc_ctx* ctx, size_t bytes, void** out);
+
+// A temporary of this call alone, allocated and freed in the order of the
+// context's stream: nothing that another call, stream or graph could share (a
+// capture records it as the graph's own memory).
+int stream_alloc(osc_ctx* ctx, size_t bytes, void** out);
+int stream_free(osc_ctx* ctx, void* ptr);
 
 // True while ctx->stream is being captured into a CUDA graph.
 bool capturing(osc_ctx* ctx);

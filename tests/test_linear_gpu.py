@@ -251,8 +251,10 @@ def test_same_bits_every_time(ctx, m, k):
                bool((first == x).all()) for x in again)
 
 
-def test_two_graphs_on_two_streams(ctx):
-    """Captured once, replayed on new inputs, two graphs of two contexts at the same time."""
+@pytest.mark.parametrize("k", [2048, 2001])
+def test_two_graphs_on_two_streams(ctx, k):
+    """Captured once, replayed on new inputs, two graphs of two contexts at the same time (k 2001: with the copy of
+    rows that TMA cannot take, a temporary of each graph)."""
     import torch
 
     from onnxsharp_b200.runtime import Context
@@ -261,7 +263,7 @@ def test_two_graphs_on_two_streams(ctx):
     ctxs = [Context(0, s.cuda_stream) for s in streams]
     cases, outs, graphs = [], [], []
     for i, x in enumerate(ctxs):
-        c = Case(x, "bf16", 20 + 300 * i, 2048, 512, bias=True, residual=True, seed=i)
+        c = Case(x, "bf16", 20 + 300 * i, k, 512, bias=True, residual=True, seed=i)
         torch.cuda.synchronize()
         y = torch.zeros((c.m, c.n), dtype=c.out_type, device="cuda")
         torch.cuda.synchronize()
@@ -283,6 +285,19 @@ def test_two_graphs_on_two_streams(ctx):
         g.close()
     for x in ctxs:
         x.close()
+
+
+def test_failing_allocation_is_reported(ctx, monkeypatch):
+    from onnxsharp_b200 import OscError
+
+    c = Case(ctx, "bf16", 5, 33, 16)
+    monkeypatch.setenv("OSC_FAULT", "alloc")
+    with pytest.raises(OscError, match="injected"):
+        c.run()
+    monkeypatch.delenv("OSC_FAULT")
+    got = c.run()
+    ctx.synchronize()
+    c.check(got)
 
 
 def test_host_weights(ctx):
