@@ -18,8 +18,13 @@
 // could decide (one element in some thousands) it is settled in FP64.
 //
 // One pass over the data: a row stays in the registers of its warp (short
-// rows) or CTA. Bandwidth bounds it from a few hundred rows on, launch latency
-// below.
+// rows) or CTA, 16 elements a thread (8 or 32 of a 16-bit type: 61.6 and 107 us
+// in place of 53.5 for 8192 rows of 4096 bf16 with a residual; CTAs that walk
+// rows, loading the next ahead, 84). Launch latency bounds a few rows: 1.9 us for
+// one of 4096. Of 8192 rows of 4096, f32 reaches 6.3 TB/s (42.5 us); bf16 with a
+// residual 5.1 (52.5 us), with e4m3 codes 3.7 (64 us): a thread's 16 elements
+// are then too little beside a row's own steps (its sum over warps, its scale),
+// and the codes' arithmetic fills 60 % of the issue slots.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -36,8 +41,7 @@ namespace {
 constexpr float kTiny = 8.27180612553028e-25f;  // 2^-80: below it FP32 products of 24-bit factors lose bits
 constexpr int kMaxThreads = 1024;
 constexpr int kRowsPerCta = 4;                        // rows of one warp each
-constexpr int kRegFloats = 16;                        // elements of a row a thread keeps at most
-constexpr int kMaxRegCols = kMaxThreads * kRegFloats; // longer rows are read again
+constexpr int kSingles = 8;                           // elements, where they are loaded one by one
 
 struct NormArgs {
   const void* x;
@@ -95,43 +99,48 @@ __device__ __forceinline__ double exact_ratio(float h, float g, const RowCode& c
   return static_cast<double>(h) * static_cast<double>(g) * static_cast<double>(c.top) / c.peak;
 }
 
-// N codes of t[e] = h[e] * g[e] as bytes. r = t * ratio is good to about 5 ulp;
-// where a border between two codes is nearer than that, FP64 decides (a branch
-// that one element in some thousands takes).
-template <int N, class H, class G>
-__device__ __forceinline__ void codes_s8(const float (&t)[N], H h, G g, const RowCode& c, uint8_t (&o)[N]) {
+// N codes of t(e) = h(e) * g(e) as bytes. r = t * ratio is good to about 5 ulp;
+// where a border between two codes is nearer than that, FP64 decides. Whether
+// any of the N is that near is one minimum or maximum, so the branch is taken
+// once for all of them (for one group in some hundreds).
+template <int N, class Tt, class H, class G>
+__device__ __forceinline__ void codes_s8(Tt t, H h, G g, const RowCode& c, uint8_t (&o)[N]) {
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even
-  float n[N];
-  uint32_t close = 0u;
+  constexpr float kNear = 0.4999f;
+  float n[N], far = 0.0f;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float r = t[e] * c.ratio;
+    const float r = t(e) * c.ratio;
     n[e] = r + kRound;
-    if (fabsf(r - (n[e] - kRound)) > 0.4999f) close |= 1u << e;
+    far = fmaxf(far, fabsf(r - (n[e] - kRound)));
   }
-  if (close != 0u) {
+  if (far > kNear) {
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if ((close >> e & 1u) != 0u) n[e] = static_cast<float>(rint(exact_ratio(h(e), g(e), c))) + kRound;
+    for (int e = 0; e < N; ++e) {
+      const float r = t(e) * c.ratio;
+      if (fabsf(r - (n[e] - kRound)) > kNear) n[e] = static_cast<float>(rint(exact_ratio(h(e), g(e), c))) + kRound;
+    }
   }
 #pragma unroll
   for (int e = 0; e < N; ++e) o[e] = static_cast<uint8_t>(__float_as_uint(n[e]));  // the integer's low byte
 }
-template <int N, class H, class G>
-__device__ __forceinline__ void codes_e4m3(const float (&t)[N], H h, G g, const RowCode& c, uint8_t (&o)[N]) {
-  float r[N];
-  uint32_t close = 0u;
+template <int N, class Tt, class H, class G>
+__device__ __forceinline__ void codes_e4m3(Tt t, H h, G g, const RowCode& c, uint8_t (&o)[N]) {
+  // 0 where the 20 bits below e4m3's are within 16 of their middle, a border from 2^-6 up
+  auto off_middle = [](float r) { return ((__float_as_uint(r) + 16u) & 0xFFFE0u) ^ 0x80000u; };
+  constexpr float kSmall = 0.015625f;  // 2^-6: under it the borders lie otherwise, and every value but 0 is looked at
+  float r[N], least = kSmall;
+  uint32_t middle = 1u;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    r[e] = t[e] * c.ratio;
-    const uint32_t u = __float_as_uint(r[e]) & 0x7fffffffu;
-    // borders: the middle of the 20 bits below e4m3's; under 2^-6, where they lie otherwise, every value but 0 is looked at
-    if ((u & 0xFFFFFu) - 0x7FFF0u <= 32u || u - 1u < 0x3C800000u - 1u) close |= 1u << e;
+    r[e] = t(e) * c.ratio;
+    least = fminf(least, fabsf(r[e]));
+    middle = min(middle, off_middle(r[e]));
   }
-  if (close != 0u) {
+  if (least < kSmall || middle == 0u) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if ((close >> e & 1u) != 0u) {
+      if (off_middle(r[e]) == 0u || (fabsf(r[e]) < kSmall && r[e] != 0.0f)) {
         // toward zero with the last bit set when inexact: the second rounding then sees which side of a border it is on
         const double v = exact_ratio(h(e), g(e), c);
         r[e] = __double2float_rz(v);
@@ -150,15 +159,27 @@ __device__ __forceinline__ void codes_e4m3(const float (&t)[N], H h, G g, const 
     for (int e = 0; e < N; ++e) o[e] = __nv_cvt_float_to_fp8(r[e], __NV_SATFINITE, __NV_E4M3);
   }
 }
+// A row that has no codes (its ratio is 0): zeros, whatever t is.
+template <int N, class Tt, class H, class G>
+__device__ __forceinline__ void codes_of(Tt t, H h, G g, const RowCode& c, int q_dtype, uint8_t (&o)[N]) {
+  if (c.ratio == 0.0f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0;
+  } else if (q_dtype == OSC_S8) {
+    codes_s8<N>(t, h, g, c, o);
+  } else {
+    codes_e4m3<N>(t, h, g, c, o);
+  }
+}
 
 // Sum and maximum over a row's threads: a warp's shuffles, then (rows of more
 // than a warp) the warps' partials through shared memory, added in warp order.
 // `peak` is the bits of a float that is not negative.
-template <bool WARP>
+template <bool WARP, bool PEAK>
 __device__ __forceinline__ void reduce_row(float& ss, uint32_t& peak, float2* part, int warps) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  peak = __reduce_max_sync(0xffffffffu, peak);
+  if (PEAK) peak = __reduce_max_sync(0xffffffffu, peak);
   if constexpr (!WARP) {
     const int lane = threadIdx.x & 31;
     if (lane == 0) part[threadIdx.x >> 5] = make_float2(ss, __uint_as_float(peak));
@@ -167,7 +188,7 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& peak, float2* pa
     peak = lane < warps ? __float_as_uint(part[lane].y) : 0u;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    peak = __reduce_max_sync(0xffffffffu, peak);
+    if (PEAK) peak = __reduce_max_sync(0xffffffffu, peak);
   }
 }
 
@@ -224,60 +245,64 @@ __device__ __forceinline__ double exact_peak_of(uint32_t peak, uint32_t rest, ui
   return static_cast<double>(__uint_as_float(peak)) + (rest != 0u ? static_cast<double>(from_ordered(rest)) : 0.0);
 }
 
-// A row in registers: WARP: one row a warp, several a CTA; else one row a CTA.
-// Element (i * threads + thread) * VEC + e of the row is this thread's (i, e).
-template <typename T, int VEC, int NV, bool WARP>
+// A row a warp (WARP) or a row a CTA, held in registers: element
+// (i * lanes + me) * VEC + e is this thread's (i, e). Codes are a kernel of their
+// own (CODES, y beside them if asked for): without them it needs fewer registers,
+// and 8192 rows of 4096 bf16 with a residual take 52.1 us for 55.7.
+template <typename T, int VEC, int NV, bool WARP, bool CODES>
 __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsnorm(const __grid_constant__ NormArgs p) {
+  using V = Vec<T, VEC>;
+  constexpr bool kKeep = sizeof(T) == 2;  // t is kept where it takes more than a product to have it again
   __shared__ float2 part[32];
   __shared__ uint32_t shared_rest;
-  const int lanes = WARP ? 32 : static_cast<int>(blockDim.x);
-  const int me = WARP ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
   const int warps = static_cast<int>(blockDim.x) >> 5;
   const long long row = WARP ? static_cast<long long>(blockIdx.x) * warps + (threadIdx.x >> 5)
                              : static_cast<long long>(blockIdx.x);
-  if (!WARP && threadIdx.x == 0) shared_rest = 0u;
+  if (!WARP && threadIdx.x == 0) shared_rest = 0u;  // (used behind the row's meeting)
   griddep_launch();
   griddep_wait();
   if (row >= p.rows) return;  // whole warps (WARP), none otherwise
-  using V = Vec<T, VEC>;
+  const int lanes = WARP ? 32 : static_cast<int>(blockDim.x);
+  const int me = static_cast<int>(WARP ? threadIdx.x & 31 : threadIdx.x);
+  auto at = [&](int i) { return (i * lanes + me) * VEC; };
+
+  V raw[NV], add[NV], gv[NV];
   const T* x = static_cast<const T*>(p.x) + row * p.x_ld;
   const T* res = p.residual != nullptr ? static_cast<const T*>(p.residual) + row * p.res_ld : nullptr;
   const T* gamma = static_cast<const T*>(p.gamma);
-  auto at = [&](int i) { return (i * lanes + me) * VEC; };
-
-  V raw[NV], gv[NV];
-  {
-    V add[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (at(i) < p.cols) {
-        raw[i] = *reinterpret_cast<const V*>(x + at(i));
-        if (res != nullptr) add[i] = *reinterpret_cast<const V*>(res + at(i));
-      } else {
+  for (int i = 0; i < NV; ++i) {
+    if (at(i) < p.cols) {
+      raw[i] = *reinterpret_cast<const V*>(x + at(i));
+      if (res != nullptr) add[i] = *reinterpret_cast<const V*>(res + at(i));
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) raw[i].v[e] = add[i].v[e] = from_f<T>(0.0f);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (at(i) < p.cols && gamma != nullptr) {
-        gv[i] = *reinterpret_cast<const V*>(gamma + at(i));
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) gv[i].v[e] = from_f<T>(1.0f);
-      }
-    }
-    if (res != nullptr) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) raw[i].v[e] = from_f<T>(to_f<T>(raw[i].v[e]) + to_f<T>(add[i].v[e]));
-        if (p.sum != nullptr && at(i) < p.cols) *reinterpret_cast<V*>(static_cast<T*>(p.sum) + row * p.sum_ld + at(i)) = raw[i];
-      }
+      for (int e = 0; e < VEC; ++e) raw[i].v[e] = add[i].v[e] = from_f<T>(0.0f);
     }
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (at(i) < p.cols && gamma != nullptr) {
+      gv[i] = *reinterpret_cast<const V*>(gamma + at(i));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) gv[i].v[e] = from_f<T>(1.0f);
+    }
+  }
+  if (res != nullptr) {
+    T* sum = p.sum != nullptr ? static_cast<T*>(p.sum) + row * p.sum_ld : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) raw[i].v[e] = from_f<T>(to_f<T>(raw[i].v[e]) + to_f<T>(add[i].v[e]));
+      if (sum != nullptr && at(i) < p.cols) *reinterpret_cast<V*>(sum + at(i)) = raw[i];
+    }
+  }
+
   auto h_of = [&](int i, int e) { return to_f<T>(raw[i].v[e]); };
   auto g_of = [&](int i, int e) { return to_f<T>(gv[i].v[e]); };
+  float t[kKeep ? NV : 1][kKeep ? VEC : 1] = {};
+  auto t_of = [&](int i, int e) { return kKeep ? t[kKeep ? i : 0][kKeep ? e : 0] : h_of(i, e) * g_of(i, e); };
   float ss = 0.0f, top = 0.0f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -285,10 +310,13 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsno
     for (int e = 0; e < VEC; ++e) {
       const float h = h_of(i, e);
       ss = fmaf(h, h, ss);
-      if (p.q != nullptr) top = max_nan(top, fabsf(h * g_of(i, e)));
+      if (CODES) {
+        if (kKeep) t[kKeep ? i : 0][kKeep ? e : 0] = h * g_of(i, e);
+        top = max_nan(top, fabsf(t_of(i, e)));
+      }
     }
   uint32_t peak = __float_as_uint(top) & 0x7fffffffu;  // a NaN is above every number
-  reduce_row<WARP>(ss, peak, part, warps);
+  reduce_row<WARP, CODES>(ss, peak, part, warps);
   float rstd = rstd_of(ss, p.cols, p.eps);
   if (!(ss < INFINITY)) {  // the same in all of the row's threads
     ss = 0.0f;
@@ -301,11 +329,11 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsno
       }
     uint32_t none = 0u;
     if (!WARP) __syncthreads();  // part is written again
-    reduce_row<WARP>(ss, none, part, warps);
+    reduce_row<WARP, false>(ss, none, part, warps);
     rstd = rstd_scaled(ss, p.cols);
   }
 
-  if (p.y != nullptr) {
+  if (!CODES || p.y != nullptr) {
     T* y = static_cast<T*>(p.y) + row * p.y_ld;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -316,29 +344,25 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsno
         *reinterpret_cast<V*>(y + at(i)) = o;
       }
   }
-  if (p.q != nullptr) {
+  if constexpr (CODES) {
     double exact = static_cast<double>(__uint_as_float(peak));
     if constexpr (std::is_same<T, float>::value) {
       uint32_t rest = 0u;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) rest = max(rest, rest_of(h_of(i, e) * g_of(i, e), h_of(i, e), g_of(i, e), peak));
+        for (int e = 0; e < VEC; ++e) rest = max(rest, rest_of(t_of(i, e), h_of(i, e), g_of(i, e), peak));
       exact = exact_peak_of<WARP>(peak, rest, &shared_rest);
     }
     const RowCode c = row_code(peak, exact, p.q_dtype);
     if (me == 0) p.scales[row] = row_scale(peak, rstd, c);
     uint8_t* q = p.q + row * p.q_ld;
-    const bool live = c.ratio != 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (at(i) < p.cols) {
         Vec<uint8_t, VEC> o;
-        float t[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = live ? h_of(i, e) * g_of(i, e) : 0.0f;
-        if (p.q_dtype == OSC_S8) codes_s8<VEC>(t, [&](int e) { return h_of(i, e); }, [&](int e) { return g_of(i, e); }, c, o.v);
-        else codes_e4m3<VEC>(t, [&](int e) { return h_of(i, e); }, [&](int e) { return g_of(i, e); }, c, o.v);
+        codes_of<VEC>([&](int e) { return t_of(i, e); }, [&](int e) { return h_of(i, e); },
+                      [&](int e) { return g_of(i, e); }, c, p.q_dtype, o.v);
         *reinterpret_cast<Vec<uint8_t, VEC>*>(q + at(i)) = o;
       }
   }
@@ -378,7 +402,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
     if (p.q != nullptr) top = max_nan(top, fabsf(h * g_at(e)));
   }
   uint32_t peak = __float_as_uint(top) & 0x7fffffffu;
-  reduce_row<false>(ss, peak, part, warps);
+  reduce_row<false, true>(ss, peak, part, warps);
   float rstd = rstd_of(ss, p.cols, p.eps);
   if (!(ss < INFINITY)) {
     ss = 0.0f;
@@ -388,7 +412,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
     }
     uint32_t none = 0u;
     __syncthreads();
-    reduce_row<false>(ss, none, part, warps);
+    reduce_row<false, true>(ss, none, part, warps);
     rstd = rstd_scaled(ss, p.cols);
   }
   RowCode c = {};
@@ -410,10 +434,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
   for (int e = threadIdx.x; e < p.cols; e += kMaxThreads) {
     const float h = h_at(e), g = g_at(e);
     if (q != nullptr) {
-      const float t[1] = {c.ratio != 0.0f ? h * g : 0.0f};
       uint8_t o[1];
-      if (p.q_dtype == OSC_S8) codes_s8<1>(t, [&](int) { return h; }, [&](int) { return g; }, c, o);
-      else codes_e4m3<1>(t, [&](int) { return h; }, [&](int) { return g; }, c, o);
+      codes_of<1>([&](int) { return h * g; }, [&](int) { return h; }, [&](int) { return g; }, c, p.q_dtype, o);
       q[e] = o[0];
     }
     if (y != nullptr) y[e] = from_f<T>(h * rstd * g);
@@ -421,33 +443,32 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
 }
 
 // ------------------------------------------------------------------ host side
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool CODES>
 int launch_rows(osc_ctx* ctx, const NormArgs& p, int threads) {
   if (threads == 32) {
     const long long blocks = (p.rows + kRowsPerCta - 1) / kRowsPerCta;
-    return launch_pdl(ctx, k_rmsnorm<T, VEC, NV, true>, dim3(static_cast<unsigned>(blocks)), dim3(32 * kRowsPerCta), 0,
-                      "k_rmsnorm", p);
+    return launch_pdl(ctx, k_rmsnorm<T, VEC, NV, true, CODES>, dim3(static_cast<unsigned>(blocks)),
+                      dim3(32 * kRowsPerCta), 0, "k_rmsnorm", p);
   }
-  return launch_pdl(ctx, k_rmsnorm<T, VEC, NV, false>, dim3(static_cast<unsigned>(p.rows)),
+  return launch_pdl(ctx, k_rmsnorm<T, VEC, NV, false, CODES>, dim3(static_cast<unsigned>(p.rows)),
                     dim3(static_cast<unsigned>(threads)), 0, "k_rmsnorm", p);
 }
 
-template <typename T>
+template <typename T, bool CODES>
 int launch_norm(osc_ctx* ctx, const NormArgs& p, bool vectors) {
-  if (p.cols > kMaxRegCols)
+  constexpr int VEC = 16 / static_cast<int>(sizeof(T)), NV = 16 / VEC;  // 16 elements a thread
+  auto threads_for = [&](int per) { return (p.cols + 32 * per - 1) / (32 * per) * 32; };
+  if (p.cols > kMaxThreads * (vectors ? VEC * NV : kSingles))
     return launch_pdl(ctx, k_rmsnorm_long<T>, dim3(static_cast<unsigned>(p.rows)), dim3(kMaxThreads), 0,
                       "k_rmsnorm_long", p);
-  constexpr int VEC = 16 / static_cast<int>(sizeof(T));
-  auto threads_for = [&](int per) { return (p.cols + 32 * per - 1) / (32 * per) * 32; };
-  // Rows spread over as many threads as fit at once; more rows than that take
-  // fewer threads a row, each with more of it.
-  const bool few = p.rows * threads_for(vectors ? VEC : 4) <= 1024ll * ctx->num_sms;
   if (vectors) {
-    if (few && threads_for(VEC) <= kMaxThreads) return launch_rows<T, VEC, 1>(ctx, p, threads_for(VEC));
-    return launch_rows<T, VEC, kRegFloats / VEC>(ctx, p, threads_for(kRegFloats));
+    // few rows are spread over as many threads as fit at once
+    if (p.rows * threads_for(VEC) <= 1024ll * ctx->num_sms && threads_for(VEC) <= kMaxThreads)
+      return launch_rows<T, VEC, 1, CODES>(ctx, p, threads_for(VEC));
+    return launch_rows<T, VEC, NV, CODES>(ctx, p, threads_for(VEC * NV));
   }
-  if (few && threads_for(4) <= kMaxThreads) return launch_rows<T, 1, 4>(ctx, p, threads_for(4));
-  return launch_rows<T, 1, kRegFloats>(ctx, p, threads_for(kRegFloats));
+  if (threads_for(4) <= kMaxThreads) return launch_rows<T, 1, 4, CODES>(ctx, p, threads_for(4));
+  return launch_rows<T, 1, kSingles, CODES>(ctx, p, threads_for(kSingles));
 }
 
 int type_bytes(int dtype) { return dtype == OSC_F32 ? 4 : 2; }
@@ -514,10 +535,11 @@ OSC_API int osc_rmsnorm(osc_ctx* ctx, int dtype, const void* x, long long x_ld, 
   const bool vectors = cols % vec == 0 && rows_fit(x, x_ld, 16) && rows_fit(residual, res_ld, 16) &&
                        rows_fit(sum, sum_ld, 16) && rows_fit(y, y_ld, 16) && rows_fit(gamma, 0, 16) &&
                        rows_fit(q, q_ld, static_cast<size_t>(vec));
+  const bool codes = q != nullptr;
   switch (dtype) {
-    case OSC_F32: return launch_norm<float>(ctx, p, vectors);
-    case OSC_F16: return launch_norm<__half>(ctx, p, vectors);
-    default: return launch_norm<__nv_bfloat16>(ctx, p, vectors);
+    case OSC_F32: return codes ? launch_norm<float, true>(ctx, p, vectors) : launch_norm<float, false>(ctx, p, vectors);
+    case OSC_F16: return codes ? launch_norm<__half, true>(ctx, p, vectors) : launch_norm<__half, false>(ctx, p, vectors);
+    default: return codes ? launch_norm<__nv_bfloat16, true>(ctx, p, vectors) : launch_norm<__nv_bfloat16, false>(ctx, p, vectors);
   }
 }
 
