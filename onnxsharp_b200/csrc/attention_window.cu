@@ -13,8 +13,9 @@
 // row r of a tile is token r / G, query head r % G of the group (G query heads
 // share a key/value head), so a key is read once for the group. A masked score
 // is -inf by selection, whatever was computed for it; keys at and behind a
-// sequence's length are never used (V rows there are zeroed where a tile
-// brings them along: 0 * NaN would not vanish).
+// sequence's length or between the sinks and every row's window are never used
+// (V rows there are zeroed where a tile brings them along: 0 * NaN would not
+// vanish).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -40,17 +41,21 @@ struct WinArgs {
   float scale2;       // scale * log2(e): softmax in powers of two
   int tokens;         // tokens of a 128-row tile (k_window_tiles)
   int token_tiles, items;
-  int split;          // CTAs that share a row tile's keys (k_window_rows)
-  int row_tiles;
+  int row_tiles;      // of 16 rows (k_window_rows)
+  int teams;          // of HK CTAs, that share all key tiles
+  void* parts;        // what they leave of cut groups
 };
 
 constexpr int kFarPos = 1 << 30;
 
 // Position of query 0 and the sequence's length, made safe whatever the device
 // holds: a start at or behind the length is padding, and so is one below -T.
-__device__ __forceinline__ void place_of(const WinArgs& p, int b, int& first, int& len) {
-  len = max(0, min(p.lengths[b], p.S));
-  first = p.starts != nullptr ? max(-kFarPos, min(p.starts[b], len)) : len - p.T;
+__device__ __forceinline__ int2 read_place(const WinArgs& p, int b) {
+  return make_int2(p.lengths[b], p.starts != nullptr ? p.starts[b] : 0);
+}
+__device__ __forceinline__ void place_of(const WinArgs& p, int2 read, int& first, int& len) {
+  len = max(0, min(read.x, p.S));
+  first = p.starts != nullptr ? max(-kFarPos, min(read.y, len)) : len - p.T;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -132,6 +137,7 @@ struct Item {
   int b, hk, t0;       // sequence, key/value head, first token
   int first, len;      // position of query 0, the sequence's length
   int lo, hi;          // live positions of its rows (none: lo > hi)
+  int wlo;             // first key of the window of the lowest
   int sink_tiles, lo_tile, n;  // key tiles: sinks', then from lo_tile on; how many
   int plain_lo, plain_hi;      // every row sees every key of the tiles that start in [plain_lo, plain_hi]
   __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : lo_tile + i - sink_tiles) * kKeys; }
@@ -143,12 +149,13 @@ __device__ __forceinline__ Item item_at(const WinArgs& p, int x) {
   w.t0 = (p.token_tiles - 1 - tile) * p.tokens;  // late tokens see the most keys of a prompt: they come first
   w.b = rest / p.HK;
   w.hk = rest - w.b * p.HK;
-  place_of(p, w.b, w.first, w.len);
+  place_of(p, read_place(p, w.b), w.first, w.len);
   w.lo = max(w.first + w.t0, 0);
   w.hi = min(w.first + min(w.t0 + p.tokens, p.T), w.len) - 1;
   w.sink_tiles = w.lo_tile = w.n = 0;
+  w.wlo = w.lo >= p.window ? w.lo - p.window + 1 : 0;
   if (w.lo <= w.hi) {
-    w.lo_tile = (w.lo >= p.window ? w.lo - p.window + 1 : 0) / kKeys;
+    w.lo_tile = w.wlo / kKeys;
     w.sink_tiles = min((min(p.sinks, w.hi + 1) + kKeys - 1) / kKeys, w.lo_tile);
     w.n = w.sink_tiles + w.hi / kKeys - w.lo_tile + 1;
   }
@@ -348,11 +355,22 @@ __global__ void __launch_bounds__(kWinThreads, 1)
     for (at.start(p); at.more; at.next(p)) {
       const int s = at.step & 1, j0 = at.w.key0(at.i);
       if (!wait(&bar->v_full[s], at.step >> 1)) break;
-      if (j0 + kKeys > at.w.len) {
-        // V rows behind the length: whatever the cache holds there must not meet P's zeros
-        for (int x = (at.w.len - j0) * 8 + lane; x < kKeys * 8; x += 32)
-          for (int c = 0; c < Cfg::CH; ++c)
-            *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+      // V rows behind the length and between the sinks and the window: whatever
+      // the cache holds there must not meet P's zeros. (Halves that consist of
+      // such rows are skipped below: what counts is the rest of the border's half.)
+      const int gone0 = max(p.sinks - j0, 0), gone1 = min(at.w.wlo - j0, kKeys), end = at.w.len - j0;
+      if (gone0 < gone1 || end < kKeys) {
+        auto clear = [&](int from, int to) {
+          for (int x = from * 8 + lane; x < to * 8; x += 32)
+            for (int c = 0; c < Cfg::CH; ++c)
+              *reinterpret_cast<uint4*>(sv + s * Cfg::TILE + c * kKeys * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto half_up = [](int row) { return (row + 63) & ~63; };
+        if (gone0 < gone1) {
+          clear(gone0, min(gone1, half_up(gone0)));
+          clear(max(half_up(gone0), gone1 & ~63), gone1);
+        }
+        if (end < kKeys) clear(end, half_up(end));
         fence_async_smem();
         __syncwarp();
       }
@@ -567,14 +585,22 @@ __global__ void __launch_bounds__(kWinThreads, 1)
 
 // ------------------------------------------------------------------ few rows
 // A decode step: 16 rows (tokens x grouped heads) against a long cache, bound
-// by the cache's bytes. The seen keys of the row tile are numbered through
-// (sinks, then the window), cut into runs for the CTAs of a cluster and walked
-// in tiles of 64 by cp.async; each of four warps takes 16 keys of a tile with
-// its own running maximum, sum and O (mma.sync m16n8k16: at 16 rows the tensor
-// rate is not the limit, and the 128-row tcgen05 tile would be seven eighths
-// empty). Warps, then CTAs, are joined in a fixed order, through shared memory
-// and the cluster's shared memory: no workspace, the same bits every run.
-constexpr int kRowKeys = 64, kRowStages = 3, kRowThreads = 128;
+// by the cache's bytes. A producer warp brings the tiles of 64 keys that some row
+// sees (sinks', then the window's) by TMA; each of four warps takes 16 keys of a
+// tile with its own running maximum, sum and O (mma.sync m16n8k16: at 16 rows
+// the tensor rate is not the limit, and the 128-row tcgen05 tile would be seven
+// eighths empty). A row tile's work for one key/value head is a "group".
+//
+// Lengths are known on the device alone and differ, so the tiles of all row
+// tiles are laid end to end and every team of CTAs, one per key/value head,
+// takes the same number of them, whatever sequence they belong to. (Heads that
+// walk the same keys side by side read whole rows of the cache between them.)
+// A group that lies in one CTA is finished there; of one that is cut the parts
+// go to a workspace of the call and k_window_join adds them up in the order of
+// the keys: where the cuts lie depends on lengths and the number of SMs alone,
+// so the bits are the same every run.
+constexpr int kRowKeys = 64, kRowStages = 3;
+constexpr int kRowThreads = 160;  // four warps of keys, the producer
 
 template <bool BF16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -601,307 +627,591 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                : "r"(addr)
                : "memory");
 }
-// 16 bytes; valid == false writes zeros without reading src.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ float ld_cluster_f(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
+// The four warps of keys.
+__device__ __forceinline__ void keys_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+struct RowBars {
+  uint64_t full[kRowStages], empty[kRowStages];
+  int part[kRowThreads / 32];
+  int found[2];
+  int abort_flag;
+};
 
 template <int D>
 struct RowCfg {
-  static constexpr int TILE = kRowKeys * D * 2;
-  static constexpr int SMEM = kRowStages * 2 * TILE;
-  // after the last tile the ring holds the warps' O [4][16][D], the CTA's O [16][D], maxima and sums
-  static constexpr int OFF_CTA = 4 * 16 * D * 4, OFF_M = OFF_CTA + 16 * D * 4, OFF_L = OFF_M + 4 * 16 * 4,
-                       OFF_CM = OFF_L + 4 * 16 * 4, OFF_CL = OFF_CM + 64;
-  static_assert(OFF_CL + 64 <= SMEM, "the join fits the ring");
+  static constexpr int CH = D / 64, CHUNK = kRowKeys * 128;  // 128-byte columns of a row
+  static constexpr int TILE = CH * CHUNK;
+  // behind the ring: O of two warps as fragments, their maxima and sums
+  static constexpr int JOIN = kRowStages * 2 * TILE, JOIN_ML = JOIN + 2 * 16 * D * 4;
+  static constexpr int BARS = JOIN_ML + 2 * 16 * 8;
+  static constexpr int SMEM = BARS + static_cast<int>(sizeof(RowBars));
+};
+
+// A row tile of a sequence ("unit": the groups of its key/value heads are alike).
+struct Unit {
+  int b, row0, first, len;
+  int lo, hi;                  // keys that some row sees: [lo, hi] and the sinks
+  int sink_tiles, lo_tile, tiles;  // key tiles: sinks', then from lo_tile on; how many
+  __device__ __forceinline__ int key0(int i) const {
+    return (i < sink_tiles ? i : lo_tile + i - sink_tiles) * kRowKeys;
+  }
+};
+__device__ __forceinline__ Unit unit_of(const WinArgs& p, int x, int2 read) {
+  Unit u;
+  u.b = x / p.row_tiles;
+  u.row0 = (x - u.b * p.row_tiles) * 16;
+  place_of(p, read, u.first, u.len);
+  const int t_lo = u.row0 / p.G, t_hi = min(u.row0 + 15, p.T * p.G - 1) / p.G;
+  const int lo_pos = max(u.first + t_lo, 0);
+  u.hi = min(u.first + t_hi, u.len - 1);
+  u.lo = lo_pos >= p.window ? lo_pos - p.window + 1 : 0;
+  u.lo_tile = u.sink_tiles = u.tiles = 0;
+  if (lo_pos <= u.hi) {
+    u.lo_tile = u.lo / kRowKeys;
+    u.sink_tiles = min((min(p.sinks, u.hi + 1) + kRowKeys - 1) / kRowKeys, u.lo_tile);
+    u.tiles = u.sink_tiles + u.hi / kRowKeys - u.lo_tile + 1;
+  }
+  return u;
+}
+__device__ __forceinline__ Unit unit_at(const WinArgs& p, int x) { return unit_of(p, x, read_place(p, x / p.row_tiles)); }
+
+// Tiles of all units before this thread's share of them, of the share, and of all.
+struct Tally {
+  int before, own, all;
+  int x0, x1;  // the share
+};
+template <int THREADS>
+__device__ __forceinline__ Tally tally(const WinArgs& p, int* part) {
+  const int units = p.B * p.row_tiles, each = (units + THREADS - 1) / THREADS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Tally t;
+  t.x0 = min(static_cast<int>(threadIdx.x) * each, units);
+  t.x1 = min(t.x0 + each, units);
+  t.own = 0;
+  for (int x = t.x0; x < t.x1; ++x) t.own += unit_at(p, x).tiles;
+  int upto = t.own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) part[warp] = upto;
+  __syncthreads();
+  t.all = 0;
+  t.before = upto - t.own;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) t.before += part[w];
+    t.all += part[w];
+  }
+  return t;
+}
+// Tiles a team takes; fewer than kMinTiles are not worth a part of their own.
+constexpr int kMinTiles = 2;
+__device__ __forceinline__ int tiles_each(const WinArgs& p, int all) {
+  return max(kMinTiles, (all + p.teams - 1) / p.teams);
+}
+
+// Where a CTA's walk stands. The next unit's place is read a unit ahead and not
+// touched until then: behind the copies in flight such a load takes microseconds.
+struct Walk {
+  Unit u;
+  int2 after;  // of unit x + 1, as read
+  int x, tile;
+  __device__ __forceinline__ void at(const WinArgs& p, int units, int unit, int first_tile) {
+    x = unit;
+    tile = first_tile;
+    u = unit_at(p, x);
+    after = read_place(p, min(x + 1, units - 1) / p.row_tiles);
+  }
+  __device__ __forceinline__ void next(const WinArgs& p, int units) {
+    if (++tile < u.tiles) return;
+    tile = 0;
+    do {
+      if (++x >= units) {  // past the last tile
+        u.tiles = 0;
+        return;
+      }
+      u = unit_of(p, x, after);
+      after = read_place(p, min(x + 1, units - 1) / p.row_tiles);
+    } while (u.tiles == 0);
+  }
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kRowThreads, 2) k_window_rows(const __grid_constant__ WinArgs p) {
+__device__ __forceinline__ uint16_t* out_row(const WinArgs& p, const Unit& u, int hk, int r) {
+  return static_cast<uint16_t*>(p.out) + u.b * p.o_b + static_cast<long long>((u.row0 + r) / p.G) * p.o_t +
+         (hk * p.G + (u.row0 + r) % p.G) * p.o_h;
+}
+
+// Parts of cut groups: CTA c leaves the group that it entered in the middle in
+// slot 2 c, the one that it began and left unfinished in slot 2 c + 1. The team
+// that begins a row tile says which teams have it: from span.x to span.y.
+template <int D>
+struct Parts {
+  float* o;     // [slots][16][D]
+  float2* ml;   // [slots][16]
+  int2* span;   // [units]
+  __device__ __forceinline__ Parts(const WinArgs& p)
+      : o(static_cast<float*>(p.parts)),
+        ml(reinterpret_cast<float2*>(o + 2ll * p.teams * p.HK * 16 * D)),
+        span(reinterpret_cast<int2*>(ml + 2ll * p.teams * p.HK * 16)) {}
+  static size_t bytes(int ctas, int units) { return 2ull * ctas * 16 * (D * 4 + 8) + 8ull * units; }
+};
+
+// CUT: the tiles of all units, evenly over p.teams teams; else a CTA a group.
+template <int D, bool BF16, bool CUT>
+__global__ void __launch_bounds__(kRowThreads, 2)
+    k_window_rows(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
+                  const __grid_constant__ WinArgs p, int* __restrict__ err) {
   using Cfg = RowCfg<D>;
   extern __shared__ __align__(1024) uint8_t ring[];
+  RowBars* bar = reinterpret_cast<RowBars*>(ring + Cfg::BARS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = static_cast<int>(blockIdx.x) % p.split, rt = static_cast<int>(blockIdx.x) / p.split;
-  const int hk = blockIdx.y, b = blockIdx.z;
+  const int units = p.B * p.row_tiles, nrows = p.T * p.G;
+  const int team = static_cast<int>(blockIdx.x / p.HK), hk = static_cast<int>(blockIdx.x - team * p.HK);
+  if (tid == 0) {
+    for (int i = 0; i < kRowStages; ++i) {
+      mbar_init(&bar->full[i], 1);
+      mbar_init(&bar->empty[i], 4);
+    }
+    bar->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch(&mK);
+    tma_prefetch(&mV);
+  }
+  __syncthreads();
   griddep_launch();
   griddep_wait();
-  int first, len;
-  place_of(p, b, first, len);
-  const int row0 = rt * 16, nrows = p.T * p.G;
-  const int t_lo = row0 / p.G, t_hi = min(row0 + 15, nrows - 1) / p.G;
-  const int lo_pos = max(first + t_lo, 0), hi_pos = min(first + t_hi, len - 1);
-  auto out_row = [&](int r) {
-    return static_cast<uint16_t*>(p.out) + b * p.o_b + static_cast<long long>((row0 + r) / p.G) * p.o_t +
-           (hk * p.G + (row0 + r) % p.G) * p.o_h;
+  auto clear = [&](const Unit& u) {  // a group that is padding alone
+    for (int y = tid; y < 16 * D / 8; y += kRowThreads) {
+      const int r = y / (D / 8);
+      if (u.row0 + r < nrows)
+        *reinterpret_cast<uint4*>(out_row<D, BF16>(p, u, hk, r) + (y % (D / 8)) * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
   };
-  if (lo_pos > hi_pos) {  // padding alone: the same in the whole cluster
-    if (rank == 0)
-      for (int x = tid; x < 16 * D / 8; x += kRowThreads) {
-        const int r = x / (D / 8);
-        if (row0 + r < nrows) *reinterpret_cast<uint4*>(out_row(r) + (x % (D / 8)) * 8) = make_uint4(0u, 0u, 0u, 0u);
+  Walk at;
+  int left, each = 0;
+  if constexpr (CUT) {
+    const Tally t = tally<kRowThreads>(p, bar->part);
+    each = tiles_each(p, t.all);
+    left = min(each, t.all - team * each);
+    const int rel = team * each - t.before;
+    if (left > 0 && rel >= 0 && rel < t.own) {
+      int rest = rel, x = t.x0;
+      for (int n = unit_at(p, x).tiles; rest >= n; n = unit_at(p, x).tiles) {
+        rest -= n;
+        ++x;
       }
-    return;
-  }
-  const int lo = lo_pos >= p.window ? lo_pos - p.window + 1 : 0;
-  const int nsink = min(p.sinks, lo);
-  const int total = nsink + hi_pos - lo + 1;
-  const int tiles = (total + kRowKeys - 1) / kRowKeys;
-  const int i0 = static_cast<int>(static_cast<long long>(rank) * tiles / p.split);
-  const int i1 = static_cast<int>(static_cast<long long>(rank + 1) * tiles / p.split);
-
-  // a thread copies the same 16 bytes of every (128 / CHUNKS)-th row of a tile
-  constexpr int CHUNKS = D / 8, ROWS_STEP = kRowThreads / CHUNKS;
-  const int ch = tid % CHUNKS, crow = tid / CHUNKS;
-  const uint16_t* kbase = static_cast<const uint16_t*>(p.k) + b * p.k_b + hk * p.k_h + ch * 8;
-  const uint16_t* vbase = static_cast<const uint16_t*>(p.v) + b * p.v_b + hk * p.v_h + ch * 8;
-  const uint32_t ring_at = smem_addr(ring);
-  auto fetch = [&](int i) {
-    const uint32_t at = ring_at + static_cast<uint32_t>(((i - i0) % kRowStages) * 2 * Cfg::TILE);
-#pragma unroll
-    for (int x = 0; x < kRowKeys / ROWS_STEP; ++x) {
-      const int row = crow + x * ROWS_STEP;
-      const int vi = i * kRowKeys + row;
-      const bool valid = vi < total;
-      const long long j = !valid ? 0 : vi < nsink ? vi : lo + vi - nsink;
-      const uint32_t off = static_cast<uint32_t>(row * D * 2 + ((ch ^ (row & 7)) << 4));
-      cp_async16(at + off, kbase + j * p.k_s, valid);
-      cp_async16(at + Cfg::TILE + off, vbase + j * p.v_s, valid);
+      bar->found[0] = x;
+      bar->found[1] = rest;
     }
-  };
-
-  // Q: the A fragments of 16 rows, straight from global memory
-  const int ra = lane >> 2, rb = ra + 8;
-  uint32_t qf[D / 16][4];
-  {
-    const bool in_a = row0 + ra < nrows, in_b = row0 + rb < nrows;
-    auto q_row = [&](int r) {
-      return static_cast<const uint16_t*>(p.q) + b * p.q_b + static_cast<long long>((row0 + r) / p.G) * p.q_t +
-             (hk * p.G + (row0 + r) % p.G) * p.q_h + (lane & 3) * 2;
-    };
-    const uint16_t* qa = q_row(in_a ? ra : 0);
-    const uint16_t* qb = q_row(in_b ? rb : 0);
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      qf[ks][0] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16) : 0u;
-      qf[ks][1] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16) : 0u;
-      qf[ks][2] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16 + 8) : 0u;
-      qf[ks][3] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16 + 8) : 0u;
-    }
-  }
-  // positions of this thread's two rows; -1 sees nothing
-  auto pos_of = [&](int r) {
-    const int pos = first + (row0 + r) / p.G;
-    return row0 + r < nrows && pos >= 0 && pos < len ? pos : -1;
-  };
-  const int pos_a = pos_of(ra), pos_b = pos_of(rb);
-
-  float o[D / 8][4];
-#pragma unroll
-  for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[x][e] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
-#pragma unroll
-  for (int s = 0; s < kRowStages - 1; ++s) {
-    if (i0 + s < i1) fetch(i0 + s);
-    cp_async_commit();
-  }
-  for (int i = i0; i < i1; ++i) {
-    cp_async_wait<kRowStages - 2>();
     __syncthreads();
-    if (i + kRowStages - 1 < i1) fetch(i + kRowStages - 1);
-    cp_async_commit();
-    const uint32_t at = ring_at + static_cast<uint32_t>(((i - i0) % kRowStages) * 2 * Cfg::TILE);
-    float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    if (left > 0) at.at(p, units, bar->found[0], bar->found[1]);
+  } else {
+    at.at(p, units, team, 0);
+    left = at.u.tiles;
+    if (left == 0) {
+      clear(at.u);
+      return;
+    }
+  }
+
+  const uint32_t ring_at = smem_addr(ring);
+  bool ok = true;  // after a wait that ran out the meetings go on, over whatever the ring holds, and nothing is stored
+  auto wait = [&](uint64_t* m, uint32_t parity) {
+    const bool fine = mbar_wait(m, parity & 1u, &bar->abort_flag, err);
+    return __all_sync(0xffffffffu, fine) != 0;
+  };
+  int slot = 0;
+  uint32_t turn = 0;  // of the ring
+  auto advance = [&]() {
+    if (++slot == kRowStages) {
+      slot = 0;
+      ++turn;
+    }
+  };
+  if (warp == 4) {
+    for (; left > 0; --left, at.next(p, units), advance()) {
+      if (!wait(&bar->empty[slot], turn ^ 1u)) break;
+      if (elect_one()) {
+        uint8_t* dst = ring + slot * 2 * Cfg::TILE;
+        const int key = at.u.key0(at.tile);
+        mbar_arrive_expect_tx(&bar->full[slot], 2 * Cfg::TILE);
+        for (int c = 0; c < Cfg::CH; ++c) {
+          tma_load_4d(dst + c * Cfg::CHUNK, &mK, &bar->full[slot], c * 64, key, hk, at.u.b);
+          tma_load_4d(dst + Cfg::TILE + c * Cfg::CHUNK, &mV, &bar->full[slot], c * 64, key, hk, at.u.b);
+        }
+      }
+    }
+    left = 0;
+  }
+
+  const int ra = lane >> 2, rb = ra + 8;
+  while (left > 0) {
+    const Unit u = at.u;
+    const int x = at.x, i0 = at.tile, i1 = i0 + min(left, u.tiles - i0);
+    // Q: the A fragments of 16 rows, straight from global memory
+    uint32_t qf[D / 16][4];
     {
-      const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
-      const uint32_t krow = at + static_cast<uint32_t>(key * D * 2);
+      const bool in_a = u.row0 + ra < nrows, in_b = u.row0 + rb < nrows;
+      auto q_row = [&](int r) {
+        return static_cast<const uint16_t*>(p.q) + u.b * p.q_b + static_cast<long long>((u.row0 + r) / p.G) * p.q_t +
+               (hk * p.G + (u.row0 + r) % p.G) * p.q_h + (lane & 3) * 2;
+      };
+      const uint16_t* qa = q_row(in_a ? ra : 0);
+      const uint16_t* qb = q_row(in_b ? rb : 0);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t kf[4];
-        ldmatrix4(kf, krow + static_cast<uint32_t>((((ks * 2 + ((lane >> 3) & 1)) ^ (key & 7)) << 4)));
-        mma_16816<BF16>(s[0], qf[ks], kf[0], kf[1]);
-        mma_16816<BF16>(s[1], qf[ks], kf[2], kf[3]);
+        qf[ks][0] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16) : 0u;
+        qf[ks][1] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16) : 0u;
+        qf[ks][2] = in_a ? *reinterpret_cast<const uint32_t*>(qa + ks * 16 + 8) : 0u;
+        qf[ks][3] = in_b ? *reinterpret_cast<const uint32_t*>(qb + ks * 16 + 8) : 0u;
       }
     }
-    // c0, c1 belong to row a, c2, c3 to row b
+    // positions of this thread's two rows; -1 sees nothing
+    auto pos_of = [&](int r) {
+      const int pos = u.first + (u.row0 + r) / p.G;
+      return u.row0 + r < nrows && pos >= 0 && pos < u.len ? pos : -1;
+    };
+    const int pos_a = pos_of(ra), pos_b = pos_of(rb);
+
+    float o[D / 8][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int x = 0; x < D / 8; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int vi = i * kRowKeys + warp * 16 + n * 8 + (lane & 3) * 2 + (e & 1);
-        const int j = vi < nsink ? vi : lo + vi - nsink;
-        const int pos = e < 2 ? pos_a : pos_b;
-        const bool seen = vi < total && j <= pos && (pos - j < p.window || j < p.sinks);
-        s[n][e] = seen ? s[n][e] * p.scale2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) o[x][e] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    // every row of the tile sees every key of the key tiles that start in [plain_lo, plain_hi]
+    const int t_lo = u.row0 / p.G;
+    const bool all_live = u.first + t_lo >= 0 && u.first + min(u.row0 + 15, nrows - 1) / p.G < u.len;
+    const int plain_lo = u.hi >= p.window ? u.hi - p.window + 1 : 0;
+    const int plain_hi = all_live ? u.first + t_lo - kRowKeys + 1 : -1;
+
+    for (int i = i0; i < i1; ++i) {
+      const int j0 = u.key0(i), key0 = j0 + warp * 16;
+      const bool plain = j0 >= plain_lo && j0 <= plain_hi;
+      const uint32_t tile = ring_at + static_cast<uint32_t>(slot * 2 * Cfg::TILE);
+      if (ok) ok = wait(&bar->full[slot], turn);
+      // V rows that no row sees: whatever the cache holds there must not meet P's zeros
+      if (!plain && (key0 + 15 > u.hi || (key0 < u.lo && key0 + 15 >= p.sinks))) {
+        const int y = lane >> 1, j = key0 + y;
+        if (j > u.hi || (j < u.lo && j >= p.sinks)) {
+          uint8_t* v = ring + slot * 2 * Cfg::TILE + Cfg::TILE + (warp * 16 + y) * 128 + (lane & 1) * 64;
+#pragma unroll
+          for (int c = 0; c < Cfg::CH; ++c)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) *reinterpret_cast<uint4*>(v + c * Cfg::CHUNK + z * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_async_smem();
+        __syncwarp();
       }
-    float alpha[2];
+      // (two sums each, of every other 16 of D: half as long a chain of products)
+      float s[2][4] = {}, s2[2][4] = {};
+      {
+        const int key = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+        const uint32_t krow = tile + static_cast<uint32_t>(key * 128);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float next = fmaxf(m[h], top);
-      const float base = next == -INFINITY ? 0.0f : next;
-      alpha[h] = exp2_fast(m[h] - base);
-      m[h] = next;
-      float sum = 0.0f;
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t kf[4];
+          const int c = (ks & 3) * 2 + ((lane >> 3) & 1);
+          ldmatrix4(kf, krow + static_cast<uint32_t>((ks >> 2) * Cfg::CHUNK + ((c ^ (key & 7)) << 4)));
+          mma_16816<BF16>(ks % 2 == 0 ? s[0] : s2[0], qf[ks], kf[0], kf[1]);
+          mma_16816<BF16>(ks % 2 == 0 ? s[1] : s2[1], qf[ks], kf[2], kf[3]);
+        }
+      }
+      // c0, c1 belong to row a, c2, c3 to row b
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[n][2 * h + e] = exp2_fast(s[n][2 * h + e] - base);
-          sum += s[n][2 * h + e];
+        for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * p.scale2;
+      if (!plain) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = key0 + n * 8 + (lane & 3) * 2 + (e & 1);
+            const int pos = e < 2 ? pos_a : pos_b;
+            if (!(j <= pos && (pos - j < p.window || j < p.sinks))) s[n][e] = -INFINITY;
+          }
+      }
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float next = fmaxf(m[h], top);
+        const float base = next == -INFINITY ? 0.0f : next;
+        alpha[h] = exp2_fast(m[h] - base);
+        m[h] = next;
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[n][2 * h + e] = exp2_fast(s[n][2 * h + e] - base);
+            sum += s[n][2 * h + e];
+          }
+        l[h] = l[h] * alpha[h] + sum;
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          o[x][0] *= alpha[0];
+          o[x][1] *= alpha[0];
+          o[x][2] *= alpha[1];
+          o[x][3] *= alpha[1];
         }
-      l[h] = l[h] * alpha[h] + sum;
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
-#pragma unroll
-      for (int x = 0; x < D / 8; ++x) {
-        o[x][0] *= alpha[0];
-        o[x][1] *= alpha[0];
-        o[x][2] *= alpha[1];
-        o[x][3] *= alpha[1];
       }
-    }
-    const uint32_t pf[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]), pack2<BF16>(s[1][0], s[1][1]),
-                            pack2<BF16>(s[1][2], s[1][3])};
-    {
-      const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
-      const uint32_t vrow = at + Cfg::TILE + static_cast<uint32_t>(key * D * 2);
+      const uint32_t pf[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]),
+                              pack2<BF16>(s[1][0], s[1][1]), pack2<BF16>(s[1][2], s[1][3])};
+      {
+        const int key = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+        const uint32_t vrow = tile + Cfg::TILE + static_cast<uint32_t>(key * 128);
 #pragma unroll
-      for (int dn = 0; dn < D / 16; ++dn) {
-        uint32_t vf[4];
-        ldmatrix4_trans(vf, vrow + static_cast<uint32_t>((((dn * 2 + (lane >> 4)) ^ (key & 7)) << 4)));
-        mma_16816<BF16>(o[2 * dn], pf, vf[0], vf[1]);
-        mma_16816<BF16>(o[2 * dn + 1], pf, vf[2], vf[3]);
+        for (int dn = 0; dn < D / 16; ++dn) {
+          uint32_t vf[4];
+          const int c = (dn & 3) * 2 + (lane >> 4);
+          ldmatrix4_trans(vf, vrow + static_cast<uint32_t>((dn >> 2) * Cfg::CHUNK + ((c ^ (key & 7)) << 4)));
+          mma_16816<BF16>(o[2 * dn], pf, vf[0], vf[1]);
+          mma_16816<BF16>(o[2 * dn + 1], pf, vf[2], vf[3]);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->empty[slot]);
+      advance();
     }
-  }
-  cp_async_wait<0>();
-  __syncthreads();
 
-  // join the warps: each leaves its O, maximum and sum in the ring
-  float* wo = reinterpret_cast<float*>(ring);
-  float* co = reinterpret_cast<float*>(ring + Cfg::OFF_CTA);
-  float* wm = reinterpret_cast<float*>(ring + Cfg::OFF_M);
-  float* wl = reinterpret_cast<float*>(ring + Cfg::OFF_L);
-  float* cm = reinterpret_cast<float*>(ring + Cfg::OFF_CM);
-  float* cl = reinterpret_cast<float*>(ring + Cfg::OFF_CL);
+    // join the warps in pairs, 2 and 3 into 0 and 1, then 1 into 0
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    const int r = ra + 8 * h;
-    if ((lane & 3) == 0) {
-      wm[warp * 16 + r] = m[h];
-      wl[warp * 16 + r] = l[h];
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
 #pragma unroll
-    for (int x = 0; x < D / 8; ++x)
-      *reinterpret_cast<float2*>(wo + (warp * 16 + r) * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * h], o[x][2 * h + 1]);
+    for (int half = 2; half > 0; half >>= 1) {
+      const int w = warp & (half - 1);
+      float4* jo = reinterpret_cast<float4*>(ring + Cfg::JOIN) + w * (16 * D / 4) + lane;
+      float2* jml = reinterpret_cast<float2*>(ring + Cfg::JOIN_ML) + w * 16 + ra;
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) jo[x * 32] = make_float4(o[x][0], o[x][1], o[x][2], o[x][3]);
+        if ((lane & 3) == 0) {
+          jml[0] = make_float2(m[0], l[0]);
+          jml[8] = make_float2(m[1], l[1]);
+        }
+      }
+      keys_meet();
+      if (warp < half) {
+        float own[2], his[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 other = jml[8 * h];
+          const float top = fmaxf(m[h], other.x), base = top == -INFINITY ? 0.0f : top;
+          own[h] = exp2_fast(m[h] - base);
+          his[h] = exp2_fast(other.x - base);
+          l[h] = l[h] * own[h] + other.y * his[h];
+          m[h] = top;
+        }
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          const float4 f = jo[x * 32];
+          o[x][0] = o[x][0] * own[0] + f.x * his[0];
+          o[x][1] = o[x][1] * own[0] + f.y * his[0];
+          o[x][2] = o[x][2] * own[1] + f.z * his[1];
+          o[x][3] = o[x][3] * own[1] + f.w * his[1];
+        }
+      }
+      keys_meet();
+    }
+    if (warp == 0 && ok) {
+      const bool whole = !CUT || (i0 == 0 && i1 == u.tiles);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = ra + 8 * h;
+        if (u.row0 + r >= nrows) continue;
+        if (whole) {
+          const float inv = l[h] > 0.0f ? 1.0f / l[h] : 0.0f;
+          uint16_t* dst = out_row<D, BF16>(p, u, hk, r) + (lane & 3) * 2;
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x)
+            *reinterpret_cast<uint32_t*>(dst + x * 8) = pack2<BF16>(o[x][2 * h] * inv, o[x][2 * h + 1] * inv);
+        } else {
+          const Parts<D> parts(p);
+          const long long row = (2ll * blockIdx.x + (i0 == 0 ? 1 : 0)) * 16 + r;
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x)
+            *reinterpret_cast<float2*>(parts.o + row * D + x * 8 + (lane & 3) * 2) = make_float2(o[x][2 * h], o[x][2 * h + 1]);
+          if ((lane & 3) == 0) parts.ml[row] = make_float2(m[h], l[h]);
+        }
+      }
+    }
+    if (CUT && tid == 0 && hk == 0 && i0 == 0)
+      Parts<D>(p).span[x] = make_int2(team, team + (u.tiles - i1 + each - 1) / each);
+    left -= i1 - i0;
+    at.tile = u.tiles - 1;
+    at.next(p, units);
+  }
+  if constexpr (CUT) {  // units without a key are shared out by number
+    for (int x = team; x < units; x += p.teams) {
+      const Unit u = unit_at(p, x);
+      if (u.tiles > 0) continue;
+      clear(u);
+      if (tid == 0 && hk == 0) Parts<D>(p).span[x] = make_int2(0, 0);
+    }
   }
   __syncthreads();
-  auto weight = [](float part, float whole) { return part == -INFINITY ? 0.0f : exp2_fast(part - whole); };
-  for (int x = tid; x < 16 * D; x += kRowThreads) {
-    const int r = x / D;
-    const float top = fmaxf(fmaxf(wm[r], wm[16 + r]), fmaxf(wm[32 + r], wm[48 + r]));
-    float acc = 0.0f, sum = 0.0f;
+  if (tid == 0 && bar->abort_flag) {  // copies in flight land before the CTA leaves
+    const uint64_t c0 = globaltimer_ns();
+    while (globaltimer_ns() - c0 < 50ull * 1000ull * 1000ull) {
+    }
+  }
+  __syncthreads();
+}
+
+// A CTA a row of a group: adds up the parts of one that was cut, in the order
+// of its keys; each of eight warps takes every eighth part.
+constexpr int kJoinThreads = 256;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) k_window_join(const __grid_constant__ WinArgs p) {
+  constexpr int WARPS = kJoinThreads / 32, EACH = D / 32;
+  __shared__ float sums[WARPS][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int x = static_cast<int>(blockIdx.x / p.HK), hk = static_cast<int>(blockIdx.x - x * p.HK);
+  const int r = static_cast<int>(blockIdx.y);
+  griddep_launch();
+  griddep_wait();
+  const Parts<D> parts(p);
+  const int2 span = parts.span[x];
+  Unit u;
+  u.b = x / p.row_tiles;
+  u.row0 = (x - u.b * p.row_tiles) * 16;
+  if (span.x == span.y || u.row0 + r >= p.T * p.G) return;  // finished where it was computed
+  auto row_of = [&](int c) { return (2ll * (c * p.HK + hk) + (c == span.x ? 1 : 0)) * 16 + r; };
+  float top = -INFINITY;
+  for (int c = span.x + lane; c <= span.y; c += 32) top = fmaxf(top, parts.ml[row_of(c)].x);
+  float part[4][EACH];  // (asked for before the maximum is known)
+  auto load = [&](int c0) {
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const float f = weight(wm[y * 16 + r], top);
-      acc = fmaf(f, wo[y * 16 * D + x], acc);
-      sum = fmaf(f, wl[y * 16 + r], sum);
+      const int c = c0 + y * WARPS;
+      if (c <= span.y) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) part[y][e] = parts.o[row_of(c) * D + e * 32 + lane];
+      }
     }
-    co[x] = acc;
-    if (x % D == 0) {
-      cm[r] = top;
-      cl[r] = sum;
+  };
+  load(span.x + warp);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, acc[EACH];
+  for (int c = span.x + lane; c <= span.y; c += 32) {
+    const float2 ml = parts.ml[row_of(c)];
+    total = fmaf(ml.y, exp2_fast(ml.x - base), total);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) acc[e] = 0.0f;
+  for (int c0 = span.x + warp; c0 <= span.y; c0 += 4 * WARPS) {
+    if (c0 != span.x + warp) load(c0);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int c = c0 + y * WARPS;
+      if (c > span.y) break;
+      const float f = exp2_fast(parts.ml[row_of(c)].x - base);
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) acc[e] = fmaf(part[y][e], f, acc[e]);
     }
   }
-  if (p.split > 1) cluster_sync_all();
-  else __syncthreads();
-  // then the CTAs: CTA `rank` finishes the pairs of columns rank, rank + split, ...
-  const uint32_t co_at = smem_addr(co), cm_at = smem_addr(cm), cl_at = smem_addr(cl);
-  for (int x = rank * kRowThreads + tid; x < 16 * D / 2; x += p.split * kRowThreads) {
-    const int r = x / (D / 2);
-    if (row0 + r >= nrows) continue;
-    float top = -INFINITY;
-    for (int c = 0; c < p.split; ++c) {
-      uint32_t at;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(cm_at + r * 4), "r"(c));
-      top = fmaxf(top, ld_cluster_f(at));
-    }
-    float a0 = 0.0f, a1 = 0.0f, sum = 0.0f;
-    for (int c = 0; c < p.split; ++c) {
-      uint32_t at_m, at_l, at_o;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(cm_at + r * 4), "r"(c));
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_l) : "r"(cl_at + r * 4), "r"(c));
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(co_at + x * 8), "r"(c));
-      const float f = weight(ld_cluster_f(at_m), top);
-      sum = fmaf(f, ld_cluster_f(at_l), sum);
-      a0 = fmaf(f, ld_cluster_f(at_o), a0);
-      a1 = fmaf(f, ld_cluster_f(at_o + 4), a1);
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    *reinterpret_cast<uint32_t*>(out_row(r) + (x % (D / 2)) * 2) = pack2<BF16>(a0 * inv, a1 * inv);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) sums[warp][e * 32 + lane] = acc[e];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) sum += sums[w][threadIdx.x];
+    sum *= total > 0.0f ? 1.0f / total : 0.0f;
+    uint16_t* dst = out_row<D, BF16>(p, u, hk, r) + threadIdx.x;
+    if constexpr (BF16) *reinterpret_cast<__nv_bfloat16*>(dst) = __float2bfloat16_rn(sum);
+    else *reinterpret_cast<__half*>(dst) = __float2half_rn(sum);
   }
-  if (p.split > 1) cluster_sync_all();  // a CTA stays until its part has been read
 }
 
 // ------------------------------------------------------------------ host side
+uint64_t map_stride(long long elems, int n, int D) {  // axes of length one may have any
+  return static_cast<uint64_t>(n > 1 ? elems : D) * 2;
+}
+template <int D>
+int cache_map(CUtensorMap* map, const WinArgs& p, const void* at, long long s_s, long long s_h, long long s_b, int keys) {
+  const uint32_t box[4] = {64, static_cast<uint32_t>(keys), 1, 1};
+  const uint64_t dims[4] = {D, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.HK), static_cast<uint64_t>(p.B)};
+  const uint64_t strides[3] = {map_stride(s_s, p.S, D), map_stride(s_h, p.HK, D), map_stride(s_b, p.B, D)};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, at, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+template <int D>
+int rows_map(CUtensorMap* map, const WinArgs& p, const void* at, long long s_t, long long s_h, long long s_b) {
+  const uint32_t box[4] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tokens), 1};
+  const uint64_t dims[4] = {D, static_cast<uint64_t>(p.H), static_cast<uint64_t>(p.T), static_cast<uint64_t>(p.B)};
+  const uint64_t strides[3] = {map_stride(s_h, p.H, D), map_stride(s_t, p.T, D), map_stride(s_b, p.B, D)};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, at, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 template <int D, bool BF16>
 int launch_tiles(osc_ctx* ctx, const WinArgs& p) {
   using Cfg = WinCfg<D>;
   CUtensorMap mQ, mK, mV, mO;
-  const uint32_t box_q[4] = {64, static_cast<uint32_t>(p.G), static_cast<uint32_t>(p.tokens), 1};
-  const uint32_t box_k[4] = {64, kKeys, 1, 1};
-  const uint64_t one = D * 2;  // a stride for axes of length one
-  auto stride = [&](long long elems, int n) { return n > 1 ? static_cast<uint64_t>(elems) * 2 : one; };
-  const uint64_t dq[4] = {D, static_cast<uint64_t>(p.H), static_cast<uint64_t>(p.T), static_cast<uint64_t>(p.B)};
-  const uint64_t sq[3] = {stride(p.q_h, p.H), stride(p.q_t, p.T), stride(p.q_b, p.B)};
-  const uint64_t dk[4] = {D, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.HK), static_cast<uint64_t>(p.B)};
-  const uint64_t sk[3] = {stride(p.k_s, p.S), stride(p.k_h, p.HK), stride(p.k_b, p.B)};
-  const uint64_t so[3] = {stride(p.o_h, p.H), stride(p.o_t, p.T), stride(p.o_b, p.B)};
-  const uint64_t sv[3] = {stride(p.v_s, p.S), stride(p.v_h, p.HK), stride(p.v_b, p.B)};
-  const auto type = CU_TENSOR_MAP_DATA_TYPE_UINT16;
-  OSC_TRY(encode_tiled(&mQ, type, 4, p.q, dq, sq, box_q, CU_TENSOR_MAP_SWIZZLE_128B));
-  OSC_TRY(encode_tiled(&mK, type, 4, p.k, dk, sk, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
-  OSC_TRY(encode_tiled(&mV, type, 4, p.v, dk, sv, box_k, CU_TENSOR_MAP_SWIZZLE_128B));
-  OSC_TRY(encode_tiled(&mO, type, 4, p.out, dq, so, box_q, CU_TENSOR_MAP_SWIZZLE_128B));
+  OSC_TRY(rows_map<D>(&mQ, p, p.q, p.q_t, p.q_h, p.q_b));
+  OSC_TRY(cache_map<D>(&mK, p, p.k, p.k_s, p.k_h, p.k_b, kKeys));
+  OSC_TRY(cache_map<D>(&mV, p, p.v, p.v_s, p.v_h, p.v_b, kKeys));
+  OSC_TRY(rows_map<D>(&mO, p, p.out, p.o_t, p.o_h, p.o_b));
   OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(k_window_tiles<D, BF16>), Cfg::SMEM));
   return launch_pdl(ctx, k_window_tiles<D, BF16>, dim3(std::min(p.items, ctx->num_sms)), dim3(kWinThreads), Cfg::SMEM, "k_window_tiles", mQ, mK, mV, mO, p,
                     ctx->d_err);
 }
 
 template <int D, bool BF16>
-int launch_rows(osc_ctx* ctx, const WinArgs& p) {
+int launch_rows(osc_ctx* ctx, WinArgs& p) {
   using Cfg = RowCfg<D>;
-  OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(k_window_rows<D, BF16>), Cfg::SMEM));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.row_tiles * p.split), p.HK, p.B);
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(p.split);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  prof_begin(ctx);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_window_rows<D, BF16>, p);
-  if (e != cudaSuccess) return cuda_fail(e, "k_window_rows launch");
-  return check_launch(ctx, "k_window_rows");
+  CUtensorMap mK, mV;
+  OSC_TRY(cache_map<D>(&mK, p, p.k, p.k_s, p.k_h, p.k_b, kRowKeys));
+  OSC_TRY(cache_map<D>(&mV, p, p.v, p.v_s, p.v_h, p.v_b, kRowKeys));
+  const long long groups = static_cast<long long>(p.row_tiles) * p.HK * p.B;
+  if (groups >= (1ll << 31)) return fail(OSC_EINVAL, "osc_attention_window: %lld row tiles are too many", groups);
+  // the keys that a row tile can see at most
+  const long long keys = std::min<long long>(p.S, static_cast<long long>(p.window) + p.T + p.sinks);
+  const long long tiles = (keys + kRowKeys - 1) / kRowKeys;
+  const int slots = 2 * ctx->num_sms;  // CTAs that run at once
+  // Uncut, the call takes a group's time; cut, the CTAs' even share of all tiles,
+  // and some 7 us (12 tiles) for the look at the lengths, the cuts and the second
+  // kernel. 8 key/value heads of 128, ragged lengths, us uncut and cut: 8 x 512
+  // keys 8.8 and 12.1, 8 x 1024 13.7 and 12.7, 16 x 1024 15.0 and 17.7, 8 x 4096
+  // 41.1 and 21.8, 24 x 4096 48.6 and 44.2, 40 x 4096 63.9 and 66.9, 72 x 4096
+  // 95.6 and 116.1. (Tiles of all groups are counted in 31 bits.)
+  const bool cut = groups < slots && groups * tiles < (1ll << 30) && 10 * (tiles - 12) * slots > 11 * tiles * groups;
+  if (!cut) {
+    const auto kernel = k_window_rows<D, BF16, false>;
+    OSC_TRY(set_smem_attr(ctx, reinterpret_cast<const void*>(kernel), Cfg::SMEM));
+    return launch_pdl(ctx, kernel, dim3(static_cast<unsigned>(groups)), dim3(kRowThreads), Cfg::SMEM, "k_window_rows",
+                      mK, mV, p, ctx->d_err);
+  }
+  const int units = p.B * p.row_tiles;
+  p.teams = static_cast<int>(std::min<long long>(slots / p.HK, (units * tiles + kMinTiles - 1) / kMinTiles));
+  const int ctas = p.teams * p.HK;
+  OSC_TRY(stream_alloc(ctx, Parts<D>::bytes(ctas, units), &p.parts));
+  const auto kernel = k_window_rows<D, BF16, true>;
+  int st = set_smem_attr(ctx, reinterpret_cast<const void*>(kernel), Cfg::SMEM);
+  if (st == OSC_OK)
+    st = launch_pdl(ctx, kernel, dim3(static_cast<unsigned>(ctas)), dim3(kRowThreads), Cfg::SMEM, "k_window_rows", mK, mV,
+                    p, ctx->d_err);
+  if (st == OSC_OK)
+    st = launch_pdl(ctx, k_window_join<D, BF16>, dim3(static_cast<unsigned>(groups), std::min(16, p.T * p.G)),
+                    dim3(kJoinThreads), 0, "k_window_join", p);
+  const int freed = stream_free(ctx, p.parts);
+  return st != OSC_OK ? st : freed;
 }
 
 template <int D, bool BF16>
@@ -909,11 +1219,6 @@ int launch(osc_ctx* ctx, WinArgs& p) {
   const long long rows = static_cast<long long>(p.T) * p.G;
   if (rows <= 32) {
     p.row_tiles = static_cast<int>((rows + 15) / 16);
-    // CTAs to fill the SMs twice, each with two tiles of keys at least
-    const long long keys = std::min<long long>(p.S, static_cast<long long>(p.window) + p.T + p.sinks);
-    const long long groups = static_cast<long long>(p.row_tiles) * p.HK * p.B;
-    p.split = 1;
-    while (p.split < 8 && groups * p.split < 2ll * ctx->num_sms && keys > 2ll * p.split * 2 * kRowKeys) p.split *= 2;
     return launch_rows<D, BF16>(ctx, p);
   }
   p.tokens = 128 / p.G;

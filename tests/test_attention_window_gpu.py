@@ -73,7 +73,7 @@ def _hide(k, v, lengths):
         k[b, n:], v[b, n:] = math.nan, math.inf
 
 
-def _case(ctx, B, T, S, H, HK, D, dtype, window, sinks, lengths, starts=None, scale=None, seed=0):
+def _case(ctx, B, T, S, H, HK, D, dtype, window, sinks, lengths, starts=None, scale=None, seed=0, gone=False):
     import torch
 
     from onnxsharp_b200.runtime import attention_window
@@ -84,6 +84,10 @@ def _case(ctx, B, T, S, H, HK, D, dtype, window, sinks, lengths, starts=None, sc
     scale = scale or D**-0.5
     ref, tol = _reference(q, k, v, lengths, starts, scale, window, sinks)
     _hide(k, v, lengths)
+    if gone:  # tokens that no row sees any more
+        for b, n in enumerate(lengths.tolist()):
+            lo = max(0, n - T if starts is None else int(starts[b])) - window + 1
+            k[b, sinks : max(lo, sinks)], v[b, sinks : max(lo, sinks)] = math.nan, math.inf
     got = attention_window(ctx, q, k, v, lengths, scale, window=window, sinks=sinks, starts=starts)
     ctx.synchronize()
     _check(got, ref, tol)
@@ -119,6 +123,33 @@ def test_starts(ctx, T, window, sinks):
 @pytest.mark.parametrize("T,G", [(1, 1), (16, 128), (1, 32), (2, 16), (4, 8), (1, 33), (64, 100)])
 def test_groups(ctx, T, G):
     _case(ctx, 1, T, 300, 2 * G, 2, 64, "bf16", 90, 2, [280])
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize(
+    "T,H,HK,S,lengths,starts",
+    [
+        (1, 8, 1, 9001, [9001], None),
+        (1, 8, 2, 3001, [3001, 1, 0, 2999, 64, 65, 0], None),
+        (8, 8, 2, 2500, [2500, 3, 1300], [2492, 0, 1000]),  # two row tiles, padded batches
+        (3, 6, 6, 1999, [5, 1999, 1998, 0], [2, 1999, 1990, 0]),
+        (1, 74, 37, 2100, [2100, 900], None),  # SMs that the heads do not divide
+        (1, 2, 1, 20000, [17777], None),
+        (2, 16, 1, 4100, [4100, 1, 3, 0, 0, 4097, 2, 1, 1, 1], None),
+    ],
+)
+@pytest.mark.parametrize("window,sinks", [(10**6, 0), (1000, 0), (1500, 70), (900, 3)])
+def test_cut_sequences(ctx, dtype, D, T, H, HK, S, lengths, starts, window, sinks):
+    """Few groups with many keys: CTAs share them, whatever sequence their keys belong to."""
+    _case(ctx, len(lengths), T, S, H, HK, D, dtype, window, sinks, lengths, starts, gone=True)
+
+
+@pytest.mark.parametrize("T", [1, 4, 9, 40, 300])
+@pytest.mark.parametrize("window,sinks", [(64, 0), (65, 5), (200, 129), (10, 1)])
+def test_forgotten_tokens(ctx, T, window, sinks):
+    """NaN and infinities between the sinks and the window of the first query."""
+    _case(ctx, 2, T, 777, 8, 2, 64, "bf16", window, sinks, [777, 600], gone=True)
+    _case(ctx, 3, T, 777, 4, 4, 128, "f16", window, sinks, [777, 700, 0], [400, 650, 0], gone=True)
 
 
 @pytest.mark.parametrize("T", [1, 200])
