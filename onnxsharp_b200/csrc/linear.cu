@@ -49,6 +49,8 @@ constexpr int kCols = 128;               // output columns of a CTA
 constexpr int kKB = 128;                 // bytes of K in a block: one swizzle row
 constexpr int kWBytes = kCols * kKB;     // 16 KB
 constexpr int kMaxStages = 8;
+constexpr int kBlocks = 2;               // k-blocks of a ring stage: one would wait, elect and commit for every block
+                                         // (8192 x 4096 x 16384 bf16 737 us for 679), three or four leave too few stages
 constexpr int kTileEpi = 16;             // epilogue warps of k_linear_tiles
 constexpr int kSplitEpi = 4;             // of k_linear_split: several CTAs share an SM
 constexpr int kSmemTail = 512;           // barriers
@@ -59,7 +61,6 @@ constexpr int kMaxSplit = 8;             // portable cluster size
 struct LinArgs {
   int M, N, num_kb, last_steps;  // last_steps: 32-byte K steps of the last block
   int bn;                        // tokens of a tile
-  int kbs;                       // k-blocks of a ring stage
   int stages, stage_bytes;
   int tiles_m, tiles_n;          // token tiles, column tiles (of 256 for a CTA pair)
   int split;                     // CTAs that share a tile's K
@@ -350,11 +351,11 @@ __global__ void k_linear_rows(const uint8_t* __restrict__ a, int m, int k_bytes,
 // ------------------------------------------------------------------ many tokens
 // Persistent CTAs (or CTA pairs, cta_group::2: 256 columns a tile, each CTA
 // streams its own 128 columns of weights and half of the tokens) walk the
-// tiles, eight token tiles by all column tiles at a time so that the tiles in
+// tiles, sixteen token tiles by all column tiles at a time so that the tiles in
 // flight share operands in L2. Two 256-column TMEM accumulators: the MMA warp
 // fills one while the epilogue warps empty the other.
 __device__ __forceinline__ void tile_at(const LinArgs& p, int t, int& tm, int& tn) {
-  constexpr int kGroup = 8;
+  constexpr int kGroup = 16;  // 8192 x 4096 x 16384 bf16, clocks settled: 809 us, with 8 815
   const int per = kGroup * p.tiles_n;
   const int g = t / per, in = t - g * per;
   const int h = min(kGroup, p.tiles_m - g * kGroup);
@@ -436,13 +437,13 @@ __global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
       if (!waited) {
         // the weights were laid out before this launch was made: their first
         // blocks travel while the previous kernel on the stream drains
-        for (int kb = 0; pre < p.stages && kb < p.num_kb; kb += p.kbs, ++pre)
-          load_w(pre, w_row + kb * kCols, min(p.kbs, p.num_kb - kb));
+        for (int kb = 0; pre < p.stages && kb < p.num_kb; kb += kBlocks, ++pre)
+          load_w(pre, w_row + kb * kCols, min(kBlocks, p.num_kb - kb));
         griddep_wait();
         waited = true;
       }
-      for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
-        const int s = at.s, blocks = min(p.kbs, p.num_kb - kb);
+      for (int kb = 0; kb < p.num_kb; kb += kBlocks, at.next(p.stages)) {
+        const int s = at.s, blocks = min(kBlocks, p.num_kb - kb);
         if (pre > 0) {
           --pre;
         } else {
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
           load_w(s, w_row + kb * kCols, blocks);
         }
         if (elect_one()) {
-          uint8_t* st = ring + s * p.stage_bytes + p.kbs * kWBytes;
+          uint8_t* st = ring + s * p.stage_bytes + kBlocks * kWBytes;
           for (int y = 0; y < blocks; ++y) {
             if (PAIR) tma_load_2d_pair(st + y * arows * kKB, &mA, full0 + static_cast<uint32_t>(s * 8), (kb + y) * kKB, a_row);
             else tma_load_2d(st + y * arows * kKB, &mA, &b->full[s], (kb + y) * kKB, a_row);
@@ -479,12 +480,12 @@ __global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
         if (!wait(&b->acc_empty[buf], ((it >> 1) & 1u) ^ 1u)) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(buf * 256);
-        for (int kb = 0; kb < p.num_kb; kb += p.kbs, at.next(p.stages)) {
-          const int s = at.s, blocks = min(p.kbs, p.num_kb - kb);
+        for (int kb = 0; kb < p.num_kb; kb += kBlocks, at.next(p.stages)) {
+          const int s = at.s, blocks = min(kBlocks, p.num_kb - kb);
           ok = wait(&b->full[s], at.phase);
           if (!ok) break;
           const uint32_t base = smem_addr(ring + s * p.stage_bytes);
-          const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + p.kbs * kWBytes);
+          const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + kBlocks * kWBytes);
           if (elect_one()) {
             for (int y = 0; y < blocks; ++y) {
               const uint64_t dw = dw0 + static_cast<uint64_t>(y * (kWBytes >> 4)), da = da0 + static_cast<uint64_t>(y * (arows * kKB >> 4));
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
                 }
             }
             commit(&b->empty[s]);
-            if (kb + p.kbs >= p.num_kb) commit(&b->acc_full[buf]);
+            if (kb + kBlocks >= p.num_kb) commit(&b->acc_full[buf]);
           }
         }
       }
@@ -568,7 +569,7 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
+__global__ void __launch_bounds__(64 + 32 * kSplitEpi, 2)
     k_linear_split(const __grid_constant__ CUtensorMap mW, const __grid_constant__ CUtensorMap mA,
                    const __grid_constant__ LinArgs p, uint32_t tmem_cols, int* __restrict__ err) {
   extern __shared__ uint8_t smem_raw[];
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
     const int w_row = (tn * p.num_kb + kb0) * kCols;
     auto load_w = [&](int s, int kc) {
       if (elect_one()) {
-        const int blocks = min(p.kbs, kbn - kc);
+        const int blocks = min(kBlocks, kbn - kc);
         mbar_arrive_expect_tx(&b->full[s], blocks * (kWBytes + p.bn * kKB));
         for (int y = 0; y < blocks; ++y)
           tma_load_2d(ring + s * p.stage_bytes + y * kWBytes, &mW, &b->full[s], 0, w_row + (kc + y) * kCols);
@@ -620,10 +621,10 @@ __global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
     // the weights were laid out before this launch was made: the first blocks
     // land while the previous kernel on the stream drains
     int pre = 0;
-    for (int kc = 0; pre < p.stages && kc < kbn; kc += p.kbs, ++pre) load_w(pre, kc);
+    for (int kc = 0; pre < p.stages && kc < kbn; kc += kBlocks, ++pre) load_w(pre, kc);
     griddep_wait();
     RingPos at;
-    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
+    for (int kc = 0; kc < kbn; kc += kBlocks, at.next(p.stages)) {
       const int s = at.s;
       if (pre > 0) {
         --pre;
@@ -632,16 +633,16 @@ __global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
         load_w(s, kc);
       }
       if (elect_one())
-        for (int y = 0; y < min(p.kbs, kbn - kc); ++y)
-          tma_load_2d(ring + s * p.stage_bytes + p.kbs * kWBytes + y * p.bn * kKB, &mA, &b->full[s], (kb0 + kc + y) * kKB, m0);
+        for (int y = 0; y < min(kBlocks, kbn - kc); ++y)
+          tma_load_2d(ring + s * p.stage_bytes + kBlocks * kWBytes + y * p.bn * kKB, &mA, &b->full[s], (kb0 + kc + y) * kKB, m0);
     }
   } else if (warp == 1) {
     RingPos at;
-    for (int kc = 0; kc < kbn; kc += p.kbs, at.next(p.stages)) {
-      const int s = at.s, blocks = min(p.kbs, kbn - kc);
+    for (int kc = 0; kc < kbn; kc += kBlocks, at.next(p.stages)) {
+      const int s = at.s, blocks = min(kBlocks, kbn - kc);
       if (!wait(&b->full[s], at.phase)) break;
       const uint32_t base = smem_addr(ring + s * p.stage_bytes);
-      const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + p.kbs * kWBytes);
+      const uint64_t dw0 = sdesc_kmajor_sw128(base), da0 = sdesc_kmajor_sw128(base + kBlocks * kWBytes);
       if (elect_one()) {
         for (int y = 0; y < blocks; ++y) {
           const uint64_t dw = dw0 + static_cast<uint64_t>(y * (kWBytes >> 4)), da = da0 + static_cast<uint64_t>(y * (p.bn * kKB >> 4));
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__(64 + 32 * kSplitEpi, 4)
             }
         }
         mma_commit(&b->empty[s]);
-        if (kc + p.kbs >= kbn) mma_commit(&b->acc_full[0]);
+        if (kc + kBlocks >= kbn) mma_commit(&b->acc_full[0]);
       }
     }
   }
@@ -800,8 +801,6 @@ struct LinPlan {
   bool split_kernel;
   bool pair;
   int bn, split;
-  int per_sm;  // CTAs of k_linear_split that an SM's shared memory is cut for
-  int kbs;     // k-blocks of a ring stage
 };
 
 int div_up(int a, int b) { return (a + b - 1) / b; }
@@ -839,7 +838,7 @@ LinPlan choose(int num_sms, const LinShape& z) {
       const double waves = std::ceil(ctas / (2 * num_sms)), per_sm = ctas > num_sms ? 2 : 1;
       const double mma = 4 * std::max(50.0, bn / 2.0) / 1800;
       const double kb = std::max({0.37, per_sm * (kWBytes + bn * kKB) / 95e3, per_sm * mma});
-      consider({true, false, bn, split, 2, 2},
+      consider({true, false, bn, split},
                3.4 + std::max(bytes_us, waves * div_up(z.num_kb, split) * kb + 0.57 * (waves - 1)) + 0.018 * bn +
                    (split > 1 ? 1.7 + 0.02 * bn : 0));
     }
@@ -852,7 +851,7 @@ LinPlan choose(int num_sms, const LinShape& z) {
       const double waves = std::ceil(tiles / (num_sms / (pair ? 2 : 1)));
       const double kb = std::max(0.154, pair ? 0.107 + 0.00052 * bn : 0.072 + 0.00093 * bn);
       const double main = z.num_kb * kb, tail = 0.76 + 0.0071 * bn;
-      consider({false, pair != 0, bn, 1, 1, 2},
+      consider({false, pair != 0, bn, 1},
                3.9 + (pair ? 0.6 : 0) + std::max(bytes_us, main + (waves - 1) * std::max(main, tail) + tail));
     }
   }
@@ -1051,9 +1050,8 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   p.bn = pl.bn;
   p.split = pl.split;
   const int arows = pl.pair ? pl.bn / 2 : pl.bn;
-  p.kbs = pl.kbs;
-  p.stage_bytes = p.kbs * (kWBytes + arows * kKB);
-  p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemSm / pl.per_sm - 2048 : kSmemOne) - kSmemTail) / p.stage_bytes);
+  p.stage_bytes = kBlocks * (kWBytes + arows * kKB);
+  p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemSm / 2 - 2048 : kSmemOne) - kSmemTail) / p.stage_bytes);
   p.tiles_m = div_up(m, pl.bn);
   p.tiles_n = div_up(w->n, pl.pair ? 2 * kCols : kCols);
   if (static_cast<long long>(p.tiles_m) * p.tiles_n * pl.split >= (1ll << 31) || m > (1 << 30))
