@@ -993,7 +993,7 @@ OSC_API int osc_linear_prepack(osc_ctx* ctx, int dtype, const void* w, int k, in
   if (dtype == OSC_S8 && k >= (1 << 17)) return fail(OSC_EINVAL, "osc_linear_prepack: k %d overflows S32 sums", k);
   // rows of 128 bytes are TMA coordinates (signed 32 bits); the grid's y axis holds groups of 32 columns
   const long long kb = (static_cast<long long>(k) * dtype_bytes(dtype) + kKB - 1) / kKB;
-  if (div_up(n, 32) > 65532 || (static_cast<long long>(div_up(n, kCols)) + 1) * kb * kCols >= (1ll << 31))
+  if (n > 65532 * 32 || (static_cast<long long>(div_up(n, kCols)) + 1) * kb * kCols >= (1ll << 31))
     return fail(OSC_EINVAL, "osc_linear_prepack: W [%d, %d] is too large", k, n);
   if (!aligned(w, dtype_bytes(dtype))) return fail(OSC_EINVAL, "osc_linear_prepack: W is not aligned to its type");
   OSC_TRY(enter(ctx));
@@ -1017,7 +1017,7 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   if (ctx == nullptr) return fail(OSC_EINVAL, "null context");
   if (w == nullptr) return fail(OSC_EINVAL, "osc_linear: null weights");
   if (w->device != ctx->device) return fail(OSC_EINVAL, "osc_linear: weights of device %d on device %d", w->device, ctx->device);
-  if (m < 0) return fail(OSC_EINVAL, "osc_linear: m = %d", m);
+  if (m < 0 || m > (1 << 30)) return fail(OSC_EINVAL, "osc_linear: m = %d", m);
   const bool coded = w->dtype == OSC_S8 || w->dtype == OSC_E4M3;
   if (out_dtype != OSC_F32 && out_dtype != OSC_F16 && out_dtype != OSC_BF16)
     return fail(OSC_EINVAL, "osc_linear: output dtype %d is not f32, f16 or bf16", out_dtype);
@@ -1054,7 +1054,7 @@ OSC_API int osc_linear(osc_ctx* ctx, const void* a, int m, long long lda, const 
   p.stages = std::min(kMaxStages, ((pl.split_kernel ? kSmemSm / 2 - 2048 : kSmemOne) - kSmemTail) / p.stage_bytes);
   p.tiles_m = div_up(m, pl.bn);
   p.tiles_n = div_up(w->n, pl.pair ? 2 * kCols : kCols);
-  if (static_cast<long long>(p.tiles_m) * p.tiles_n * pl.split >= (1ll << 31) || m > (1 << 30))
+  if (static_cast<long long>(p.tiles_m) * p.tiles_n * pl.split >= (1ll << 31))
     return fail(OSC_EINVAL, "osc_linear: %d rows are too many", m);
   const uint32_t rows = pl.pair ? 256u : 128u;
   const uint32_t size = (static_cast<uint32_t>(pl.bn >> 3) << 17) | ((rows >> 4) << 24);
