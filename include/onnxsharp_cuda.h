@@ -67,7 +67,7 @@ enum osc_act { OSC_ACT_NONE = 0, OSC_ACT_SILU = 1, OSC_ACT_RELU = 2, OSC_ACT_SIG
                OSC_ACT_GELU_TANH = 5,  /* its tanh form; osc_linear only */
                OSC_ACT_FAST = 16 };
 
-/* Element types of the entries that take more than FP32 (osc_rmsnorm, osc_linear). */
+/* Element types of the entries that take more than FP32 (osc_rmsnorm, osc_linear, osc_attention_window). */
 enum osc_dtype { OSC_F32 = 0, OSC_F16 = 1, OSC_BF16 = 2, OSC_S8 = 3, OSC_E4M3 = 4 };
 
 typedef struct osc_ctx osc_ctx;
@@ -421,10 +421,13 @@ OSC_API int osc_attention_f32(osc_ctx* ctx, const float* q, const float* k, cons
  *
  * FP32 scores, softmax and sums; the probabilities are rounded to the type for
  * the product with v, the result once more. Queries outside 0 .. lengths[b] - 1
- * (padding) give zeros. What the cache holds at and behind lengths[b] does not
- * matter (NaN included); v before it must be finite. window >= 1 (INT_MAX:
- * none), sinks >= 0, scale > 0. out may not overlap the inputs. No scratch
- * memory; results do not change from run to run. */
+ * (padding) give zeros. What the cache holds at and behind lengths[b], and
+ * between the sinks and the window of the call's first query, does not matter
+ * (NaN included); other v must be finite. window >= 1 (INT_MAX: none), sinks >=
+ * 0, scale > 0. out may not overlap the inputs. Calls with few rows and many
+ * keys take a temporary, allocated and freed in stream order; calls on different
+ * streams or in different graphs share nothing. Results do not change from run
+ * to run. */
 OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const long long* q_strides, const void* k,
                                  const long long* k_strides, const void* v, const long long* v_strides,
                                  const int* lengths, const int* starts, int B, int T, int S, int H, int HK, int D,

@@ -266,3 +266,71 @@ def test_refusals(ctx):
         attention_window(ctx, q.cpu(), k, v, n, 1.0)
     with pytest.raises(ValueError, match="dense"):
         attention_window(ctx, q.transpose(2, 3).contiguous().transpose(2, 3), k, v, n, 1.0)
+
+
+def test_cut_sequences_in_two_graphs():
+    """The parts of cut sequences belong to a call: two graphs of one context and an eager call on another stream."""
+    import torch
+
+    from onnxsharp_b200.runtime import Context, attention_window
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [Context(0, s.cuda_stream) for s in streams]
+    lengths = torch.tensor([6000, 100, 3500], dtype=torch.int32, device="cuda")
+    cases = []
+    for i in range(2):
+        q, k, v = _inputs(3, 1, 6000, 8, 2, 128, "bf16", seed=i)
+        cases.append((q, k, v, torch.empty_like(q)))
+    torch.cuda.synchronize()
+    run = lambda c, x: attention_window(c, x[0], x[1], x[2], lengths, 0.1, out=x[3])  # noqa: E731
+    graphs = [ctxs[0].capture(lambda x=x: run(ctxs[0], x)) for x in cases]
+    want = [x[3].clone() for x in cases]
+    for x, w in zip(cases, want):
+        _check(w, *_reference(x[0], x[1], x[2], lengths, None, 0.1, 10**6, 0))
+    for _ in range(5):
+        for x in cases:
+            x[3].fill_(7.0)
+        torch.cuda.synchronize()
+        graphs[0].launch()
+        run(ctxs[1], cases[1])
+        ctxs[1].synchronize()
+        graphs[1].launch()
+        graphs[0].launch()
+        ctxs[0].synchronize()
+        assert all(bool((x[3] == w).all()) for x, w in zip(cases, want))
+    for g in graphs:
+        g.close()
+    for c in ctxs:
+        c.close()
+
+
+@pytest.mark.parametrize("T,S", [(1, 40), (1, 3001), (60, 300)])
+def test_shared_cache(ctx, T, S):
+    """One cache behind several sequences, one key/value head behind several groups (strides of 0)."""
+    import torch
+
+    from onnxsharp_b200.runtime import attention_window
+
+    q, k, v = _inputs(3, T, S, 8, 1, 64, "bf16")
+    k, v = (t[:1].expand(3, S, 2, 64) for t in (k, v))
+    lengths = torch.tensor([S, S - 1, S // 2], dtype=torch.int32, device="cuda")
+    got = attention_window(ctx, q, k, v, lengths, 0.1, window=200, sinks=1)
+    ctx.synchronize()
+    _check(got, *_reference(q, k, v, lengths, None, 0.1, 200, 1))
+
+
+def test_failing_allocation_is_reported(ctx, monkeypatch):
+    import torch
+
+    from onnxsharp_b200 import OscError
+    from onnxsharp_b200.runtime import attention_window
+
+    q, k, v = _inputs(1, 1, 6000, 8, 2, 128, "bf16")
+    lengths = torch.tensor([6000], dtype=torch.int32, device="cuda")
+    monkeypatch.setenv("OSC_FAULT", "alloc")
+    with pytest.raises(OscError, match="injected"):
+        attention_window(ctx, q, k, v, lengths, 0.1)
+    monkeypatch.delenv("OSC_FAULT")
+    got = attention_window(ctx, q, k, v, lengths, 0.1)
+    ctx.synchronize()
+    _check(got, *_reference(q, k, v, lengths, None, 0.1, 10**6, 0))
