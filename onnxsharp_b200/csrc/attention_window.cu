@@ -108,7 +108,10 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 //   producer warps one for Q and K, one for V, two TMA stages each
 // The result goes out by TMA from the Q buffer that it replaces. The
 // special-function units bound it: 128 x 128 exponentials are 1024 cycles of an
-// SM, as are the two products (16 MMAs of 64).
+// SM, as are the two products (16 MMAs of 64). Two prompts of 4096 (16 heads over
+// 4, window 1024): 65.5 us, some 1400 cycles a key tile and 3000 from row tile to
+// row tile. (Four more warps that finish row tiles meanwhile, on registers that
+// the others give up: 82 us; the softmax then has too few.)
 constexpr int kKeys = 128;
 constexpr int kWinThreads = 384;  // Q and K producer, S, V producer, P V; 8 softmax warps
 constexpr float kLazy = 8.0f;     // O is rescaled when a maximum has grown by more than 2^8: P stays
@@ -598,7 +601,9 @@ __global__ void __launch_bounds__(kWinThreads, 1)
 // A group that lies in one CTA is finished there; of one that is cut the parts
 // go to a workspace of the call and k_window_join adds them up in the order of
 // the keys: where the cuts lie depends on lengths and the number of SMs alone,
-// so the bits are the same every run.
+// so the bits are the same every run. One token of 16 sequences (8 key/value
+// heads of 128, 210 MB of cache): 43.4 us, 4.8 TB/s; a cluster of up to 8 CTAs a
+// group took 48.3. One of 32768 keys: 32.7 for 57.3.
 constexpr int kRowKeys = 64, kRowStages = 3;
 constexpr int kRowThreads = 160;  // four warps of keys, the producer
 
