@@ -148,3 +148,70 @@ def test_prompt_then_tokens(kind, batch, prompt):
         graph.close()
     torch.cuda.synchronize()
     c.close()
+
+
+def _far(shape, seed):
+    """A large bf16 tensor, cheaply: random rows repeated."""
+    import torch
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    row = torch.randn((4099, shape[-1]), generator=g, device="cuda").bfloat16()
+    return row[torch.arange(shape[0], device="cuda") % 4099]
+
+
+def test_norm_rows_behind_two_to_the_31(ctx):
+    import torch
+
+    from onnxsharp_b200 import ops
+
+    rows, cols = 530000, 4096
+    x = _far((rows, cols), 1)
+    q, s = torch.empty((rows, cols), dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    ops.rmsnorm_quant(ctx, x, None, 1e-6, q, s)
+    y = ops.rmsnorm(ctx, x, None, 1e-6, torch.empty_like(x))
+    ctx.synchronize()
+    for part in (slice(0, 8), slice(2**31 // cols - 4, 2**31 // cols + 4), slice(rows - 8, rows)):
+        norm._check(x[part], None, None, 1e-6, "s8", y=y[part], q=q[part], scales=s[part])
+
+
+def test_product_rows_behind_two_to_the_31(ctx):
+    import torch
+
+    from onnxsharp_b200.runtime import LinearWeights, linear
+
+    m, k, n = 140001, 72, 16000
+    a, res = _far((m, k), 2), torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+    w = _far((k, n), 3)
+    spots = (slice(0, 8), slice(2**31 // n - 4, 2**31 // n + 4), slice(m - 8, m))
+    for p in spots:
+        res[p] = _far((8, n), 4)
+    kept = [res[p].clone() for p in spots]
+    linear(ctx, a, LinearWeights(ctx, w), residual=res, out=res)
+    ctx.synchronize()
+    for p, r in zip(spots, kept):
+        v = a[p].double() @ w.double()
+        err = (math.ceil(k * 2 / 32) + 1) * 2.0**-22 * (a[p].double().abs() @ w.double().abs()) + 2.0**-22 * v.abs()
+        v = v + r.double()
+        tol = err + 2.0**-8 * (v.abs() + err) * 1.0001 + 2.0**-23 * v.abs()
+        assert bool(((res[p].double() - v).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_cache_rows_behind_two_to_the_31(ctx, T):
+    import torch
+
+    from onnxsharp_b200.runtime import attention_window
+
+    S, heads, dim, near = 2**21 + 700, 8, 128, 6000
+    cache = torch.zeros((1, S, heads, dim), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    n = S - 37
+    cache[:, n - near : n] = torch.randn((1, near, heads, dim), generator=g, device="cuda").bfloat16()
+    q = torch.randn((1, T, 16, dim), generator=g, device="cuda").bfloat16()
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    got = attention_window(ctx, q, cache, cache, lengths, dim**-0.5, window=4000)
+    ctx.synchronize()
+    part = cache[:, n - near : n]
+    win._check(got, *win._reference(q, part, part, torch.tensor([near]), None, dim**-0.5, 4000, 0))
