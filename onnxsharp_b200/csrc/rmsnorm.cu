@@ -462,8 +462,10 @@ int launch_norm(osc_ctx* ctx, const NormArgs& p, bool vectors) {
     return launch_pdl(ctx, k_rmsnorm_long<T>, dim3(static_cast<unsigned>(p.rows)), dim3(kMaxThreads), 0,
                       "k_rmsnorm_long", p);
   if (vectors) {
-    // few rows are spread over as many threads as fit at once
-    if (p.rows * threads_for(VEC) <= 1024ll * ctx->num_sms && threads_for(VEC) <= kMaxThreads)
+    // few rows are spread over as many threads as the SMs hold: a vector a thread
+    // instead of 16 elements takes 300 x 2048 f32 -> s8 from 5.4 to 4.2 us, 2048 x
+    // 1024 bf16 from 5.5 to 5.3, but 1000 x 4096 bf16 -> e4m3 from 11.3 to 12.7
+    if (p.rows * threads_for(VEC) <= 2048ll * ctx->num_sms && threads_for(VEC) <= kMaxThreads)
       return launch_rows<T, VEC, 1, CODES>(ctx, p, threads_for(VEC));
     return launch_rows<T, VEC, NV, CODES>(ctx, p, threads_for(VEC * NV));
   }
