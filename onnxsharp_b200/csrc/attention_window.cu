@@ -984,6 +984,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
           mma_16816<BF16>(o[2 * dn + 1], pf, vf[2], vf[3]);
         }
       }
+      // every lane's reads of the tile come before the copies that take its place:
+      // without the fence the last 16 columns of V were now and then the next tile's
+      fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->empty[slot]);
       advance();
@@ -1089,7 +1092,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_window_join(const __grid_const
   griddep_launch();
   griddep_wait();
   const Parts<D> parts(p);
-  const int2 span = parts.span[x];
+  int2 span = parts.span[x];
+  span.x = max(0, min(span.x, p.teams - 1));
+  span.y = max(span.x, min(span.y, p.teams - 1));  // (in bounds whatever memory holds)
   Unit u;
   u.b = x / p.row_tiles;
   u.row0 = (x - u.b * p.row_tiles) * 16;
@@ -1222,12 +1227,25 @@ int launch_rows(osc_ctx* ctx, WinArgs& p) {
 template <int D, bool BF16>
 int launch(osc_ctx* ctx, WinArgs& p) {
   const long long rows = static_cast<long long>(p.T) * p.G;
-  if (rows <= 32) {
+  p.tokens = 128 / p.G;
+  p.token_tiles = (p.T + p.tokens - 1) / p.tokens;
+  // Up to 16 rows the cache's bytes count alone. From there to 64 k_window_rows
+  // takes them once more for every 16 rows, but all SMs share them; k_window_tiles
+  // takes them once and walks a row tile's keys one after the other. 32/8 heads of
+  // 128, us by rows and by tiles: 1 x 4096 keys, 8 tokens 14.5 and 37.7, 16 tokens
+  // 19.3 and 37.6; 4 x 1024, 8 tokens 17.1 and 13.7; 16 x 8192, 5 tokens 55.3 and
+  // 44.5; 64 x 1024, 8 tokens 44.6 and 35.0.
+  bool by_rows = rows <= 16;
+  if (!by_rows && rows <= 64) {
+    const double keys = std::min<double>(p.S, static_cast<double>(p.window) + p.T + p.sinks), sms = ctx->num_sms;
+    const double groups = std::ceil(rows / 16.0) * p.HK * p.B;
+    const double waves = std::ceil(static_cast<double>(p.token_tiles) * p.HK * p.B / sms);
+    by_rows = 12 + 1.5 * groups * std::ceil(keys / kRowKeys) / (2 * sms) < 4 + 1.1 * waves * std::ceil(keys / kKeys);
+  }
+  if (by_rows) {
     p.row_tiles = static_cast<int>((rows + 15) / 16);
     return launch_rows<D, BF16>(ctx, p);
   }
-  p.tokens = 128 / p.G;
-  p.token_tiles = (p.T + p.tokens - 1) / p.tokens;
   const long long items = static_cast<long long>(p.token_tiles) * p.HK * p.B;
   if (items >= (1ll << 30)) return fail(OSC_EINVAL, "osc_attention_window: %lld row tiles are too many", items);
   p.items = static_cast<int>(items);
