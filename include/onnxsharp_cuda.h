@@ -421,9 +421,11 @@ OSC_API int osc_attention_f32(osc_ctx* ctx, const float* q, const float* k, cons
  *
  * FP32 scores, softmax and sums; the probabilities are rounded to the type for
  * the product with v, the result once more. Queries outside 0 .. lengths[b] - 1
- * (padding) give zeros. What the cache holds at and behind lengths[b], and
- * between the sinks and the window of the call's first query, does not matter
- * (NaN included); other v must be finite. window >= 1 (INT_MAX: none), sinks >=
+ * (padding) give zeros, whatever q holds there. What the cache holds at and
+ * behind lengths[b], and between the sinks and the window of the call's first
+ * query, does not matter (NaN included); other v must be finite. A query that is
+ * not finite, or sees such a key, gives what the formula does: NaN where a score
+ * is NaN or +inf, in its own rows alone. window >= 1 (INT_MAX: none), sinks >=
  * 0, scale > 0. out may not overlap the inputs. Calls with few rows and many
  * keys take a temporary, allocated and freed in stream order; calls on different
  * streams or in different graphs share nothing. Results do not change from run

@@ -519,12 +519,14 @@ __global__ void __launch_bounds__(kWinThreads, 1)
         const float2 his = exchange[(part ^ 1) * 128];
         if (ok) ok = wait(&bar->o_full, item);
         tc_fence_after();
-        // weights of the halves' O; a half without a key has l = 0
-        const float top = l > 0.0f ? (his.y > 0.0f ? fmaxf(m, his.x) : m) : his.x;
-        const float mine_w = l > 0.0f ? exp2_fast(m - top) : 0.0f, his_w = his.y > 0.0f ? exp2_fast(his.x - top) : 0.0f;
-        const float total = l * mine_w + his.y * his_w;
-        const float inv = live && total > 0.0f ? 1.0f / total : 0.0f;
-        const float f_mine = mine_w * inv, f_his = his_w * inv;
+        // weights of the halves' O; a half without a key has l = 0. (Asked by !=, not by
+        // >: a NaN among the row's scores has made l NaN and has to come out. A row that
+        // is padding may hold one too, and is zeros.)
+        const bool mine_has = live && l != 0.0f, his_has = live && his.y != 0.0f;
+        const float top = mine_has ? (his_has ? fmaxf(m, his.x) : m) : his.x;
+        const float mine_w = mine_has ? exp2_fast(m - top) : 0.0f, his_w = his_has ? exp2_fast(his.x - top) : 0.0f;
+        const float inv = 1.0f / (l * mine_w + his.y * his_w);
+        const float f_mine = mine_has ? mine_w * inv : 0.0f, f_his = his_has ? his_w * inv : 0.0f;
         const uint32_t o_his = lane_base + 256u + static_cast<uint32_t>((part ^ 1) * 128);
         uint8_t* stage = sq + (item & 1u) * Cfg::TILE;
 #pragma unroll
@@ -539,8 +541,8 @@ __global__ void __launch_bounds__(kWinThreads, 1)
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
             // selected, not multiplied away: a half without a product was never written
-            const float own = f_mine > 0.0f ? __uint_as_float(a[y]) * f_mine : 0.0f;
-            o[y] = f_his > 0.0f ? fmaf(__uint_as_float(c[y]), f_his, own) : own;
+            const float own = f_mine != 0.0f ? __uint_as_float(a[y]) * f_mine : 0.0f;
+            o[y] = f_his != 0.0f ? fmaf(__uint_as_float(c[y]), f_his, own) : own;
           }
           const int col = (c0 >> 6) * kKeys * 128, chunk0 = (c0 & 63) >> 3;
 #pragma unroll
