@@ -197,12 +197,14 @@ __device__ __forceinline__ float rstd_of(float ss, int cols, float eps) {
   return rsqrtf(ss / static_cast<float>(cols) + eps);
 }
 
-// Of a row whose finite elements' squares overflow FP32: the sum of (h / 2^64)^2
-// (eps is lost against it). An infinite or NaN element gives 0 or NaN, as the formula does.
-__device__ __forceinline__ float rstd_scaled(float ss, int cols) {
-  return rsqrtf(ss / static_cast<float>(cols)) * 5.421010862427522e-20f;
+// Of a row whose finite elements' squares overflow FP32: the sum of (h / 2^80)^2.
+// 2^31 elements below 2^128 stay below 2^127 so, a sum that overflowed is 2^-32 at
+// least, and eps counts where it is large too. An infinite or NaN element gives 0
+// or NaN, as the formula does.
+constexpr float kDown = 8.27180612553028e-25f;  // 2^-80
+__device__ __forceinline__ float rstd_scaled(float ss, int cols, float eps) {
+  return rsqrtf(ss / static_cast<float>(cols) + eps * kDown * kDown) * kDown;
 }
-constexpr float kDown = 5.421010862427522e-20f;  // 2^-64
 
 __device__ __forceinline__ bool live_peak(uint32_t peak) {
   return __uint_as_float(peak) >= kTiny && peak < 0x7f800000u;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsno
     uint32_t none = 0u;
     if (!WARP) __syncthreads();  // part is written again
     reduce_row<WARP, false>(ss, none, part, warps);
-    rstd = rstd_scaled(ss, p.cols);
+    rstd = rstd_scaled(ss, p.cols, p.eps);
   }
 
   if (!CODES || p.y != nullptr) {
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
     uint32_t none = 0u;
     __syncthreads();
     reduce_row<false, true>(ss, none, part, warps);
-    rstd = rstd_scaled(ss, p.cols);
+    rstd = rstd_scaled(ss, p.cols, p.eps);
   }
   RowCode c = {};
   if (p.q != nullptr) {
