@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(64 + 32 * kTileEpi, 1)
       }
     }
   } else if (warp == 1) {
+    griddep_wait();  // (its limited waits begin with this kernel's own work, not while the previous one runs)
     if (rank == 0) {
       const uint32_t own = PAIR ? mapa_shared(b, 0) : 0u, peer = PAIR ? mapa_shared(b, 1) : 0u;
       auto commit = [&](uint64_t* bar) {
@@ -667,6 +668,7 @@ __global__ void __launch_bounds__(64 + 32 * kSplitEpi, 2)
           tma_load_2d(ring + s * p.stage_bytes + kBlocks * kWBytes + y * p.bn * kKB, &mA, &b->full[s], (kb0 + kc + y) * kKB, m0);
     }
   } else if (warp == 1) {
+    griddep_wait();  // (its limited waits begin with this kernel's own work, not while the previous one runs)
     RingPos at;
     for (int kc = 0; kc < kbn; kc += kBlocks, at.next(p.stages)) {
       const int s = at.s, blocks = min(kBlocks, kbn - kc);
