@@ -95,12 +95,11 @@ def layernorm(ctx, x, gamma, beta, eps, y, inner=None):
 
 def _row_pitch(name, t, cols):
     """Row pitch of a [..., cols] tensor whose rows are dense and follow one another at one pitch."""
-    shape, stride = t.shape, t.stride()
-    ok = stride[-1] == 1 or cols == 1
-    for d in range(len(shape) - 2):  # leading dimensions fold into one run of rows
-        ok = ok and (shape[d] == 1 or stride[d] == stride[d + 1] * shape[d + 1])
-    pitch = stride[-2] if len(shape) > 1 and shape[-2] > 1 else next((s for n, s in zip(shape[-3::-1], stride[-3::-1])
-                                                                       if n > 1), cols)
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()) if n > 1]  # (a dimension of one may have any stride)
+    ok = t.stride(-1) == 1 or cols == 1
+    for (_, outer), (n, inner) in zip(lead, lead[1:]):  # leading dimensions fold into one run of rows
+        ok = ok and outer == inner * n
+    pitch = lead[-1][1] if lead else cols
     if not ok or pitch < cols:
         raise ValueError(f"{name}: rows must be dense and follow one another at one pitch")
     return pitch
