@@ -33,6 +33,8 @@ ACT_NONE, ACT_SILU, ACT_RELU, ACT_SIGMOID = 0, 1, 2, 3
 ACT_GELU, ACT_GELU_TANH = 4, 5  # osc_linear only
 ACT_FAST = 16  # OR into conv2d_direct's activation: hardware ex2/rcp Sigmoid/SiLU
 
+INT_MAX = 2**31 - 1  # ctypes keeps the low 32 bits of a larger number, without a word
+
 # element types (enum osc_dtype)
 F32, F16, BF16, S8, E4M3 = 0, 1, 2, 3, 4
 _dtypes: dict = {}

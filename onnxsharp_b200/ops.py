@@ -127,6 +127,8 @@ def _rmsnorm(ctx, x, gamma, eps, residual, sum_out, y, q, scales):
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError(f"x has no columns: {tuple(shape)}")
     cols = shape[-1]
+    if cols > _lib.INT_MAX:
+        raise ValueError(f"x has {cols} columns, more than an int counts")
     rows = x.numel() // cols
     ld, ld_r, ld_s, ld_y, ld_q = _rows_like("x", x, device, shape, dtype), 0, 0, 0, 0
     r = s = o = c = f = g = None

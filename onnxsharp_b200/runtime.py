@@ -318,6 +318,8 @@ class LinearWeights:
         if w.is_cuda and w.device.index != ctx.device:
             raise ValueError(f"LinearWeights: w is on {w.device}, the context on cuda:{ctx.device}")
         k, n = (w.shape[1], w.shape[0]) if layout else (w.shape[0], w.shape[1])
+        if max(k, n) > _lib.INT_MAX:
+            raise ValueError(f"LinearWeights: w is {tuple(w.shape)}: too large")
         h = C.c_void_p()
         call("osc_linear_prepack", ctx.handle, _lib.dtype_code(w.dtype), ptr(w), int(k), int(n), int(layout),
              0 if w.is_cuda else 1, C.byref(h))
@@ -360,6 +362,8 @@ def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NON
     if a.dim() != 2:
         raise ValueError(f"linear: a is {tuple(a.shape)}, expected (m, {w.k})")
     m, n = a.shape[0], w.n
+    if m > _lib.INT_MAX:
+        raise ValueError(f"linear: a has {m} rows, more than an int counts")
     if a.dtype != w.dtype:
         raise TypeError(f"linear: a is {a.dtype}, the weights are {w.dtype}")
     lda = _pitch("a", a, ctx, (m, w.k))
@@ -408,6 +412,11 @@ def attention(ctx: Context, q, k, v, heads: int, scale: float, mask=None, out_he
     return out
 
 
+def _int32(n: int) -> int:
+    """The nearest number that an int holds (INT_MAX: a window or sinks without an end)."""
+    return max(-_lib.INT_MAX - 1, min(n, _lib.INT_MAX))
+
+
 def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int | None = None, sinks: int = 0,
                      starts=None, out=None):
     """Causal attention over a cache: q [B, T, heads, D], k and v [B, capacity, kv heads, D] (float16 or bfloat16,
@@ -420,6 +429,8 @@ def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int |
     if len(shape) != 4 or len(keys) != 4 or v.shape != keys or shape[0] != keys[0] or shape[3] != keys[3]:
         raise ValueError(f"attention_window: q {tuple(shape)}, k {tuple(keys)}, v {tuple(v.shape)}")
     (B, T, H, D), (_, S, HK, _) = shape, keys
+    if max(shape + keys) > _lib.INT_MAX:
+        raise ValueError(f"attention_window: q {tuple(shape)}, k {tuple(keys)}: too large")
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=q.device)
     elif out.shape != shape:
@@ -443,7 +454,7 @@ def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int |
     st = (C.c_longlong * 12)(*strides)
     call("osc_attention_window", ctx.handle, _lib.dtype_code(dtype), q.data_ptr(), st, k.data_ptr(), C.byref(st, 24),
          v.data_ptr(), C.byref(st, 48), lengths.data_ptr(), None if starts is None else starts.data_ptr(), B, T, S, H, HK, D,
-         2**31 - 1 if window is None else window, sinks, scale, out.data_ptr(), C.byref(st, 72))
+         _lib.INT_MAX if window is None else _int32(window), _int32(sinks), scale, out.data_ptr(), C.byref(st, 72))
     return out
 
 
