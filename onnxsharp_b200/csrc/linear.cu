@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
 #include <new>
 
 #include "runtime.h"
@@ -916,7 +917,9 @@ int launch_tiles(osc_ctx* ctx, const LinPlan& pl, const CUtensorMap& mW, const C
   prof_begin(ctx);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mW, mA, p, ctx->d_err);
   if (e != cudaSuccess) return cuda_fail(e, "k_linear_tiles launch");
-  return check_launch(ctx, "k_linear_tiles");
+  char name[48] = "k_linear_tiles";  // with the plan where launches are recorded
+  if (ctx->prof_pending != nullptr) std::snprintf(name, sizeof(name), "k_linear_tiles %s %d", pl.pair ? "pair" : "single", pl.bn);
+  return check_launch(ctx, name);
 }
 
 template <int KIND>
@@ -943,7 +946,9 @@ int launch_split(osc_ctx* ctx, const CUtensorMap& mW, const CUtensorMap& mA, con
   prof_begin(ctx);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mW, mA, p, cols, ctx->d_err);
   if (e != cudaSuccess) return cuda_fail(e, "k_linear_split launch");
-  return check_launch(ctx, "k_linear_split");
+  char name[48] = "k_linear_split";
+  if (ctx->prof_pending != nullptr) std::snprintf(name, sizeof(name), "k_linear_split %d %d", p.split, p.bn);
+  return check_launch(ctx, name);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0; }
