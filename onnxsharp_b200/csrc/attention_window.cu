@@ -428,19 +428,15 @@ __global__ void __launch_bounds__(kWinThreads, 1)
       bool seen = false;     // the row has had a key of this half
       int had = 0;           // steps of this item that wanted this half
       uint32_t s[64];
-      bool loaded = false;   // the scores of the step at hand are on their way to s
       for (int i = 0; i < w.n; ++i, ++step) {
         const int j0 = w.key0(i);
         const uint32_t s_at = lane_base + static_cast<uint32_t>((step & 1u) * kKeys + part * 64);
         const bool plain = j0 >= w.plain_lo && j0 <= w.plain_hi;
         // both halves take part in every step: the scores after next wait for both
-        if (!loaded) {
-          if (ok) ok = wait(&bar->s_full[step & 1u], step >> 1);
-          tc_fence_after();
-        }
+        if (ok) ok = wait(&bar->s_full[step & 1u], step >> 1);
+        tc_fence_after();
         if (plain || wanted(p, w, j0 + part * 64)) {
-          if (!loaded) tmem_ld64(s_at, s);
-          loaded = false;
+          tmem_ld64(s_at, s);
           // The probabilities are taken relative to the maximum so far (0 before a
           // row's first key) while this tile's own is still being found; should that
           // be more than 2^8 above it, or a row's first keys all below it, the
