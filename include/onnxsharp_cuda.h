@@ -380,9 +380,11 @@ OSC_API int osc_linear_weights_free(osc_linear_weights* w);
 
 /* m >= 0 (0: nothing is done). lda, ldr, ldy: row pitches in elements (0 =
  * dense), of any alignment; rows of a that do not start on 16-byte boundaries
- * are first copied to a temporary, allocated and freed in stream order. The
- * scales (8-bit types only) and the bias are FP32 and may be NULL: a_scale [m]
- * (what osc_rmsnorm writes), w_scale n_scale entries (1 or n), bias [n].
+ * are first copied to a temporary, allocated and freed in stream order (its
+ * memory stays with the context for such calls until osc_destroy). The scales
+ * (8-bit types only) and the bias are FP32 and may be NULL: a_scale [m] (what
+ * osc_rmsnorm writes), w_scale n_scale entries (1 or n), bias [n]; the product of
+ * the two scales is taken first, in FP32.
  * out_dtype: OSC_F32, OSC_F16 or OSC_BF16, also the residual's type. act: any
  * osc_act up to OSC_ACT_GELU_TANH. residual may be NULL, and may be y itself
  * (same pointer and pitch); no other argument may overlap y. Calls on different
@@ -426,10 +428,11 @@ OSC_API int osc_attention_f32(osc_ctx* ctx, const float* q, const float* k, cons
  * query, does not matter (NaN included); other v must be finite. A query that is
  * not finite, or sees such a key, gives what the formula does: NaN where a score
  * is NaN or +inf, in its own rows alone. window >= 1 (INT_MAX: none), sinks >=
- * 0, scale > 0. out may not overlap the inputs. Calls with few rows and many
- * keys take a temporary, allocated and freed in stream order; calls on different
- * streams or in different graphs share nothing. Results do not change from run
- * to run. */
+ * 0, scale > 0; B and HK at most 65535. out may not overlap the inputs. Calls with
+ * few rows and many keys take a temporary, allocated and freed in stream order (its
+ * memory stays with the context for such calls until osc_destroy); calls on
+ * different streams or in different graphs share nothing. Results do not change
+ * from run to run. */
 OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const long long* q_strides, const void* k,
                                  const long long* k_strides, const void* v, const long long* v_strides,
                                  const int* lengths, const int* starts, int B, int T, int S, int H, int HK, int D,

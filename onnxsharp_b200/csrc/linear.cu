@@ -841,7 +841,11 @@ int div_up(int a, int b) { return (a + b - 1) / b; }
 // Which kernel, tile and split: the least of a cost in microseconds whose
 // constants were fitted to 8400 measured launches (m 1 to 4096, nine (n, k) from
 // 256 x 256 to 16384 x 1024, bf16 and s8, every tile and split here): its choice
-// is 1.8 % from the best of them in the geometric mean and 20 % at worst.
+// is 1.8 % from the best of them in the geometric mean and 20 % at worst. Neither
+// an FP32 output nor a residual was among them, and the times were bursts: it ranks
+// plans and foretells no times (4096 x 512 x 2048 s8 to f32 with residual 12.1 us for
+// 20.5, since a tile's last step knows nothing of the bytes it moves; 8192 x 4096 x
+// 16384 bf16 437 for 676).
 //   k_linear_split: a k-block of a CTA takes its issue and landing latency or its
 //     share of what an SM takes in; a split adds the meeting of the cluster.
 //   k_linear_tiles: a k-block takes its MMAs and their issue (a pair's tile of the

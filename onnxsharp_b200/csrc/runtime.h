@@ -71,7 +71,9 @@ int scratch(osc_ctx* ctx, size_t bytes, void** out);
 
 // A temporary of this call alone, allocated and freed in the order of the
 // context's stream: nothing that another call, stream or graph could share (a
-// capture records it as the graph's own memory).
+// capture records it as the graph's own memory). What is freed stays with the
+// context's pool for the next call that asks, as the scratch arena stays: about
+// the largest sum of temporaries that were alive at once, until osc_destroy.
 int stream_alloc(osc_ctx* ctx, size_t bytes, void** out);
 int stream_free(osc_ctx* ctx, void* ptr);
 
