@@ -192,18 +192,18 @@ __device__ __forceinline__ void reduce_row(float& ss, uint32_t& peak, float2* pa
   }
 }
 
-// 1 / sqrt(mean + eps) from the row's sum of squares.
-__device__ __forceinline__ float rstd_of(float ss, int cols, float eps) {
-  return rsqrtf(ss / static_cast<float>(cols) + eps);
+// What rstd is the inverse root of, from the row's sum of squares.
+__device__ __forceinline__ float square_of(float ss, int cols, float eps) {
+  return ss / static_cast<float>(cols) + eps;
 }
 
-// Of a row whose finite elements' squares overflow FP32: the sum of (h / 2^80)^2.
+// Where that overflows FP32 from finite elements: ss is the sum of (h / 2^80)^2.
 // 2^31 elements below 2^128 stay below 2^127 so, a sum that overflowed is 2^-32 at
 // least, and eps counts where it is large too. An infinite or NaN element gives 0
 // or NaN, as the formula does.
 constexpr float kDown = 8.27180612553028e-25f;  // 2^-80
 __device__ __forceinline__ float rstd_scaled(float ss, int cols, float eps) {
-  return rsqrtf(ss / static_cast<float>(cols) + eps * kDown * kDown) * kDown;
+  return rsqrtf(square_of(ss, cols, eps * kDown * kDown)) * kDown;
 }
 
 __device__ __forceinline__ bool live_peak(uint32_t peak) {
@@ -319,8 +319,9 @@ __global__ void __launch_bounds__(WARP ? 32 * kRowsPerCta : kMaxThreads) k_rmsno
     }
   uint32_t peak = __float_as_uint(top) & 0x7fffffffu;  // a NaN is above every number
   reduce_row<WARP, CODES>(ss, peak, part, warps);
-  float rstd = rstd_of(ss, p.cols, p.eps);
-  if (!(ss < INFINITY)) {  // the same in all of the row's threads
+  const float square = square_of(ss, p.cols, p.eps);
+  float rstd = rsqrtf(square);
+  if (!(square < INFINITY)) {  // the same in all of the row's threads
     ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -425,8 +426,9 @@ __global__ void __launch_bounds__(kMaxThreads, 1) k_rmsnorm_long(const __grid_co
   });
   uint32_t peak = __float_as_uint(top) & 0x7fffffffu;
   reduce_row<false, true>(ss, peak, part, warps);
-  float rstd = rstd_of(ss, p.cols, p.eps);
-  if (!(ss < INFINITY)) {
+  const float square = square_of(ss, p.cols, p.eps);
+  float rstd = rsqrtf(square);
+  if (!(square < INFINITY)) {
     ss = squares([&](uint32_t e) { return h_at(e) * kDown; });
     uint32_t none = 0u;
     __syncthreads();

@@ -51,3 +51,19 @@ def test_a_large_eps_counts_beside_large_rows(ctx, cols):
     ops.rmsnorm(ctx, x, None, 2.0**125, y)
     ctx.synchronize()
     norm._check(x, None, None, 2.0**125, "", y)
+
+
+@pytest.mark.parametrize("cols", [1, 3, 64, 20000])
+def test_the_largest_eps(ctx, cols):
+    """Squares and eps each fit FP32, their sum does not."""
+    import torch
+
+    from onnxsharp_b200 import ops
+
+    x = torch.full((1, cols), 1.8e19, device="cuda")
+    if cols > 3:
+        x[0, 1:] = 1e17
+    y = torch.empty_like(x)
+    ops.rmsnorm(ctx, x, None, 3e38, y)
+    ctx.synchronize()
+    norm._check(x, None, None, 3e38, "", y)
