@@ -1274,7 +1274,8 @@ OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const l
   if (H % HK != 0 || H / HK > 128) return fail(OSC_EINVAL, "osc_attention_window: %d heads over %d key/value heads", H, HK);
   if (D != 64 && D != 128) return fail(OSC_EUNSUPPORTED, "osc_attention_window: head size %d (64 and 128 are built)", D);
   if (window < 1 || sinks < 0) return fail(OSC_EINVAL, "osc_attention_window: window %d, sinks %d", window, sinks);
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(OSC_EINVAL, "osc_attention_window: scale %g", static_cast<double>(scale));
+  constexpr float kLog2E = 1.4426950408889634f;
+  if (!(scale > 0.0f) || !std::isfinite(scale * kLog2E)) return fail(OSC_EINVAL, "osc_attention_window: scale %g", static_cast<double>(scale));
   if (HK > 65535 || B > 65535) return fail(OSC_EINVAL, "osc_attention_window: %d sequences, %d key/value heads: at most 65535", B, HK);
   if (q_strides == nullptr || k_strides == nullptr || v_strides == nullptr || out_strides == nullptr)
     return fail(OSC_EINVAL, "osc_attention_window: null strides");
@@ -1313,7 +1314,7 @@ OSC_API int osc_attention_window(osc_ctx* ctx, int dtype, const void* q, const l
   p.G = H / HK;
   p.window = window;
   p.sinks = std::min(sinks, kFarPos);
-  p.scale2 = scale * 1.4426950408889634f;
+  p.scale2 = scale * kLog2E;
   if (D == 64) return dtype == OSC_BF16 ? launch<64, true>(ctx, p) : launch<64, false>(ctx, p);
   return dtype == OSC_BF16 ? launch<128, true>(ctx, p) : launch<128, false>(ctx, p);
 }

@@ -73,3 +73,17 @@ def test_window_shapes(calls, q, k):
     with pytest.raises(ValueError, match="too large"):
         runtime.attention_window(CTX, _empty(*q), _empty(*k), _empty(*k), _empty(q[0], dtype=torch.int32), 0.1)
     assert not calls
+
+
+def test_a_scale_too_large_for_powers_of_two():
+    """scale * log2(e) has to be finite: against infinity a score of 0 would be NaN."""
+    import ctypes as C
+
+    from onnxsharp_b200 import _lib
+
+    lib, at = _lib.load(), 1 << 20
+    strides = (C.c_longlong * 3)(512, 512, 64)
+    args = lambda scale: [C.create_string_buffer(1 << 12), _lib.BF16, at, strides, at, strides, at, strides, at, 0, 2, 1,  # noqa: E731
+                          500, 8, 2, 64, 100, 4, scale, at, strides]
+    assert lib.osc_attention_window(*args(3e38)) != 0
+    assert "scale" in lib.osc_last_error().decode()
