@@ -353,6 +353,23 @@ def _vector(name: str, t, ctx: Context, n: int, also: int = 0):
     return t.data_ptr()
 
 
+def _result(ctx: Context, shape, like, dtype):
+    """A result of `like`'s device for a call on the context's stream. torch's allocator hands blocks out in the order
+    of its current stream, whose kernels may still read what was there: on another stream the block is that stream's,
+    and torch's current one, which will read it, is noted with it."""
+    import torch
+
+    if not like.is_cuda:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    here, stream = torch.cuda.current_stream(ctx.device), ctx.get_stream() or 0
+    if stream == here.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, ctx.device)):
+        out = torch.empty(shape, dtype=dtype, device=like.device)
+    out.record_stream(here)
+    return out
+
+
 def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NONE, residual=None, a_scale=None,
            w_scale=None, out=None, out_dtype=None):
     """act((a @ w) * a_scale[:, None] * w_scale + bias) + residual for 16- and 8-bit operands, rounded once.
@@ -373,7 +390,7 @@ def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NON
         if out_dtype is None:
             coded = a.dtype in (torch.int8, torch.float8_e4m3fn)
             out_dtype = residual.dtype if residual is not None else torch.float32 if coded else a.dtype
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        out = _result(ctx, (m, n), a, out_dtype)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"linear: out is {out.dtype}, not {out_dtype}")
     ldy, ldr = _pitch("out", out, ctx, (m, n)), 0
@@ -432,7 +449,7 @@ def attention_window(ctx: Context, q, k, v, lengths, scale: float, window: int |
     if max(shape + keys) > _lib.INT_MAX:
         raise ValueError(f"attention_window: q {tuple(shape)}, k {tuple(keys)}: too large")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = _result(ctx, shape, q, dtype)
     elif out.shape != shape:
         raise ValueError(f"attention_window: out is {tuple(out.shape)}, q {tuple(shape)}")
     strides = []
