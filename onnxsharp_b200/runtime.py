@@ -185,6 +185,23 @@ def conv_out(size: int, k: int, s: int, p0: int, p1: int, d: int) -> int:
     return (size + p0 + p1 - ((k - 1) * d + 1)) // s + 1
 
 
+def _result(ctx: Context, shape, like, dtype):
+    """A result of `like`'s device for a call on the context's stream. torch's allocator hands blocks out in the order
+    of its current stream, whose kernels may still read what was there: on another stream the block is that stream's,
+    and torch's current one, which will read it, is noted with it."""
+    import torch
+
+    if not like.is_cuda:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    here, stream = torch.cuda.current_stream(ctx.device), ctx.get_stream() or 0
+    if stream == here.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, ctx.device)):
+        out = torch.empty(shape, dtype=dtype, device=like.device)
+    out.record_stream(here)
+    return out
+
+
 def conv2d(ctx: Context, x, w: ConvWeights, bias=None, stride=(1, 1), pads=(0, 0, 0, 0), dil=(1, 1), group: int = 1,
            act: int = _lib.ACT_NONE, out=None):
     """y = act(conv(x, W) + bias); x NCHW FP32 on the device; pads = (top, left, bottom, right)."""
@@ -195,7 +212,7 @@ def conv2d(ctx: Context, x, w: ConvWeights, bias=None, stride=(1, 1), pads=(0, 0
     OH = conv_out(H, kh, stride[0], pads[0], pads[2], dil[0])
     OW = conv_out(W, kw, stride[1], pads[1], pads[3], dil[1])
     if out is None:
-        out = torch.empty((N, M, OH, OW), dtype=torch.float32, device=x.device)
+        out = _result(ctx, (N, M, OH, OW), x, torch.float32)
     call("osc_conv2d_bias_act_f32", ctx.handle, ptr(x), N, Cc, H, W, w.handle, stride[0], stride[1], pads[0], pads[1],
          pads[2], pads[3], dil[0], dil[1], group, ptr(bias), int(act), ptr(out), OH, OW)
     return out
@@ -226,7 +243,7 @@ def dqmm(ctx: Context, a, w: DqmmWeights, w_scale, bias=None, out=None, minmax_o
 
     m = a.shape[0]
     if out is None:
-        out = torch.empty((m, w.n), dtype=torch.float32, device=a.device)
+        out = _result(ctx, (m, w.n), a, torch.float32)
     if row0 is not None:
         call("osc_dqmm_shard_f32", ctx.handle, ptr(a), int(m), w.k, int(a.stride(0)), w.handle, ptr(w_scale),
              int(w_scale.numel()), ptr(bias), ptr(out), ptr(minmax_override), int(row0), int(rows_total), ptr(q_out),
@@ -259,7 +276,7 @@ def matmul_batched(ctx: Context, a, b, col_bias=None, out=None):
     ao, ai = ([0, 0] + a_st)[-2:]
     bo, bi = ([0, 0] + b_st)[-2:]
     if out is None:
-        out = torch.empty(batch + [m, n], dtype=torch.float32, device=a.device)
+        out = _result(ctx, batch + [m, n], a, torch.float32)
     call("osc_matmul_batched_f32", ctx.handle, outer, inner, m, k, n, ptr(a), ao, ai, a.stride(-2), a.stride(-1),
          ptr(b), bo, bi, b.stride(-2), b.stride(-1), ptr(col_bias), ptr(out))
     return out
@@ -273,7 +290,7 @@ def gemm_onnx(ctx: Context, a, trans_a: bool, w=None, b=None, trans_b: bool = Fa
     m, k = (a.shape[1], a.shape[0]) if trans_a else (a.shape[0], a.shape[1])
     n = w.n if w is not None else (b.shape[0] if trans_b else b.shape[1])
     if out is None:
-        out = torch.empty((m, n), dtype=torch.float32, device=a.device)
+        out = _result(ctx, (m, n), a, torch.float32)
     call("osc_gemm_onnx_f32", ctx.handle, ptr(a), int(trans_a), int(m), int(k), None if w is None else w.handle,
          ptr(b), int(trans_b), int(n), float(alpha), float(beta), ptr(c), 0 if c is None else int(c.numel()), ptr(out))
     return out
@@ -284,11 +301,11 @@ def dynamic_quantize_linear(ctx: Context, x, y=None, y_scale=None, y_zero_point=
     import torch
 
     if y is None:
-        y = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+        y = _result(ctx, x.shape, x, torch.uint8)
     if y_scale is None:
-        y_scale = torch.empty(1, dtype=torch.float32, device=x.device)
+        y_scale = _result(ctx, 1, x, torch.float32)
     if y_zero_point is None:
-        y_zero_point = torch.empty(1, dtype=torch.uint8, device=x.device)
+        y_zero_point = _result(ctx, 1, x, torch.uint8)
     call("osc_dynamic_quantize_linear_f32", ctx.handle, ptr(x), int(x.numel()), ptr(y), ptr(y_scale),
          ptr(y_zero_point))
     return y, y_scale, y_zero_point
@@ -300,7 +317,7 @@ def matmul_integer(ctx: Context, a, a_zero_point: int, w: "DqmmWeights", out=Non
 
     m = a.shape[0]
     if out is None:
-        out = torch.empty((m, w.n), dtype=torch.int32, device=a.device)
+        out = _result(ctx, (m, w.n), a, torch.int32)
     signed = 1 if a.dtype == torch.int8 else 0
     call("osc_matmul_integer_i8", ctx.handle, ptr(a), signed, int(m), w.k, int(a.stride(0)), int(a_zero_point),
          w.handle, ptr(out))
@@ -353,23 +370,6 @@ def _vector(name: str, t, ctx: Context, n: int, also: int = 0):
     return t.data_ptr()
 
 
-def _result(ctx: Context, shape, like, dtype):
-    """A result of `like`'s device for a call on the context's stream. torch's allocator hands blocks out in the order
-    of its current stream, whose kernels may still read what was there: on another stream the block is that stream's,
-    and torch's current one, which will read it, is noted with it."""
-    import torch
-
-    if not like.is_cuda:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    here, stream = torch.cuda.current_stream(ctx.device), ctx.get_stream() or 0
-    if stream == here.cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, ctx.device)):
-        out = torch.empty(shape, dtype=dtype, device=like.device)
-    out.record_stream(here)
-    return out
-
-
 def linear(ctx: Context, a, w: LinearWeights, bias=None, act: int = _lib.ACT_NONE, residual=None, a_scale=None,
            w_scale=None, out=None, out_dtype=None):
     """act((a @ w) * a_scale[:, None] * w_scale + bias) + residual for 16- and 8-bit operands, rounded once.
@@ -409,7 +409,7 @@ def minmax(ctx: Context, x, out=None):
     import torch
 
     if out is None:
-        out = torch.empty(2, dtype=torch.float32, device=x.device)
+        out = _result(ctx, 2, x, torch.float32)
     call("osc_minmax_f32", ctx.handle, ptr(x), int(x.numel()), ptr(out))
     return out
 
@@ -422,7 +422,7 @@ def attention(ctx: Context, q, k, v, heads: int, scale: float, mask=None, out_he
     D = width // heads
     if out is None:
         shape = (B, heads, T, D) if out_head_space else (B, T, width)
-        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+        out = _result(ctx, shape, q, torch.float32)
     mask_rows = 0 if mask is None else int(mask.shape[2])
     call("osc_attention_f32", ctx.handle, ptr(q), ptr(k), ptr(v), ptr(mask), mask_rows, int(B), int(T), int(heads),
          int(D), float(scale), 1 if out_head_space else 0, ptr(out))
@@ -487,8 +487,8 @@ def gemm_split_a(ctx: Context, a, k: int, out=None):
 
     m, kp = int(a.shape[0]), (int(k) + 3) // 4 * 4
     if out is None:
-        out = (torch.empty((m, kp), dtype=torch.float32, device=a.device),
-               torch.empty((m, kp), dtype=torch.float32, device=a.device))
+        out = (_result(ctx, (m, kp), a, torch.float32),
+               _result(ctx, (m, kp), a, torch.float32))
     call("osc_gemm_split_a_f32", ctx.handle, ptr(a), m, int(k), int(a.stride(0)), kp, ptr(out[0]), ptr(out[1]))
     return out
 
@@ -501,7 +501,7 @@ def gemm_bias_presplit(ctx: Context, split, w: GemmWeights, bias=None, act: int 
     hi, lo = split
     m, kp = int(hi.shape[0]), int(hi.shape[1])
     if out is None:
-        out = torch.empty((m, w.n), dtype=torch.float32, device=hi.device)
+        out = _result(ctx, (m, w.n), hi, torch.float32)
     call("osc_gemm_bias_presplit_f32", ctx.handle, ptr(hi), ptr(lo), m, kp, w.handle, ptr(bias), int(act), ptr(out),
          int(ldc or out.stride(0)))
     return out
@@ -514,7 +514,7 @@ def gemm_bias(ctx: Context, a, w: GemmWeights, bias=None, act: int = _lib.ACT_NO
 
     m, k = a.shape[0], w.k
     if out is None:
-        out = torch.empty((m, w.n), dtype=torch.float32, device=a.device)
+        out = _result(ctx, (m, w.n), a, torch.float32)
     call("osc_gemm_bias_f32", ctx.handle, ptr(a), int(m), int(k), int(lda or a.stride(0)), w.handle, ptr(bias),
          int(act), ptr(out), int(ldc or out.stride(0)))
     return out
