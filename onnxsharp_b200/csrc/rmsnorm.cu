@@ -20,7 +20,7 @@
 // One pass over the data: a row stays in the registers of its warp (short
 // rows) or CTA, 16 elements a thread (8 or 32 of a 16-bit type: 61.6 and 107 us
 // in place of 53.5 for 8192 rows of 4096 bf16 with a residual; CTAs that walk
-// rows, loading the next ahead, 84). Launch latency bounds a few rows: 1.9 us for
+// rows, loading the next ahead, 84). Launch latency bounds a few rows: 1.7 us for
 // one of 4096. Of 8192 rows of 4096, f32 reaches 6.3 TB/s (42.5 us); bf16 with a
 // residual 5.1 (52.5 us), with e4m3 codes 3.7 (64 us): a thread's 16 elements
 // are then too little beside a row's own steps (its sum over warps, its scale),
