@@ -186,9 +186,11 @@ def conv_out(size: int, k: int, s: int, p0: int, p1: int, d: int) -> int:
 
 
 def _result(ctx: Context, shape, like, dtype):
-    """A result of `like`'s device for a call on the context's stream. torch's allocator hands blocks out in the order
-    of its current stream, whose kernels may still read what was there: on another stream the block is that stream's,
-    and torch's current one, which will read it, is noted with it."""
+    """A result on `like`'s device for a call on the context's stream. torch's allocator hands blocks out in the order
+    of its current stream: where that is another one, its kernels may still read what was there, and what is dropped
+    early goes to its next kernels. So the block is the context's stream's, which also waits for what torch's current
+    stream has queued (earlier results may be read there). record_stream would leave events that the allocator asks
+    for at its next call, which a capture does not allow."""
     import torch
 
     if not like.is_cuda:
@@ -196,10 +198,12 @@ def _result(ctx: Context, shape, like, dtype):
     here, stream = torch.cuda.current_stream(ctx.device), ctx.get_stream() or 0
     if stream == here.cuda_stream:
         return torch.empty(shape, dtype=dtype, device=like.device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, ctx.device)):
-        out = torch.empty(shape, dtype=dtype, device=like.device)
-    out.record_stream(here)
-    return out
+    apart = torch.cuda.is_current_stream_capturing()
+    own = torch.cuda.ExternalStream(stream, ctx.device)
+    with torch.cuda.stream(own):
+        if not apart and not torch.cuda.is_current_stream_capturing():  # (a wait would tie the two captures together)
+            own.wait_stream(here)
+        return torch.empty(shape, dtype=dtype, device=like.device)
 
 
 def conv2d(ctx: Context, x, w: ConvWeights, bias=None, stride=(1, 1), pads=(0, 0, 0, 0), dil=(1, 1), group: int = 1,
